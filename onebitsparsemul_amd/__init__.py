@@ -10,6 +10,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
+from .decoder import QuantizedCache, block_norm, cache_append, cache_attention, rotary, rotary_table
 from ._semi_structured_conversions import (
     mask_creator,
     sparse_semi_structured_from_dense_cutlass,
@@ -20,6 +21,7 @@ __all__ = [
     "cuda_binary_mul", "cuda_binary_mul_", "binary_quant", "pack_binary", "unpack_binary", "dequant_desparse_tile",
     "py_binary_gemm", "BinaryLinear_2_4", "PreparedWeight", "mask_creator", "sparse_semi_structured_from_dense_cutlass",
     "sparse_semi_structured_to_dense_cutlass", "set_weight_cache", "clear_weight_cache",
+    "QuantizedCache", "block_norm", "cache_append", "cache_attention", "rotary", "rotary_table",
 ]
 
 

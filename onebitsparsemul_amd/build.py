@@ -27,19 +27,26 @@ def _run(cmd):
     subprocess.run(cmd, check=True)
 
 
-def build_library():
-    # one compiler per source, side by side
-    objs, compilers = [], []
-    for src in ("onebit_gemm.hip", "onebit_gemm_tokens.hip", "onebit_skinny.hip", "onebit_skinny_tokens.hip",
-                "onebit_wide.hip", "onebit_wide_tokens.hip", "onebit_format.hip", "onebit_capi.hip", "onebit_diag.hip"):
-        obj = os.path.join(CSRC, src.replace(".hip", ".o"))
-        cmd = [HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
+def _run_side_by_side(cmds):
+    compilers = []
+    for cmd in cmds:
         print("+", " ".join(cmd), flush=True)
-        compilers.append((cmd, subprocess.Popen(cmd)))
-        objs.append(obj)
-    failed = [cmd for cmd, compiler in compilers if compiler.wait() != 0]
+        compilers.append(subprocess.Popen(cmd))
+    failed = [cmd for cmd, compiler in zip(cmds, compilers) if compiler.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
+
+
+def build_library():
+    # one compiler per source, side by side
+    objs, cmds = [], []
+    for src in ("onebit_gemm.hip", "onebit_gemm_tokens.hip", "onebit_skinny.hip", "onebit_skinny_tokens.hip",
+                "onebit_wide.hip", "onebit_wide_tokens.hip", "onebit_format.hip", "onebit_capi.hip", "onebit_diag.hip",
+                "onebit_cache.hip", "onebit_attention.hip", "onebit_norm.hip", "onebit_decoder_capi.hip"):
+        obj = os.path.join(CSRC, src.replace(".hip", ".o"))
+        cmds.append([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
+        objs.append(obj)
+    _run_side_by_side(cmds)
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
     if os.path.exists(STATIC_LIB):
         os.remove(STATIC_LIB)
@@ -63,10 +70,12 @@ def build_binding():
         inc += ["-isystem", p]
     inc += ["-isystem", sysconfig.get_paths()["include"], "-isystem", "/opt/rocm/include", "-I", INCLUDE]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *inc, os.path.join(CSRC, "torch_binding.cpp"), "-o", out,
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    objs = [os.path.join(CSRC, name + ".o") for name in ("torch_binding", "torch_decoder")]
+    _run_side_by_side([["g++", *flags, *inc, "-c", obj[:-2] + ".cpp", "-o", obj] for obj in objs])
+    cmd = ["g++", "-shared", *objs, "-o", out,
            "-L", PKG, "-lonebitmul", "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
            "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     _run(cmd)

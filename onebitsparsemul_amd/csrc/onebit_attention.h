@@ -1,0 +1,93 @@
+// Attention over the 8-bit cache: what its kernels share (internal to libonebitmul).
+//
+// Mathematics: out = sum_j p_j v_j / sum_j p_j with p_j = exp2(t_j - m), t_j = log2(e) scale k_scale q . k_code_j and m the largest t so far, in
+// one pass over the keys; where m grows, what is summed so far is multiplied by exp2(m_old - m). Codes are exact in fp16, and so
+// is q (bf16 rows as q 2^-e), so that the products of the matrix instructions are exact and their sums fp32. p_j takes its key's
+// v_scale, by the power of two that the largest scale seen so far gives, and 2^15 on top: then fp16 keeps eleven bits of each p_j down to 2^-29.
+//
+// Scores are computed as K Q^T: a lane then holds scores of one row of q (matrix column) and of the keys that the next product,
+// V^T P^T, wants from it as its own operand: p goes from one matrix instruction to the next without leaving its register.
+#pragma once
+#include "onebit_decoder_device.h"
+#include "onebit_decoder_launch.h"
+
+namespace onebit {
+
+constexpr float kLog2E = 1.44269504088896340736f;
+
+// Four codes of a word as fp16, exact. e4m3 by the conversion instruction; int8: the byte plus 128 as the low byte of 1024 + n, minus 1152.
+template <int CODE>
+__device__ inline void codes_to_f16(uint32_t word, h2_t& low, h2_t& high) {
+  if constexpr (CODE == ONEBIT_CODE_E4M3) {
+    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false));
+    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true));
+  } else {
+    const uint32_t shifted = word ^ 0x80808080u;
+    const h2_t offset = {(_Float16)1152.f, (_Float16)1152.f};
+    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04010400u)) - offset;
+    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04030402u)) - offset;
+  }
+}
+template <int CODE>
+__device__ inline h8_t codes_to_f16(uint32_t first, uint32_t second) {
+  h2_t a, b, c, d;
+  codes_to_f16<CODE>(first, a, b);
+  codes_to_f16<CODE>(second, c, d);
+  return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Words of four tokens' codes at four dims -> words of four dims' codes of the four tokens
+__device__ inline void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&out)[4]) {
+  const uint32_t ab_low = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_high = __builtin_amdgcn_perm(b, a, 0x07030602u);
+  const uint32_t cd_low = __builtin_amdgcn_perm(d, c, 0x05010400u), cd_high = __builtin_amdgcn_perm(d, c, 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(cd_low, ab_low, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(cd_low, ab_low, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(cd_high, ab_high, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(cd_high, ab_high, 0x07060302u);
+}
+
+// The larger of each lane's value and those of the lanes 16, 32 and 48 further on
+__device__ inline float max_over_16(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float sum_over_16(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+// Exponent of a magnitude, at least `least` (a NaN and infinities: 128)
+__device__ inline int exponent_of(uint32_t magnitude_bits, int least) { return max((int)(magnitude_bits >> 23) - 127, least); }
+
+__device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+__device__ inline float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
+// 16 values of a row of q as they lie in memory, and as fp16 times `factor` (a power of two; not used on fp16)
+struct RawQ {
+  u4_t low, high;
+};
+__device__ inline uint32_t magnitude_bf16(const RawQ& q) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    most = max(max(most, max((q.low[i] << 16) & 0x7fff0000u, q.low[i] & 0x7fff0000u)),
+               max((q.high[i] << 16) & 0x7fff0000u, q.high[i] & 0x7fff0000u));
+  return most;
+}
+__device__ inline h8_t q_to_f16(u4_t raw, int dtype, float factor) {
+  if (dtype == ONEBIT_DTYPE_F16) return __builtin_bit_cast(h8_t, raw);
+  h8_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[2 * i] = (_Float16)(__uint_as_float(raw[i] << 16) * factor);
+    r[2 * i + 1] = (_Float16)(__uint_as_float(raw[i] & 0xffff0000u) * factor);
+  }
+  return r;
+}
+
+}  // namespace onebit

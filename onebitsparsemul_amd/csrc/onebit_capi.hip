@@ -922,6 +922,16 @@ int linear_prepared_impl(const void* prepared, const void* x, const void* bias, 
 
 }  // namespace
 
+namespace onebit {
+
+int report(int code, const char* message) {
+  g_last_error = message;
+  return code;
+}
+int device_compute_units() { return current_compute_units(); }
+
+}  // namespace onebit
+
 extern "C" {
 
 const char* onebit_sparse_last_error(void) { return g_last_error.c_str(); }

@@ -139,4 +139,9 @@ hipError_t launch_wide_tokens(SkinnyArgs args, int rows_per_group, hipStream_t s
 hipError_t launch_wide(SkinnyArgs args, int rows_per_group, hipStream_t stream);
 hipError_t launch_wide_tokens_group(SkinnyGroupArgs group, int rows_per_group, hipStream_t stream);
 
+// onebit_capi.hip, for the other files with entry points: keeps the message of a failure for onebit_sparse_last_error ("" and ONEBIT_OK at the
+// start of a call); the current device's compute units.
+int report(int code, const char* message);
+int device_compute_units();
+
 }  // namespace onebit

@@ -13,12 +13,7 @@
 // The package's own calls (layer forward, grouped forward, prepared product, one-call product, packing) have their host
 // side here too: a decode-sized product takes 4 to 7 us on the GPU, and checking the operands, allocating the result and
 // making the library call from Python took 9 to 27 us.
-#include <torch/extension.h>
-// PyTorch on ROCm presents its devices as type "cuda"; these are the guard and stream accessors for that.
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-
-#include "onebit_sparse_tensor.h"
+#include "torch_binding.h"
 
 namespace {
 
@@ -57,34 +52,11 @@ void onebit_mul(const torch::Tensor& A, const torch::Tensor& B, const torch::Ten
   TORCH_CHECK(rc == ONEBIT_OK, "onebit_sparse_matmul_ex failed: ", onebit_sparse_last_error());
 }
 
-using OptionalTensor = std::optional<torch::Tensor>;
-
-int dtype_code(c10::ScalarType type) {
-  switch (type) {
-    case torch::kFloat32: return ONEBIT_DTYPE_F32;
-    case torch::kFloat16: return ONEBIT_DTYPE_F16;
-    case torch::kBFloat16: return ONEBIT_DTYPE_BF16;
-    default: return -1;
-  }
-}
-
-void* current_stream(const c10::Device& device) {
-  return static_cast<void*>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream());
-}
-
-void check_status(int rc) {
-  TORCH_CHECK(rc == ONEBIT_OK, "libonebitmul: ", onebit_sparse_last_error(), " (status ", rc, ")");
-}
-
 // every operand on one GPU, contiguous
 void check_placement(const torch::Tensor& t, const c10::Device& device) {
   TORCH_CHECK_VALUE(t.is_cuda(), "all operands must live on the GPU");
   TORCH_CHECK_VALUE(t.is_contiguous(), "all operands must be contiguous");
   TORCH_CHECK_VALUE(t.device() == device, "all operands must be on the same device");
-}
-
-torch::Tensor empty_result(at::IntArrayRef sizes, c10::ScalarType type, const c10::Device& device) {
-  return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
 }
 
 size_t prepared_bytes(int64_t m, int64_t k) { return ((size_t)m + 31) / 32 * (((size_t)k + 255) / 256) * 1536; }
@@ -338,4 +310,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("binary_mul", &binary_mul, NoGil());
   m.def("prepare", &prepare, NoGil());
   m.def("pack_weight", &pack_weight, NoGil());
+  bind_decoder(m);
 }
