@@ -67,16 +67,11 @@ __device__ inline int exponent_of(uint32_t magnitude_bits, int least) { return m
 __device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 __device__ inline float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 
-// 16 values of a row of q as they lie in memory, and as fp16 times `factor` (a power of two; not used on fp16)
-struct RawQ {
-  u4_t low, high;
-};
-__device__ inline uint32_t magnitude_bf16(const RawQ& q) {
+// Eight values of a row of q: the largest magnitude, and as fp16 times `factor` (a power of two; not used on fp16)
+__device__ inline uint32_t magnitude_bf16(u4_t q) {
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    most = max(max(most, max((q.low[i] << 16) & 0x7fff0000u, q.low[i] & 0x7fff0000u)),
-               max((q.high[i] << 16) & 0x7fff0000u, q.high[i] & 0x7fff0000u));
+  for (int i = 0; i < 4; ++i) most = max(most, max((q[i] << 16) & 0x7fff0000u, q[i] & 0x7fff0000u));
   return most;
 }
 __device__ inline h8_t q_to_f16(u4_t raw, int dtype, float factor) {
@@ -88,6 +83,26 @@ __device__ inline h8_t q_to_f16(u4_t raw, int dtype, float factor) {
     r[2 * i + 1] = (_Float16)(__uint_as_float(raw[i] & 0xffff0000u) * factor);
   }
   return r;
+}
+
+// The pages of a sequence from entry `first` of its table on, one to a lane
+struct Window {
+  int first;
+  int page;  // -1: none
+  float k_scale, v_scale;
+};
+// Fills the window with the entries from `entry` to `last`, and returns the exponent of the largest finite v_scale among them (-100 to 110).
+__device__ inline int fill_window(Window& window, int entry, int last, const int* table, const onebit_cache& cache, int head) {
+  const int own = entry + (int)(threadIdx.x % 64);
+  window = {entry, own <= last ? table[own] : -1, 0.f, 0.f};
+  if (window.page >= cache.pages) window.page = -1;
+  if (window.page >= 0) {
+    const long long at = (long long)window.page * cache.kv_heads + head;
+    window.k_scale = cache.k_scale[at];
+    window.v_scale = cache.v_scale[at];
+  }
+  const uint32_t bits = magnitude(window.v_scale);
+  return min(exponent_of(wave_max(bits < 0x7f800000u ? bits : 0), -100), 110);
 }
 
 }  // namespace onebit

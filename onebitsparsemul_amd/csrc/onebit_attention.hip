@@ -21,13 +21,6 @@ struct Chunk {
   int valid[2];  // keys of the tile that are there
 };
 
-// The pages from entry `first` on, one to a lane
-struct Window {
-  int first;
-  int page;  // -1: none
-  float k_scale, v_scale;
-};
-
 template <int D, int CODE, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(AttentionArgs args, int row_tiles) {
   constexpr int kStride = D + 4;  // floats of a row of sums in LDS
@@ -55,24 +48,24 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(AttentionArgs args
     h8_t q[D / 64][2];
     float row_factor = args.scale * kLog2E;
     {
-      RawQ raw[D / 64] = {};
+      u4_t raw[D / 64][2] = {};
       if (row < rows) {
         const uint16_t* const at = (const uint16_t*)args.q.data + (seq.start + token) * args.q.token_stride + query_head * args.q.head_stride + 16 * g;
 #pragma unroll
-        for (int u = 0; u < D / 64; ++u) raw[u] = {*(const u4_t*)(at + 64 * u), *(const u4_t*)(at + 64 * u + 8)};
+        for (int u = 0; u < D / 64; ++u) raw[u][0] = *(const u4_t*)(at + 64 * u), raw[u][1] = *(const u4_t*)(at + 64 * u + 8);
       }
       float factor = 1.f;
       if (args.dtype == ONEBIT_DTYPE_BF16) {  // rows as q 2^(8 - e), e the exponent of their largest value
         uint32_t most = 0;
 #pragma unroll
-        for (int u = 0; u < D / 64; ++u) most = max(most, magnitude_bf16(raw[u]));
+        for (int u = 0; u < D / 64; ++u) most = max(most, max(magnitude_bf16(raw[u][0]), magnitude_bf16(raw[u][1])));
         most = __float_as_uint(max_over_16(__uint_as_float(min(most, 0x7f800000u))));
         const int e = exponent_of(most, -100);
         factor = power_of_two(8 - e);
         row_factor *= power_of_two(e - 8);
       }
 #pragma unroll
-      for (int u = 0; u < D / 64; ++u) q[u][0] = q_to_f16(raw[u].low, args.dtype, factor), q[u][1] = q_to_f16(raw[u].high, args.dtype, factor);
+      for (int u = 0; u < D / 64; ++u) q[u][0] = q_to_f16(raw[u][0], args.dtype, factor), q[u][1] = q_to_f16(raw[u][1], args.dtype, factor);
     }
 
     f4_t sums[D / 16] = {};
@@ -81,18 +74,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(AttentionArgs args
 
     Window window = {0, -1, 0.f, 0.f};
     auto refill = [&](int entry) {
-      window.first = entry;
-      const int own = entry + lane;
-      window.page = own <= (end - 1) >> block_bits ? table[own] : -1;
-      if (window.page >= cache.pages) window.page = -1;
-      window.k_scale = window.v_scale = 0.f;
-      if (window.page >= 0) {
-        const long long at = (long long)window.page * cache.kv_heads + head;
-        window.k_scale = cache.k_scale[at];
-        window.v_scale = cache.v_scale[at];
-      }
-      const uint32_t bits = magnitude(window.v_scale);
-      const int e = min(exponent_of(wave_max(bits < 0x7f800000u ? bits : 0), -100), 110);
+      const int e = fill_window(window, entry, (end - 1) >> block_bits, table, cache, head);
       if (e > v_exponent) {
         const float down = v_exponent == -100 ? 0.f : power_of_two(max(v_exponent - e, -126));
 #pragma unroll
@@ -283,28 +265,36 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttentionArgs args) {
 }
 
 template <int D, int CODE>
-hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
+hipError_t launch_few_rows(const AttentionArgs& args, hipStream_t stream) {
   constexpr int kWaves = 8;
   const onebit_sequences& q = args.sequences;
   const int row_tiles = (int)(((long long)q.max_new * args.group + kRows - 1) / kRows);
   const dim3 grid(row_tiles * args.splits, args.cache.kv_heads, q.count);
-  hipError_t status = launch_kernel(few_rows_kernel<D, CODE, kWaves>, grid, dim3(kWaves * 64), 0, stream, args, row_tiles);
+  return launch_kernel(few_rows_kernel<D, CODE, kWaves>, grid, dim3(kWaves * 64), 0, stream, args, row_tiles);
+}
+template <int D>
+hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
+  const bool int8 = args.cache.code == ONEBIT_CODE_INT8;
+  const hipError_t status = args.rows > kRows ? launch_many_rows(args, stream)
+                            : int8            ? launch_few_rows<D, ONEBIT_CODE_INT8>(args, stream)
+                                              : launch_few_rows<D, ONEBIT_CODE_E4M3>(args, stream);
   if (status != hipSuccess || args.splits == 1) return status;
-  const dim3 rows((unsigned)((long long)q.tokens * args.heads));
+  const dim3 rows((unsigned)((long long)args.sequences.tokens * args.heads));
   if (args.splits <= 4) return launch_kernel(join_kernel<D, 64>, rows, dim3(64), 0, stream, args);
   return launch_kernel(join_kernel<D, 256>, rows, dim3(256), 0, stream, args);
 }
 
 }  // namespace
 
-// Keys are split over workgroups where a call has fewer workgroups than the device holds at once.
+// Rows of q to a workgroup, and how its keys are split over workgroups where a call has fewer of them than the device holds at once.
 void plan_attention(AttentionArgs& args, int compute_units) {
   const onebit_sequences& q = args.sequences;
-  const long long row_tiles = ((long long)q.max_new * args.group + kRows - 1) / kRows;
-  const long long units = row_tiles * args.cache.kv_heads * q.count, room = (long long)q.width * args.cache.block;
+  const long long rows = (long long)q.max_new * args.group, room = (long long)q.width * args.cache.block;
   const long long most = std::max(1ll, q.max_length > 0 ? std::min(room, (long long)q.max_length) : room);
-  long long splits = std::max(1ll, 4ll * compute_units / units);
-  long long keys = std::max(256ll, ((most + splits - 1) / splits + 255) / 256 * 256);
+  args.rows = rows <= 32 ? kRows : 128;
+  const long long units = (rows + args.rows - 1) / args.rows * args.cache.kv_heads * q.count;
+  const long long splits = std::max(1ll, (args.rows == kRows ? 4ll : 1ll) * compute_units / units);
+  const long long keys = std::max(args.rows == kRows ? 256ll : 512ll, ((most + splits - 1) / splits + 255) / 256 * 256);
   args.splits = (int)((most + keys - 1) / keys);
   args.keys_per_split = (int)keys;
 }
@@ -314,9 +304,7 @@ size_t attention_workspace(const AttentionArgs& args) {
 }
 
 hipError_t launch_attention(const AttentionArgs& args, hipStream_t stream) {
-  const bool int8 = args.cache.code == ONEBIT_CODE_INT8;
-  if (args.cache.head_dim == 64) return int8 ? launch_as<64, ONEBIT_CODE_INT8>(args, stream) : launch_as<64, ONEBIT_CODE_E4M3>(args, stream);
-  return int8 ? launch_as<128, ONEBIT_CODE_INT8>(args, stream) : launch_as<128, ONEBIT_CODE_E4M3>(args, stream);
+  return args.cache.head_dim == 64 ? launch_as<64>(args, stream) : launch_as<128>(args, stream);
 }
 
 }  // namespace onebit

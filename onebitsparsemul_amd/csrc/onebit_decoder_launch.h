@@ -34,15 +34,17 @@ struct AttentionArgs {
   int heads, group;  // group: heads of a key/value head
   int dtype;
   float scale;
+  int rows;  // of q to a workgroup: 16 (few_rows_kernel), 128 or 256 (many_rows_kernel)
   // keys split over workgroups: split i takes keys [i * keys_per_split, ...) of its sequence; workspace: splits x tokens x heads rows of
   // head_dim fp32 sums, then as many pairs (running maximum, sum); splits == 1: none
   int splits, keys_per_split;
   float* workspace;
 };
-// Fills the split of `args`.
+// Fills rows and the split of `args`.
 void plan_attention(AttentionArgs& args, int compute_units);
 size_t attention_workspace(const AttentionArgs& args);
 hipError_t launch_attention(const AttentionArgs& args, hipStream_t stream);
+hipError_t launch_many_rows(const AttentionArgs& args, hipStream_t stream);  // without the pass that joins splits
 
 hipError_t launch_norm(const onebit_norm& args, hipStream_t stream);
 
