@@ -1,0 +1,314 @@
+// Attention over the 8-bit cache (onebit_decoder.h) for many rows of q to a key/value head: prompts.
+//
+// A workgroup takes 128 rows (tokens x heads of the key/value head), 32 to a wavefront, and walks over the keys in tiles of 64. Each tile's
+// codes are read once, turned into fp16 by the wavefronts together, and lie in LDS twice (one tile in use, one being written): keys by rows of
+// dims, values by rows of keys, so that both matrix products (32x32x16, fp16) read their left operand with one 16-byte load a lane.
+#include "onebit_attention.h"
+
+#include <type_traits>
+
+namespace onebit {
+namespace {
+
+typedef float f16x_t __attribute__((ext_vector_type(16)));
+constexpr int kTile = 64;  // keys
+constexpr int kWaves = 4, kRows = kWaves * 32;
+
+// Where the 16-byte piece `piece` of a row lies: moved within its row, so that neighbouring rows' pieces fall on different banks for reads (32
+// rows, one piece) and writes alike.
+template <int PIECES>
+__device__ inline int place(int row, int piece) {
+  if (PIECES == 16) return row * 16 + (piece ^ (row & 15));
+  return row * 8 + (piece ^ (((row >> 1) + (row >> 3)) & 7));
+}
+
+template <int D, int CODE, bool ONE_PAGE>
+__global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs args, int row_tiles) {
+  constexpr int kOwn = kTile / kWaves;  // keys a wavefront brings in
+  constexpr int kKeyBytes = kOwn * D / 64, kValueBytes = D * kOwn / 256;
+  typedef uint32_t key_words __attribute__((ext_vector_type(kKeyBytes / 4)));
+  typedef uint32_t value_words __attribute__((ext_vector_type(kValueBytes / 4)));
+  __shared__ __align__(16) h8_t keys[2][kTile * D / 8];
+  __shared__ __align__(16) h8_t values[2][kTile * D / 8];
+  const onebit_cache& cache = args.cache;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 32, h = lane / 32;
+  const int head = blockIdx.x % cache.kv_heads, split = blockIdx.x / cache.kv_heads % args.splits, s = blockIdx.z;
+  const Sequence seq = read_sequence(args.sequences, s, cache.block);
+  const int rows = seq.fresh * args.group, block_bits = __builtin_ctz(cache.block);
+  const int* const table = args.sequences.page_table + (long long)s * args.sequences.width;
+  const long long all_rows = (long long)args.sequences.tokens * args.heads;
+  float* const pairs = args.workspace + (long long)args.splits * all_rows * D;
+
+  // the last rows see the most keys: first
+  for (int tile = row_tiles - 1 - (int)blockIdx.y + (rows > row_tiles * kRows ? ((rows + kRows - 1) / kRows - 1) / row_tiles * row_tiles : 0); tile >= 0; tile -= row_tiles) {
+    if (tile * kRows >= rows) continue;
+    const int last_token = (min(tile * kRows + kRows, rows) - 1) / args.group;
+    const int total = max(seq.length - seq.fresh + last_token + 1, 0);
+    const int low = split * args.keys_per_split, high = split == args.splits - 1 ? total : min(total, low + args.keys_per_split);
+    const int tiles = max(high - low + kTile - 1, 0) / kTile;
+    const int wave_row = tile * kRows + wave * 32;
+    // keys that all rows of the wavefront see, and that one of them sees
+    const int all_see = wave_row + 32 <= rows ? max(seq.length - seq.fresh + wave_row / args.group + 1, 0) : 0;
+    const int one_sees = wave_row < rows ? max(seq.length - seq.fresh + (min(wave_row + 32, rows) - 1) / args.group + 1, 0) : 0;
+    // the row of this lane's column
+    const int row = wave_row + r;
+    const long long token = seq.start + row / args.group;
+    const int query_head = head * args.group + row % args.group;
+    const int seen = row < rows ? max(seq.length - seq.fresh + row / args.group + 1, 0) : 0;
+
+    h8_t q[D / 16];
+    float row_factor = args.scale * kLog2E;
+    {
+      u4_t raw[D / 16] = {};
+      if (row < rows) {
+        const uint16_t* const at = (const uint16_t*)args.q.data + token * args.q.token_stride + query_head * args.q.head_stride + 8 * h;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) raw[c] = *(const u4_t*)(at + 16 * c);
+      }
+      float factor = 1.f;
+      if (args.dtype == ONEBIT_DTYPE_BF16) {  // rows as q 2^(8 - e), e the exponent of their largest value
+        uint32_t most = 0;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) most = max(most, magnitude_bf16(raw[c]));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+        const int e = exponent_of(most, -100);
+        factor = power_of_two(8 - e);
+        row_factor *= power_of_two(e - 8);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) q[c] = q_to_f16(raw[c], args.dtype, factor);
+    }
+
+    f16x_t sums[D / 32] = {};
+    float most = -INFINITY, total_p = 0.f;
+    int v_exponent = -100;  // p takes v_scale 2^(8 - v_exponent)
+
+    Window window = {0, -1, 0.f, 0.f};
+    float v_log = 0.f, v_inverse = 0.f;  // of the window's v_scale 2^(8 - v_exponent)
+    uint64_t careful = 0;                // entries without a page, or with a scale that an exponent does not take on well
+    auto refill = [&](int entry) {
+      const int e = fill_window(window, entry, (high - 1) >> block_bits, table, cache, head);
+      if (e > v_exponent) {
+        const float down = v_exponent == -100 ? 0.f : power_of_two(max(v_exponent - e, -126));
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) sums[j] *= down;
+        v_exponent = e;
+      }
+      window.v_scale *= power_of_two(8 - v_exponent);
+      v_log = __builtin_amdgcn_logf(window.v_scale);
+      v_inverse = 1.f / window.v_scale;
+      careful = __ballot(!(window.page >= 0 && window.v_scale >= 0x1p-10f && window.v_scale <= 0x1p9f));
+    };
+
+    // the wavefront's share of a tile: kOwn keys, in one page
+    key_words raw_k;
+    value_words raw_v[4];
+    auto load = [&](int key) {
+      const int own = key + wave * kOwn, entry = min((own >> block_bits) - window.first, 63);
+      const int page = __builtin_amdgcn_readlane(window.page, entry);
+      const int valid = page < 0 ? 0 : min(max(high - own, 0), kOwn);
+      const long long at = valid == 0 ? 0 : (((long long)page * cache.kv_heads + head) * cache.block + (own & (cache.block - 1))) * D;
+      raw_k = *(const key_words*)((const uint8_t*)cache.k + at + lane * kKeyBytes);
+      constexpr int kLanes = D / kValueBytes;  // of a token
+      const int first = lane / kLanes * 4;
+      const uint8_t* const v = (const uint8_t*)cache.v + at + first * D + lane % kLanes * kValueBytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw_v[i] = *(const value_words*)(v + i * D);
+      if (valid < kOwn) {  // codes of keys that are not there may be NaN, which a p of 0 would not hide
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (first + i >= valid) raw_v[i] = 0;
+      }
+    };
+    auto put = [&](auto buffer) {
+      constexpr int to = decltype(buffer)::value;
+      constexpr int kKeyLanes = D / kKeyBytes, kLanes = D / kValueBytes;
+      const int key = wave * kOwn + lane / kKeyLanes, piece = lane % kKeyLanes * (kKeyBytes / 8);
+#pragma unroll
+      for (int i = 0; i < kKeyBytes / 8; ++i) keys[to][place<D / 8>(key, piece + i)] = codes_to_f16<CODE>(raw_k[2 * i], raw_k[2 * i + 1]);
+      const int group = (wave * kOwn + lane / kLanes * 4) / 4, dim = lane % kLanes * kValueBytes;
+      const int piece_v = (group >> 2) * 2 + (group & 1), half = group >> 1 & 1;
+#pragma unroll
+      for (int w = 0; w < kValueBytes / 4; ++w) {
+        uint32_t by_dim[4];
+        transpose_bytes(raw_v[0][w], raw_v[1][w], raw_v[2][w], raw_v[3][w], by_dim);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h2_t a, b;
+          codes_to_f16<CODE>(by_dim[i], a, b);
+          h4_t* const to_row = (h4_t*)&values[to][place<8>(dim + 4 * w + i, piece_v)];
+          to_row[half] = h4_t{a.x, a.y, b.x, b.y};
+        }
+      }
+    };
+
+    auto multiply = [&](auto buffer, int key) {
+      constexpr int kFrom = decltype(buffer)::value;
+      f16x_t scores[2] = {};
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+          scores[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[kFrom][place<D / 8>(32 * half + r, 2 * c + h)], q[c], scores[half], 0, 0, 0);
+      // a lane's scores: key 32 i + 8 a + 4 h + e of the tile is scores[i][4 a + e]; 16 keys are eight of them
+      int entry[4];
+      float k_scale[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        entry[i] = ONE_PAGE && i > 0 ? entry[0] : min(((key + 16 * i) >> block_bits) - window.first, 63);
+        k_scale[i] = ONE_PAGE && i > 0 ? k_scale[0] : lane_value(window.k_scale, entry[i]);
+      }
+      float factor[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) factor[i] = ONE_PAGE && i > 0 ? factor[0] : row_factor * k_scale[i];
+      bool slow = key + kTile > all_see;
+#pragma unroll
+      for (int i = 0; i < (ONE_PAGE ? 1 : 4); ++i) slow |= careful >> entry[i] & 1;
+      if (slow) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int own = key + i / 16 * 32 + i % 16 / 4 * 8 + 4 * h + i % 4;
+          const bool missing = own >= seen || __builtin_amdgcn_readlane(window.page, entry[i / 8]) < 0;
+          scores[i / 16][i % 16] = missing ? -INFINITY : scores[i / 16][i % 16] * factor[i / 8];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) factor[i] = 1.f;
+      }
+      float top = -INFINITY;
+      if (ONE_PAGE) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, scores[i / 16][i % 16]);
+        top *= factor[0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float own = scores[i / 2][i % 2 * 8];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) own = fmaxf(own, scores[i / 2][i % 2 * 8 + e]);
+          top = fmaxf(top, own * factor[i]);
+        }
+      }
+      const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(swapped[0]), __uint_as_float(swapped[1]));
+      // p up to 2^6 is fine: where the maximum grows by less, the sums stay as they are
+      if (__any(top > most + 6.f)) {
+        const float next = fmaxf(top, most), keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - next);
+        most = next;
+        total_p *= keep;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) sums[j] *= keep;
+      }
+      const float base = most == -INFINITY ? 0.f : most;
+      h8_t p[4];
+      if (slow) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v_scale = lane_value(window.v_scale, entry[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float score = scores[i / 2][i % 2 * 8 + e], own = __builtin_amdgcn_exp2f(score - base);
+            total_p += own;
+            // whatever the scale of a page that the row does not see
+            p[i][e] = (_Float16)(score == -INFINITY ? 0.f : own * v_scale);
+          }
+        }
+      } else {  // v_scale as a part of the exponent
+        const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float shift = lane_value(v_log, entry[i]) - base;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e], factor[i], shift));
+            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e + 1], factor[i], shift));
+            const h2_t pair = {(_Float16)a, (_Float16)b};
+            sum = __builtin_amdgcn_fdot2(pair, ones, sum, false);
+            p[i][e] = pair.x, p[i][e + 1] = pair.y;
+          }
+          if (!ONE_PAGE || i == 3) {
+            total_p += sum * lane_value(v_inverse, entry[i]);
+            sum = 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+          sums[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[kFrom][place<8>(32 * j + r, 2 * i + h)], p[i], sums[j], 0, 0, 0);
+    };
+
+    auto step = [&](auto buffer, int t) {
+      constexpr int kFrom = decltype(buffer)::value;
+      const int key = low + t * kTile;
+      __syncthreads();
+      const bool more = t + 1 < tiles;
+      const bool turn = more && (key + 2 * kTile - 1) >> block_bits >= window.first + 64;
+      if (more && !turn) load(key + kTile);
+      if (key < one_sees) multiply(buffer, key);
+      if (turn) {
+        refill((key + kTile) >> block_bits);
+        load(key + kTile);
+      }
+      if (more) put(std::integral_constant<int, 1 - kFrom>());
+    };
+    if (tiles > 0) {
+      refill(low >> block_bits);
+      load(low);
+      put(std::integral_constant<int, 0>());
+      for (int t = 0; t < tiles; t += 2) {
+        step(std::integral_constant<int, 0>(), t);
+        if (t + 1 < tiles) step(std::integral_constant<int, 1>(), t + 1);
+      }
+    }
+
+    const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(total_p), __float_as_uint(total_p), false, false);
+    const float sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]), v_factor = power_of_two(v_exponent - 8);
+    if (row < rows) {
+      if (args.splits > 1) {
+        const long long at = split * all_rows + token * args.heads + query_head;
+        if (sum != 0.f) {
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+              *(f4_t*)(args.workspace + at * D + 32 * j + 8 * a + 4 * h) =
+                  f4_t{sums[j][4 * a], sums[j][4 * a + 1], sums[j][4 * a + 2], sums[j][4 * a + 3]} * v_factor;
+        }
+        if (h == 0) *(f2_t*)(pairs + 2 * at) = f2_t{most, sum};
+      } else {
+        const float factor = sum != 0.f ? v_factor / sum : 0.f;  // (a row that sees nothing: 0)
+        const long long at = token * args.out.token_stride + query_head * args.out.head_stride;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const float out[4] = {sums[j][4 * a] * factor, sums[j][4 * a + 1] * factor, sums[j][4 * a + 2] * factor, sums[j][4 * a + 3] * factor};
+            if (args.dtype == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 4>(args.out.data, at + 32 * j + 8 * a + 4 * h, out);
+            else store_values<ONEBIT_DTYPE_BF16, 4>(args.out.data, at + 32 * j + 8 * a + 4 * h, out);
+          }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int D, int CODE>
+hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
+  const onebit_sequences& q = args.sequences;
+  const int tiles = (int)(((long long)q.max_new * args.group + kRows - 1) / kRows);
+  const dim3 grid(args.cache.kv_heads * args.splits, tiles, q.count);
+  const auto kernel = args.cache.block >= kTile ? many_rows_kernel<D, CODE, true> : many_rows_kernel<D, CODE, false>;
+  return launch_kernel(kernel, grid, dim3(kWaves * 64), 0, stream, args, tiles);
+}
+
+}  // namespace
+
+hipError_t launch_many_rows(const AttentionArgs& args, hipStream_t stream) {
+  const bool int8 = args.cache.code == ONEBIT_CODE_INT8;
+  if (args.cache.head_dim == 64) return int8 ? launch_as<64, ONEBIT_CODE_INT8>(args, stream) : launch_as<64, ONEBIT_CODE_E4M3>(args, stream);
+  return int8 ? launch_as<128, ONEBIT_CODE_INT8>(args, stream) : launch_as<128, ONEBIT_CODE_E4M3>(args, stream);
+}
+
+}  // namespace onebit
