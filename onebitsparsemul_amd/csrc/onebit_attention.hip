@@ -293,7 +293,7 @@ void plan_attention(AttentionArgs& args, int compute_units) {
   const long long most = std::max(1ll, q.max_length > 0 ? std::min(room, (long long)q.max_length) : room);
   args.rows = rows <= 32 ? kRows : 128;
   const long long units = (rows + args.rows - 1) / args.rows * args.cache.kv_heads * q.count;
-  const long long splits = std::max(1ll, (args.rows == kRows ? 4ll : 1ll) * compute_units / units);
+  const long long splits = std::max(1ll, (args.rows == kRows ? 4ll : 2ll) * compute_units / units);
   const long long keys = std::max(args.rows == kRows ? 256ll : 512ll, ((most + splits - 1) / splits + 255) / 256 * 256);
   args.splits = (int)((most + keys - 1) / keys);
   args.keys_per_split = (int)keys;

@@ -13,13 +13,18 @@ namespace {
 typedef float f16x_t __attribute__((ext_vector_type(16)));
 constexpr int kTile = 64;  // keys
 constexpr int kWaves = 4, kRows = kWaves * 32;
+constexpr int kSchedProduct = 0x8, kSchedRead = 0x100;  // kinds of instructions for the scheduler
 
-// Where the 16-byte piece `piece` of a row lies: moved within its row, so that neighbouring rows' pieces fall on different banks for reads (32
-// rows, one piece) and writes alike.
+// Where the 16-byte piece `piece` of a row lies: moved within its row, so that eight neighbouring rows' pieces fall on different banks, and rows
+// eight apart do too (the values' writes). The piece takes part by exclusive or: other pieces of a row are one such operation away.
 template <int PIECES>
 __device__ inline int place(int row, int piece) {
-  if (PIECES == 16) return row * 16 + (piece ^ (row & 15));
-  return row * 8 + (piece ^ (((row >> 1) + (row >> 3)) & 7));
+  return row * PIECES + (piece ^ (PIECES == 16 ? row & 15 : (row >> 1 & 3) ^ (row >> 3 & 7)));
+}
+// The same value, for which the compiler keeps no register with what a loop makes of it
+__device__ inline int made_here(int x) {
+  asm("" : "+v"(x));
+  return x;
 }
 
 template <int D, int CODE, bool ONE_PAGE>
@@ -84,8 +89,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
     int v_exponent = -100;  // p takes v_scale 2^(8 - v_exponent)
 
     Window window = {0, -1, 0.f, 0.f};
-    float v_log = 0.f, v_inverse = 0.f;  // of the window's v_scale 2^(8 - v_exponent)
-    uint64_t careful = 0;                // entries without a page, or with a scale that an exponent does not take on well
+    // of the window's v_scale 2^(8 - v_exponent): logarithm and reciprocal
+    float v_log = 0.f, v_inverse = 0.f;
+    // entries whose scale p does not take on as a part of the exponent: too small beside the largest (p would lose bits in fp16), 0 or not finite.
+    // There p takes 2^8, and the scale multiplies the products.
+    uint64_t odd = 0;
     auto refill = [&](int entry) {
       const int e = fill_window(window, entry, (high - 1) >> block_bits, table, cache, head);
       if (e > v_exponent) {
@@ -95,9 +103,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
         v_exponent = e;
       }
       window.v_scale *= power_of_two(8 - v_exponent);
-      v_log = __builtin_amdgcn_logf(window.v_scale);
-      v_inverse = 1.f / window.v_scale;
-      careful = __ballot(!(window.page >= 0 && window.v_scale >= 0x1p-10f && window.v_scale <= 0x1p9f));
+      const bool plain = window.v_scale >= 0x1p-4f && window.v_scale <= 0x1p9f;
+      odd = __ballot(window.page >= 0 && !plain);
+      v_log = plain ? __builtin_amdgcn_logf(window.v_scale) : 8.f;
+      v_inverse = plain ? 1.f / window.v_scale : 0x1p-8f;
     };
 
     // the wavefront's share of a tile: kOwn keys, in one page
@@ -123,11 +132,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
     auto put = [&](auto buffer) {
       constexpr int to = decltype(buffer)::value;
       constexpr int kKeyLanes = D / kKeyBytes, kLanes = D / kValueBytes;
-      const int key = wave * kOwn + lane / kKeyLanes, piece = lane % kKeyLanes * (kKeyBytes / 8);
+      const int key_at = made_here(place<D / 8>(wave * kOwn + lane / kKeyLanes, lane % kKeyLanes * (kKeyBytes / 8)));
 #pragma unroll
-      for (int i = 0; i < kKeyBytes / 8; ++i) keys[to][place<D / 8>(key, piece + i)] = codes_to_f16<CODE>(raw_k[2 * i], raw_k[2 * i + 1]);
-      const int group = (wave * kOwn + lane / kLanes * 4) / 4, dim = lane % kLanes * kValueBytes;
-      const int piece_v = (group >> 2) * 2 + (group & 1), half = group >> 1 & 1;
+      for (int i = 0; i < kKeyBytes / 8; ++i) keys[to][key_at ^ i] = codes_to_f16<CODE>(raw_k[2 * i], raw_k[2 * i + 1]);
+      // four keys are half a piece of each dim's row; pieces are in the order in which the products want them
+      const int group = (wave * kOwn + lane / kLanes * 4) / 4, half = group >> 1 & 1;
+      const int value_at = made_here(place<8>(lane % kLanes * kValueBytes, (group >> 2) * 2 + (group & 1)));
 #pragma unroll
       for (int w = 0; w < kValueBytes / 4; ++w) {
         uint32_t by_dim[4];
@@ -136,8 +146,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
         for (int i = 0; i < 4; ++i) {
           h2_t a, b;
           codes_to_f16<CODE>(by_dim[i], a, b);
-          h4_t* const to_row = (h4_t*)&values[to][place<8>(dim + 4 * w + i, piece_v)];
-          to_row[half] = h4_t{a.x, a.y, b.x, b.y};
+          ((h4_t*)&values[to][(value_at ^ (4 * w + i) >> 1) + (4 * w + i) * 8])[half] = h4_t{a.x, a.y, b.x, b.y};
         }
       }
     };
@@ -145,11 +154,20 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
     auto multiply = [&](auto buffer, int key) {
       constexpr int kFrom = decltype(buffer)::value;
       f16x_t scores[2] = {};
+      const int own_key = made_here(place<D / 8>(r, h)), own_value = made_here(place<8>(r, h));
+      constexpr int kAhead = 6;  // LDS reads in front of the first product: their latency is that of several
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-          scores[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[kFrom][place<D / 8>(32 * half + r, 2 * c + h)], q[c], scores[half], 0, 0, 0);
+        for (int half = 0; half < 2; ++half)
+          scores[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[kFrom][32 * (D / 8) * half + (own_key ^ 2 * c ^ (D == 64 ? 4 * half : 0))], q[c], scores[half], 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedRead, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < D / 8 - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kSchedProduct, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedRead, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedProduct, kAhead, 0);
       // a lane's scores: key 32 i + 8 a + 4 h + e of the tile is scores[i][4 a + e]; 16 keys are eight of them
       int entry[4];
       float k_scale[4];
@@ -161,18 +179,24 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
       float factor[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) factor[i] = ONE_PAGE && i > 0 ? factor[0] : row_factor * k_scale[i];
-      bool slow = key + kTile > all_see;
+      bool masked = key + kTile > all_see, any_odd = false;
 #pragma unroll
-      for (int i = 0; i < (ONE_PAGE ? 1 : 4); ++i) slow |= careful >> entry[i] & 1;
-      if (slow) {
+      for (int i = 0; i < (ONE_PAGE ? 1 : 4); ++i) {
+        masked |= __builtin_amdgcn_readlane(window.page, entry[i]) < 0;
+        any_odd |= odd >> entry[i] & 1;
+      }
+      if (masked) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int own = key + i / 16 * 32 + i % 16 / 4 * 8 + 4 * h + i % 4;
-          const bool missing = own >= seen || __builtin_amdgcn_readlane(window.page, entry[i / 8]) < 0;
-          scores[i / 16][i % 16] = missing ? -INFINITY : scores[i / 16][i % 16] * factor[i / 8];
+        for (int i = 0; i < 4; ++i) {
+          // the row sees this many of the tile's keys from here on; none of a page that is not there
+          const int left = __builtin_amdgcn_readlane(window.page, entry[i]) < 0 ? 0 : seen - (key + i / 2 * 32 + i % 2 * 16 + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float score = scores[i / 2][i % 2 * 8 + e] * factor[i];
+            scores[i / 2][i % 2 * 8 + e] = e / 4 * 8 + e % 4 < left ? score : -INFINITY;
+          }
+          factor[i] = 1.f;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) factor[i] = 1.f;
       }
       float top = -INFINITY;
       if (ONE_PAGE) {
@@ -200,43 +224,55 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
       }
       const float base = most == -INFINITY ? 0.f : most;
       h8_t p[4];
-      if (slow) {
+      const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
+      float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v_scale = lane_value(window.v_scale, entry[i]);
+      for (int i = 0; i < 4; ++i) {
+        const float shift = lane_value(v_log, entry[i]) - base;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float score = scores[i / 2][i % 2 * 8 + e], own = __builtin_amdgcn_exp2f(score - base);
-            total_p += own;
-            // whatever the scale of a page that the row does not see
-            p[i][e] = (_Float16)(score == -INFINITY ? 0.f : own * v_scale);
-          }
+        for (int e = 0; e < 8; e += 2) {
+          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e], factor[i], shift));
+          const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e + 1], factor[i], shift));
+          const h2_t pair = {(_Float16)a, (_Float16)b};
+          sum = __builtin_amdgcn_fdot2(pair, ones, sum, false);
+          p[i][e] = pair.x, p[i][e + 1] = pair.y;
         }
-      } else {  // v_scale as a part of the exponent
-        const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
-        float sum = 0.f;
+        if (!ONE_PAGE || i == 3) {
+          total_p += sum * lane_value(v_inverse, entry[i]);
+          sum = 0.f;
+        }
+      }
+      // rows 32 j + r of the values, pieces 2 i + h: place() moves a row's pieces by 4 with every 32 rows
+      auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 4 * (j & 1))]; };
+      if (any_odd) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float shift = lane_value(v_log, entry[i]) - base;
+        for (int page = 0; page < (ONE_PAGE ? 1 : 4); ++page) {
+          if (!(odd >> entry[page] & 1)) continue;
+          // whatever the scale of a page that the row does not see
+          const float v_scale = key + 16 * page < seen ? lane_value(window.v_scale, entry[page]) * 0x1p-8f : 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e], factor[i], shift));
-            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e + 1], factor[i], shift));
-            const h2_t pair = {(_Float16)a, (_Float16)b};
-            sum = __builtin_amdgcn_fdot2(pair, ones, sum, false);
-            p[i][e] = pair.x, p[i][e + 1] = pair.y;
+          for (int j = 0; j < D / 32; ++j) {
+            f16x_t own = {};
+#pragma unroll
+            for (int i = page; i < (ONE_PAGE ? 4 : page + 1); ++i) own = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p[i], own, 0, 0, 0);
+            sums[j] += own * v_scale;
+            asm volatile("" : "+v"(sums[j]));  // here, and not further down: one product's registers at a time
           }
-          if (!ONE_PAGE || i == 3) {
-            total_p += sum * lane_value(v_inverse, entry[i]);
-            sum = 0.f;
-          }
+#pragma unroll
+          for (int i = page; i < (ONE_PAGE ? 4 : page + 1); ++i) p[i] = h8_t{};
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-          sums[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[kFrom][place<8>(32 * j + r, 2 * i + h)], p[i], sums[j], 0, 0, 0);
+        for (int j = 0; j < D / 32; ++j) sums[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p[i], sums[j], 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedRead, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < D / 8 - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kSchedProduct, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedRead, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedProduct, kAhead, 0);
     };
 
     auto step = [&](auto buffer, int t) {
