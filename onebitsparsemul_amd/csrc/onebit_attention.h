@@ -91,18 +91,39 @@ struct Window {
   int page;  // -1: none
   float k_scale, v_scale;
 };
-// Fills the window with the entries from `entry` to `last`, and returns the exponent of the largest finite v_scale among them (-100 to 110).
-__device__ inline int fill_window(Window& window, int entry, int last, const int* table, const onebit_cache& cache, int head) {
+__device__ inline Window load_pages(int entry, int width, const int* table, const onebit_cache& cache) {
   const int own = entry + (int)(threadIdx.x % 64);
-  window = {entry, own <= last ? table[own] : -1, 0.f, 0.f};
+  Window window = {entry, own < width ? table[own] : -1, 0.f, 0.f};
   if (window.page >= cache.pages) window.page = -1;
+  return window;
+}
+// Drops the window's pages behind entry `last`.
+__device__ inline void drop_pages(Window& window, int last) {
+  if (window.first + (int)(threadIdx.x % 64) > last) window.page = -1;
+}
+__device__ inline void load_scales(Window& window, const onebit_cache& cache, int head) {
+  window.k_scale = window.v_scale = 0.f;
   if (window.page >= 0) {
     const long long at = (long long)window.page * cache.kv_heads + head;
     window.k_scale = cache.k_scale[at];
     window.v_scale = cache.v_scale[at];
   }
+}
+// Exponent of the window's largest finite v_scale (-100 to 110)
+__device__ inline int largest_exponent(const Window& window) {
   const uint32_t bits = magnitude(window.v_scale);
   return min(exponent_of(wave_max(bits < 0x7f800000u ? bits : 0), -100), 110);
+}
+
+// token and head of the key/value head of a row of q, `step` rows behind the first of a tile
+struct Rows {
+  int token, head;  // of the tile's first row
+};
+__device__ inline Rows first_row(int row, int group) { return row == 0 ? Rows{0, 0} : Rows{row / group, row % group}; }
+__device__ inline Rows behind(Rows first, int step, const AttentionArgs& args) {
+  // exact: numbers below group + 128, whose product with group is below 2^32
+  const uint32_t n = first.head + step, tokens = args.group == 1 ? n : __umulhi(n, args.group_inverse);
+  return {first.token + (int)tokens, (int)(n - tokens * args.group)};
 }
 
 }  // namespace onebit

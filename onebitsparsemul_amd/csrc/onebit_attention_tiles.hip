@@ -47,19 +47,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
   // the last rows see the most keys: first
   for (int tile = row_tiles - 1 - (int)blockIdx.y + (rows > row_tiles * kRows ? ((rows + kRows - 1) / kRows - 1) / row_tiles * row_tiles : 0); tile >= 0; tile -= row_tiles) {
     if (tile * kRows >= rows) continue;
-    const int last_token = (min(tile * kRows + kRows, rows) - 1) / args.group;
+    const Rows own_first = first_row(tile * kRows, args.group);
+    const int last_token = behind(own_first, min(kRows, rows - tile * kRows) - 1, args).token;
     const int total = max(seq.length - seq.fresh + last_token + 1, 0);
     const int low = split * args.keys_per_split, high = split == args.splits - 1 ? total : min(total, low + args.keys_per_split);
     const int tiles = max(high - low + kTile - 1, 0) / kTile;
     const int wave_row = tile * kRows + wave * 32;
     // keys that all rows of the wavefront see, and that one of them sees
-    const int all_see = wave_row + 32 <= rows ? max(seq.length - seq.fresh + wave_row / args.group + 1, 0) : 0;
-    const int one_sees = wave_row < rows ? max(seq.length - seq.fresh + (min(wave_row + 32, rows) - 1) / args.group + 1, 0) : 0;
+    const int before = seq.length - seq.fresh + 1, here = min(max(rows - wave_row, 0), 32);
+    const int all_see = here == 32 ? max(before + behind(own_first, wave * 32, args).token, 0) : 0;
+    const int one_sees = here > 0 ? max(before + behind(own_first, wave * 32 + here - 1, args).token, 0) : 0;
     // the row of this lane's column
     const int row = wave_row + r;
-    const long long token = seq.start + row / args.group;
-    const int query_head = head * args.group + row % args.group;
-    const int seen = row < rows ? max(seq.length - seq.fresh + row / args.group + 1, 0) : 0;
+    const Rows own_row = behind(own_first, wave * 32 + r, args);
+    const long long token = seq.start + own_row.token;
+    const int query_head = head * args.group + own_row.head;
+    const int seen = row < rows ? max(before + own_row.token, 0) : 0;
 
     h8_t q[D / 16];
     float row_factor = args.scale * kLog2E;
@@ -95,7 +98,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
     // There p takes 2^8, and the scale multiplies the products.
     uint64_t odd = 0;
     auto refill = [&](int entry) {
-      const int e = fill_window(window, entry, (high - 1) >> block_bits, table, cache, head);
+      window = load_pages(entry, args.sequences.width, table, cache);
+      drop_pages(window, (high - 1) >> block_bits);
+      load_scales(window, cache, head);
+      const int e = largest_exponent(window);
       if (e > v_exponent) {
         const float down = v_exponent == -100 ? 0.f : power_of_two(max(v_exponent - e, -126));
 #pragma unroll

@@ -71,6 +71,8 @@ int attention_args(const onebit_cache* cache, const onebit_sequences* sequences,
   args.sequences = planned(*sequences);
   args.heads = heads;
   args.group = heads / cache->kv_heads;
+  if (args.group > 32768) return refuse("%d heads to a key/value head: at most 32768", args.group);
+  args.group_inverse = (uint32_t)(((1ull << 32) + args.group - 1) / args.group);
   onebit::plan_attention(args, onebit::device_compute_units());
   return ONEBIT_OK;
 }

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "onebit_decoder.h"
 
 namespace onebit {
@@ -59,15 +61,29 @@ constexpr float kMostE4M3 = 448.f, kMostInt8 = 127.f;
 // Magnitudes as integers: their order is that of the floats, and NaN is the largest, so that a maximum does not lose it.
 __device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// Over the 64 lanes, the same in each: neighbours, pairs, halves of a row of 16 and rows by cross-lane moves, then rows and halves by swaps.
+template <class Value, class Combine>
+__device__ inline Value over_wave(Value x, Combine combine) {
+  auto moved = [&](auto pattern) {
+    return __builtin_bit_cast(Value, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(pattern)::value, 0xf, 0xf, true));
+  };
+  x = combine(x, moved(std::integral_constant<int, 0xb1>()));   // lane ^ 1
+  x = combine(x, moved(std::integral_constant<int, 0x4e>()));   // lane ^ 2
+  x = combine(x, moved(std::integral_constant<int, 0x141>()));  // the other four of eight
+  x = combine(x, moved(std::integral_constant<int, 0x140>()));  // the other eight of sixteen
+  auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = combine(__builtin_bit_cast(Value, (uint32_t)r[0]), __builtin_bit_cast(Value, (uint32_t)r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return combine(__builtin_bit_cast(Value, (uint32_t)r[0]), __builtin_bit_cast(Value, (uint32_t)r[1]));
+}
 __device__ inline uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) x = max(x, (uint32_t)__shfl_xor((int)x, step));
-  return x;
+  return over_wave(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ inline float wave_max(float x) {
+  return over_wave(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ inline float wave_sum(float x) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) x += __shfl_xor(x, step);
-  return x;
+  return over_wave(x, [](float a, float b) { return a + b; });
 }
 
 // A sequence of a call, its numbers brought into range.

@@ -32,6 +32,7 @@ struct AttentionArgs {
   onebit_sequences sequences;
   onebit_heads q, out;
   int heads, group;  // group: heads of a key/value head
+  uint32_t group_inverse;  // 2^32 / group, rounded up
   int dtype;
   float scale;
   int rows;  // of q to a workgroup: 16 (few_rows_kernel), 128 or 256 (many_rows_kernel)
