@@ -3,7 +3,8 @@
 // Mathematics: out = sum_j p_j v_j / sum_j p_j with p_j = exp2(t_j - m), t_j = log2(e) scale k_scale q . k_code_j and m the largest t so far, in
 // one pass over the keys; where m grows, what is summed so far is multiplied by exp2(m_old - m). Codes are exact in fp16, and so
 // is q (bf16 rows as q 2^-e), so that the products of the matrix instructions are exact and their sums fp32. p_j takes its key's
-// v_scale, by the power of two that the largest scale seen so far gives, and 2^15 on top: then fp16 keeps eleven bits of each p_j down to 2^-29.
+// v_scale by its power of two beside that of the keys around it, and some powers on top, so that fp16 keeps the bits of small p_j; the sums follow
+// that power exactly.
 //
 // Scores are computed as K Q^T: a lane then holds scores of one row of q (matrix column) and of the keys that the next product,
 // V^T P^T, wants from it as its own operand: p goes from one matrix instruction to the next without leaving its register.
@@ -61,8 +62,26 @@ __device__ inline float sum_over_16(float x) {
 }
 
 __device__ inline float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
-// Exponent of a magnitude, at least `least` (a NaN and infinities: 128)
-__device__ inline int exponent_of(uint32_t magnitude_bits, int least) { return max((int)(magnitude_bits >> 23) - 127, least); }
+// Exponent of a normal magnitude (a NaN and infinities: 128)
+__device__ inline int exponent_of(uint32_t magnitude_bits) { return (int)(magnitude_bits >> 23) - 127; }
+
+// What takes a v_scale's part in exponents: one below 2^-100 is as good as 0, one that is not finite is dealt with apart.
+__device__ inline float usable_scale(float scale) {
+  return magnitude(scale) >= 0x7f800000u ? 0x1p-100f : fminf(fmaxf(scale, 0x1p-100f), 0x1p110f);
+}
+// The exponent that the sums stand in: that of the keys' v_scale at hand, followed where it grows or falls by more than a few, for fp16 to keep the
+// bits of small p beside it. Never further below the largest so far than fp32 has room for.
+struct Exponent {
+  int now = -100, largest = -100;
+  // The power of two that the sums take on.
+  __device__ float follow(int power) {
+    if (power <= now && power >= now - 6) return 1.f;
+    largest = max(largest, power);
+    const int next = max(power, largest - 60), down = max(now - next, -126);
+    now = next;
+    return power_of_two(down);
+  }
+};
 
 __device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 __device__ inline float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
@@ -109,12 +128,6 @@ __device__ inline void load_scales(Window& window, const onebit_cache& cache, in
     window.v_scale = cache.v_scale[at];
   }
 }
-// Exponent of the window's largest finite v_scale (-100 to 110)
-__device__ inline int largest_exponent(const Window& window) {
-  const uint32_t bits = magnitude(window.v_scale);
-  return min(exponent_of(wave_max(bits < 0x7f800000u ? bits : 0), -100), 110);
-}
-
 // token and head of the key/value head of a row of q, `step` rows behind the first of a tile
 struct Rows {
   int token, head;  // of the tile's first row

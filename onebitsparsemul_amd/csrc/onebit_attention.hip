@@ -50,16 +50,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
 
     f4_t sums[D / 16] = {};
     float most = -INFINITY, total_p = 0.f;
-    int v_exponent = -100;  // p takes v_scale 2^(14 - v_exponent)
-    auto take_scales = [&] {
-      const int e = largest_exponent(window);
-      if (e > v_exponent) {
-        const float down = v_exponent == -100 ? 0.f : power_of_two(max(v_exponent - e, -126));
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) sums[j] *= down;
-        v_exponent = e;
-      }
-    };
+    Exponent v_exponent;  // p takes v_scale 2^(14 - exponent of the step's largest)
 
     // Codes of a chunk as they come from memory: lane (r, g) takes key r of each tile for the scores (bytes 64 u + 16 g of its row), and keys
     // 4 g ... 4 g + 3 of each tile for the values (D / 16 bytes from r D / 16 on). The next chunk's are asked for as soon as this one's are used.
@@ -69,16 +60,21 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
     long long place[kTiles];
     int entries[kTiles];
     float k_scale[kTiles], v_scale[kTiles];
+    int powers[kTiles];  // exponents of v_scale
     auto find_scales = [&] {
+      const int power = exponent_of(magnitude(usable_scale(window.v_scale)));
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) k_scale[t] = lane_value(window.k_scale, entries[t]), v_scale[t] = lane_value(window.v_scale, entries[t]);
+      for (int t = 0; t < kTiles; ++t) {
+        k_scale[t] = lane_value(window.k_scale, entries[t]);
+        v_scale[t] = lane_value(window.v_scale, entries[t]);
+        powers[t] = __builtin_amdgcn_readlane(power, entries[t]);
+      }
     };
     auto find = [&](int key) {
       if ((key + kChunk - 1) >> block_bits >= window.first + 64) {
         window = load_pages(key >> block_bits, args.sequences.width, table, cache);
         drop_pages(window, (end - 1) >> block_bits);
         load_scales(window, cache, head);
-        take_scales();
       }
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
@@ -109,8 +105,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
       find(first);
       load_keys();
       load_values();
-      take_scales();  // (behind the first codes' loads: they wait for the pages alone)
-      find_scales();
+      find_scales();  // (behind the first codes' loads: they wait for the pages alone)
     }
     h8_t q[D / 64][2];
     float row_factor = args.scale * kLog2E;
@@ -121,7 +116,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) largest = max(largest, max(magnitude_bf16(raw[u][0]), magnitude_bf16(raw[u][1])));
         largest = __float_as_uint(max_over_16(__uint_as_float(min(largest, 0x7f800000u))));
-        const int e = exponent_of(largest, -100);
+        const int e = max(exponent_of(largest), -100);
         factor = power_of_two(8 - e);
         row_factor *= power_of_two(e - 8);
       }
@@ -140,12 +135,14 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
         }
       int there[kTiles], there_all = 0;
       float k_factor[kTiles], own_v[kTiles];
+      int power = -1000;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         there[t] = valid[t];
         there_all += valid[t];
         k_factor[t] = row_factor * k_scale[t];
         own_v[t] = v_scale[t];
+        power = max(power, powers[t]);
       }
       const bool more = key + kChunk < end;
       if (more) {
@@ -171,14 +168,15 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
 #pragma unroll
       for (int i = 1; i < 4 * kTiles; ++i) top = fmaxf(top, scores[i / 4][i % 4]);
       top = max_over_16(top);
-      if (__any(top > most)) {
+      const float v_keep = v_exponent.follow(power);
+      if (__any(top > most) || v_keep != 1.f) {
         const float next = fmaxf(top, most), keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - next);
         most = next;
         total_p *= keep;
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) sums[j] *= keep;
+        for (int j = 0; j < D / 16; ++j) sums[j] *= keep * v_keep;
       }
-      const float base = most == -INFINITY ? 0.f : most, v_factor = power_of_two(14 - v_exponent);
+      const float base = most == -INFINITY ? 0.f : most, v_factor = power_of_two(14 - v_exponent.now);
       h8_t p_high[kTiles / 2], p_low[kTiles / 2];  // together 22 bits of p: the eight rows that fp16 alone would cost are there anyway
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
@@ -228,7 +226,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w * kRows + r]);
     // (NaN goes on: a maximum that is none has no keys, or a NaN in its sum)
-    const float share = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(most - top), v_factor = power_of_two(v_exponent - 14);
+    const float share = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(most - top), v_factor = power_of_two(v_exponent.now - 14);
     if (row < rows) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) most = max(most, magnitude_bf16(raw[c]));
         most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-        const int e = exponent_of(most, -100);
+        const int e = max(exponent_of(most), -100);
         factor = power_of_two(8 - e);
         row_factor *= power_of_two(e - 8);
       }
@@ -89,30 +89,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
 
     f16x_t sums[D / 32] = {};
     float most = -INFINITY, total_p = 0.f;
-    int v_exponent = -100;  // p takes v_scale 2^(8 - v_exponent)
+    Exponent v_exponent;  // p takes v_scale 2^(8 - exponent of the tile's largest)
 
     Window window = {0, -1, 0.f, 0.f};
-    // of the window's v_scale 2^(8 - v_exponent): logarithm and reciprocal
+    // of the window's v_scale: exponent, logarithm and reciprocal
+    int v_power = 0;
     float v_log = 0.f, v_inverse = 0.f;
-    // entries whose scale p does not take on as a part of the exponent: too small beside the largest (p would lose bits in fp16), 0 or not finite.
-    // There p takes 2^8, and the scale multiplies the products.
-    uint64_t odd = 0;
+    uint64_t bad = 0;  // entries whose scale is not finite
     auto refill = [&](int entry) {
       window = load_pages(entry, args.sequences.width, table, cache);
       drop_pages(window, (high - 1) >> block_bits);
       load_scales(window, cache, head);
-      const int e = largest_exponent(window);
-      if (e > v_exponent) {
-        const float down = v_exponent == -100 ? 0.f : power_of_two(max(v_exponent - e, -126));
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) sums[j] *= down;
-        v_exponent = e;
-      }
-      window.v_scale *= power_of_two(8 - v_exponent);
-      const bool plain = window.v_scale >= 0x1p-4f && window.v_scale <= 0x1p9f;
-      odd = __ballot(window.page >= 0 && !plain);
-      v_log = plain ? __builtin_amdgcn_logf(window.v_scale) : 8.f;
-      v_inverse = plain ? 1.f / window.v_scale : 0x1p-8f;
+      bad = __ballot(magnitude(window.v_scale) >= 0x7f800000u);
+      const float scale = usable_scale(window.v_scale);
+      v_power = exponent_of(magnitude(scale));
+      v_log = __builtin_amdgcn_logf(scale);
+      v_inverse = 1.f / scale;
     };
 
     // the wavefront's share of a tile: kOwn keys, in one page
@@ -185,11 +177,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
       float factor[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) factor[i] = ONE_PAGE && i > 0 ? factor[0] : row_factor * k_scale[i];
-      bool masked = key + kTile > all_see, any_odd = false;
+      bool masked = key + kTile > all_see, any_bad = false;
+      int power = -1000, powers[4];
 #pragma unroll
-      for (int i = 0; i < (ONE_PAGE ? 1 : 4); ++i) {
+      for (int i = 0; i < 4; ++i) {
+        if (ONE_PAGE && i > 0) {
+          powers[i] = powers[0];
+          continue;
+        }
         masked |= __builtin_amdgcn_readlane(window.page, entry[i]) < 0;
-        any_odd |= odd >> entry[i] & 1;
+        any_bad |= bad >> entry[i] & 1;
+        powers[i] = __builtin_amdgcn_readlane(v_power, entry[i]);
+        power = max(power, powers[i]);
       }
       if (masked) {
 #pragma unroll
@@ -221,52 +220,72 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
       const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(swapped[0]), __uint_as_float(swapped[1]));
       // p up to 2^6 is fine: where the maximum grows by less, the sums stay as they are
-      if (__any(top > most + 6.f)) {
+      const float v_keep = v_exponent.follow(power);
+      if (__any(top > most + 6.f) || v_keep != 1.f) {
         const float next = fmaxf(top, most), keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - next);
         most = next;
         total_p *= keep;
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) sums[j] *= keep;
+        for (int j = 0; j < D / 32; ++j) sums[j] *= keep * v_keep;
       }
       const float base = most == -INFINITY ? 0.f : most;
-      h8_t p[4];
+      // rows 32 j + r of the values, pieces 2 i + h: place() moves a row's pieces by 4 with every 32 rows
+      auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 4 * (j & 1))]; };
       const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
       float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float shift = lane_value(v_log, entry[i]) - base;
+      // p of 16 keys, with v_scale as a part of the exponent
+      auto weigh = [&](int i, float log) {
+        const float shift = log + (float)(8 - v_exponent.now) - base;
+        h8_t p;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e], factor[i], shift));
           const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[i / 2][i % 2 * 8 + e + 1], factor[i], shift));
           const h2_t pair = {(_Float16)a, (_Float16)b};
           sum = __builtin_amdgcn_fdot2(pair, ones, sum, false);
-          p[i][e] = pair.x, p[i][e + 1] = pair.y;
+          p[e] = pair.x, p[e + 1] = pair.y;
         }
+        return p;
+      };
+      int least = powers[0];
+#pragma unroll
+      for (int i = 1; i < (ONE_PAGE ? 1 : 4); ++i) least = min(least, powers[i]);
+      if (least < v_exponent.now - 6) {
+        // Pages of one tile whose scales are far apart (p of the smaller ones would lose its bits beside the largest), or a scale too small for the sums
+        // to follow, which counts as the smallest that they can: nothing beside the largest. By themselves, and then no more.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (powers[i] >= power - 6 && powers[i] >= v_exponent.now - 6) continue;
+          const float own_keep = v_exponent.follow(powers[i]);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) sums[j] *= own_keep;
+          const bool negligible = powers[i] < v_exponent.now;
+          const h8_t p = weigh(i, negligible ? (float)v_exponent.now : lane_value(v_log, entry[i]));
+          total_p += sum * (negligible ? 0x1p-8f : lane_value(v_inverse, entry[i]) * power_of_two(v_exponent.now - 8));
+          sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) sums[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p, sums[j], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) scores[i / 2][i % 2 * 8 + e] = -INFINITY;
+          factor[i] = 1.f;
+        }
+        const float own_keep = v_exponent.follow(power);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) sums[j] *= own_keep;
+      }
+      h8_t p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = weigh(i, lane_value(v_log, entry[i]));
         if (!ONE_PAGE || i == 3) {
-          total_p += sum * lane_value(v_inverse, entry[i]);
+          total_p += sum * (lane_value(v_inverse, entry[i]) * power_of_two(v_exponent.now - 8));
           sum = 0.f;
         }
       }
-      // rows 32 j + r of the values, pieces 2 i + h: place() moves a row's pieces by 4 with every 32 rows
-      auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 4 * (j & 1))]; };
-      if (any_odd) {
+      if (any_bad) {
 #pragma unroll
-        for (int page = 0; page < (ONE_PAGE ? 1 : 4); ++page) {
-          if (!(odd >> entry[page] & 1)) continue;
-          // whatever the scale of a page that the row does not see
-          const float v_scale = key + 16 * page < seen ? lane_value(window.v_scale, entry[page]) * 0x1p-8f : 0.f;
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            f16x_t own = {};
-#pragma unroll
-            for (int i = page; i < (ONE_PAGE ? 4 : page + 1); ++i) own = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p[i], own, 0, 0, 0);
-            sums[j] += own * v_scale;
-            asm volatile("" : "+v"(sums[j]));  // here, and not further down: one product's registers at a time
-          }
-#pragma unroll
-          for (int i = page; i < (ONE_PAGE ? 4 : page + 1); ++i) p[i] = h8_t{};
-        }
+        for (int i = 0; i < 4; ++i)  // a row sees the scale of a page if it sees one of its keys
+          if ((bad >> entry[i] & 1) && key + 16 * i < seen) total_p = __builtin_nanf("");
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -306,7 +325,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
     }
 
     const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(total_p), __float_as_uint(total_p), false, false);
-    const float sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]), v_factor = power_of_two(v_exponent - 8);
+    const float sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]), v_factor = v_exponent.largest > -100 ? power_of_two(v_exponent.now - 8) : 0.f;
     if (row < rows) {
       if (args.splits > 1) {
         const long long at = split * all_rows + token * args.heads + query_head;
