@@ -372,9 +372,10 @@ void plan_attention(AttentionArgs& args, int compute_units) {
   const onebit_sequences& q = args.sequences;
   const long long rows = (long long)q.max_new * args.group, room = (long long)q.width * args.cache.block;
   const long long most = std::max(1ll, q.max_length > 0 ? std::min(room, (long long)q.max_length) : room);
-  args.rows = rows <= 32 ? kRows : 128;
+  args.rows = rows <= 32 ? kRows : many_rows(args.cache.head_dim);
   const long long units = (rows + args.rows - 1) / args.rows * args.cache.kv_heads * q.count;
-  const long long slots = (args.rows == kRows ? 3ll : 2ll) * compute_units, splits = std::max(1ll, slots / units);
+  // workgroups that the device holds
+  const long long slots = (args.rows == kRows ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units, splits = std::max(1ll, slots / units);
   // one step of each wavefront
   const long long least = args.rows == kRows ? kWaves * 4096 / args.cache.head_dim : 512;
   long long keys = std::max(least, ((most + splits - 1) / splits + least - 1) / least * least);

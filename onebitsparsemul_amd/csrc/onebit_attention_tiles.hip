@@ -1,6 +1,6 @@
 // Attention over the 8-bit cache (onebit_decoder.h) for many rows of q to a key/value head: prompts.
 //
-// A workgroup takes 128 rows (tokens x heads of the key/value head), 32 to a wavefront, and walks over the keys in tiles of 64. Each tile's
+// A workgroup takes 256 rows (128 where heads are of 64; tokens x heads of the key/value head), 32 to a wavefront, and walks over the keys in tiles of 64. Each tile's
 // codes are read once, turned into fp16 by the wavefronts together, and lie in LDS twice (one tile in use, one being written): keys by rows of
 // dims, values by rows of keys, so that both matrix products (32x32x16, fp16) read their left operand with one 16-byte load a lane.
 #include "onebit_attention.h"
@@ -12,7 +12,6 @@ namespace {
 
 typedef float f16x_t __attribute__((ext_vector_type(16)));
 constexpr int kTile = 64;  // keys
-constexpr int kWaves = 4, kRows = kWaves * 32;
 constexpr int kSchedProduct = 0x8, kSchedRead = 0x100;  // kinds of instructions for the scheduler
 
 // Where the 16-byte piece `piece` of a row lies: moved within its row, so that eight neighbouring rows' pieces fall on different banks, and rows
@@ -28,7 +27,8 @@ __device__ inline int made_here(int x) {
 }
 
 template <int D, int CODE, bool ONE_PAGE>
-__global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs args, int row_tiles) {
+__global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(AttentionArgs args, int row_tiles) {
+  constexpr int kRows = many_rows(D), kWaves = kRows / 32;
   constexpr int kOwn = kTile / kWaves;  // keys a wavefront brings in
   constexpr int kKeyBytes = kOwn * D / 64, kValueBytes = D * kOwn / 256;
   typedef uint32_t key_words __attribute__((ext_vector_type(kKeyBytes / 4)));
@@ -358,10 +358,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void many_rows_kernel(AttentionArgs
 template <int D, int CODE>
 hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
   const onebit_sequences& q = args.sequences;
+  constexpr int kRows = many_rows(D);
   const int tiles = (int)(((long long)q.max_new * args.group + kRows - 1) / kRows);
   const dim3 grid(args.cache.kv_heads * args.splits, tiles, q.count);
   const auto kernel = args.cache.block >= kTile ? many_rows_kernel<D, CODE, true> : many_rows_kernel<D, CODE, false>;
-  return launch_kernel(kernel, grid, dim3(kWaves * 64), 0, stream, args, tiles);
+  return launch_kernel(kernel, grid, dim3(kRows * 2), 0, stream, args, tiles);
 }
 
 }  // namespace

@@ -35,12 +35,14 @@ struct AttentionArgs {
   uint32_t group_inverse;  // 2^32 / group, rounded up
   int dtype;
   float scale;
-  int rows;  // of q to a workgroup: 16 (few_rows_kernel), 128 or 256 (many_rows_kernel)
+  int rows;  // of q to a workgroup: 16 (few_rows_kernel) or many_rows() (many_rows_kernel)
   // keys split over workgroups: split i takes keys [i * keys_per_split, ...) of its sequence; workspace: splits x tokens x heads rows of
   // head_dim fp32 sums, then as many pairs (running maximum, sum); splits == 1: none
   int splits, keys_per_split;
   float* workspace;
 };
+// Rows of q to a workgroup of many_rows_kernel
+constexpr int many_rows(int head_dim) { return head_dim == 64 ? 128 : 256; }
 // Fills rows and the split of `args`.
 void plan_attention(AttentionArgs& args, int compute_units);
 size_t attention_workspace(const AttentionArgs& args);
