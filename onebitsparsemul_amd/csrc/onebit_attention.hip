@@ -368,18 +368,26 @@ hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
 }  // namespace
 
 // Rows of q to a workgroup, and how its keys are split over workgroups where a call has fewer of them than the device holds at once.
+//
+// few_rows_kernel reads the keys for every 16 rows again but starts and ends quickly and fills the device with few rows; many_rows_kernel does
+// with a quarter of the work. Both sides of the rule, head_dim 64 | 128: one prompt of 512 tokens (8 heads on 4: 256 workgroups) 6.8 | 8.7 us with the
+// first, 13.4 | 21.5 with the second; 8 prompts of 128 (32 heads on 8: 2048 workgroups) 14.8 | 19.7 and 7.8 | 13.3; 64 tokens behind 20000 (32 heads on 8: 128
+// workgroups, but 2.5 million keys for them) 47 | 69 and 34 | 41.
+// A split costs its join, some 3 us: few rows go unsplit up to three steps (500 keys, heads of 64: 6.5 us, 7.8 in two splits), four where the device is full.
 void plan_attention(AttentionArgs& args, int compute_units) {
   const onebit_sequences& q = args.sequences;
   const long long rows = (long long)q.max_new * args.group, room = (long long)q.width * args.cache.block;
   const long long most = std::max(1ll, q.max_length > 0 ? std::min(room, (long long)q.max_length) : room);
-  args.rows = rows <= 32 ? kRows : many_rows(args.cache.head_dim);
-  const long long units = (rows + args.rows - 1) / args.rows * args.cache.kv_heads * q.count;
+  auto workgroups = [&](int of) { return (rows + of - 1) / of * args.cache.kv_heads * q.count; };
+  const bool few = rows <= 32 || (workgroups(kRows) <= 3ll * compute_units && workgroups(kRows) * most * args.cache.head_dim <= 148000ll * compute_units);
+  args.rows = few ? kRows : many_rows(args.cache.head_dim);
+  const long long units = workgroups(args.rows);
   // workgroups that the device holds
-  const long long slots = (args.rows == kRows ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units, splits = std::max(1ll, slots / units);
-  // one step of each wavefront
-  const long long least = args.rows == kRows ? kWaves * 4096 / args.cache.head_dim : 512;
+  const long long slots = (few ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units, splits = std::max(1ll, slots / units);
+  // few rows: one step of each wavefront
+  const long long least = few ? kWaves * 4096 / args.cache.head_dim : 8 * units <= compute_units && most >= 1024 ? 256 : 512;
   long long keys = std::max(least, ((most + splits - 1) / splits + least - 1) / least * least);
-  if (args.rows == kRows && most <= (units >= compute_units ? 4 : 3) * least) keys = most;
+  if (few && most <= (units >= compute_units ? 4 : 3) * least) keys = most;
   args.splits = (int)((most + keys - 1) / keys);
   args.keys_per_split = (int)keys;
 }

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
           const float own_keep = v_exponent.follow(powers[i]);
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) sums[j] *= own_keep;
-          const bool negligible = powers[i] < v_exponent.now;
+          const bool negligible = powers[i] < v_exponent.now - 6;
           const h8_t p = weigh(i, negligible ? (float)v_exponent.now : lane_value(v_log, entry[i]));
           total_p += sum * (negligible ? 0x1p-8f : lane_value(v_inverse, entry[i]) * power_of_two(v_exponent.now - 8));
           sum = 0.f;

@@ -199,7 +199,9 @@ hipError_t launch_norm(const onebit_norm& a, hipStream_t stream) {
                        whole(a.h_out, a.h_out ? a.h_stride : 0) && whole(a.y, a.y_stride) && whole(a.weight, 0) && whole(a.bias, 0) &&
                        whole(a.post_weight, 0) && whole(a.post_bias, 0) && (!a.gate_column_stride || whole(a.gate, a.gate_row_stride));
   const int units = (a.hidden + kVector - 1) / kVector;
-  const int per_thread = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
+  // One vector to a thread is the shortest way for few rows (16 x 4096 3.6 us, with two 4.4). Of many long rows a compute unit then holds one at a time
+  // and waits for it: two vectors, half the wavefronts, and the next row under way (2048 x 8192 with a norm behind the block 51.0 us, with two 40.3).
+  const int per_thread = units <= 1024 && (units < 512 || a.rows < 512) ? 1 : units <= 2048 ? 2 : 4;
   const int threads = ((units + per_thread - 1) / per_thread + 63) / 64 * 64;
   auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3(a.rows), dim3(threads), 0, stream, a); };
   if (per_thread == 1) return vectors ? launch(norm_kernel<1, true>) : launch(norm_kernel<1, false>);

@@ -58,6 +58,16 @@ class Case:
                                       torch.tensor(self.lengths, dtype=torch.int32).cuda(), starts=d(self.starts) if starts else None,
                                       scale=scale, **options)
 
+    def crowd(self, copies, **options):
+        """The call with its sequences `copies` times over, which the launch is planned for; the first ones' rows"""
+        rows = self.q.shape[0]
+        starts = torch.cat([self.starts[:-1] + i * rows for i in range(copies)] + [torch.tensor([copies * rows])]).to(torch.int32)
+        cuda = lambda t: t.cuda()  # noqa: E731
+        out = onebit.cache_attention(cuda(self.q.repeat(copies, 1, 1)), cuda(self.k), cuda(self.v), cuda(self.k_scale), cuda(self.v_scale),
+                                     cuda(self.pages.repeat(copies, 1)), torch.tensor(self.lengths * copies, dtype=torch.int32).cuda(), starts=cuda(starts), **options)
+        assert torch.equal(out[:rows], out[-rows:])
+        return out[:rows]
+
     def want(self, scale=None):
         """(outputs, sum p |v|) in 64 bits"""
         scale = 1 / math.sqrt(self.dim) if scale is None else scale
@@ -167,21 +177,48 @@ def test_attention_ignores_what_a_row_does_not_see(new):
         assert torch.equal(got[:new + 18], clean[:new + 18]) and not bool(torch.isfinite(got[new + 18:]).any())
 
 
-@pytest.mark.parametrize("new", [1, 48])
+@pytest.mark.parametrize("length,new,copies", [(400, 1, 1), (400, 48, 1), (400, 400, 1), (400, 130, 24), (130, 130, 24)])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("decades", [3, 13])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attention_with_scales_far_apart(new, dtype):
-    """Scales of the pages over thirteen decades, some 0: p takes them on without leaving fp16's range"""
-    case = Case([400], [new], 4, 2, 64, 16, E4M3, dtype, seed=3)
+def test_attention_with_scales_far_apart(length, new, copies, block, decades, dtype):
+    """Scales of the pages over some decades, some 0: p takes them on without leaving fp16's range, and a row that sees small ones
+    alone, beside large ones that it does not see, loses nothing"""
+    case = Case([length], [new], 4, 2, 64, block, E4M3, dtype, seed=3)
     g = generator(9)
-    case.v_scale = 10 ** (13 * torch.rand(case.v_scale.shape, generator=g) - 10)
-    case.v_scale[case.pages[0, 3].long()] = 0
-    case.k_scale[case.pages[0, 5].long()] = 0
+    case.v_scale = 10 ** (decades * torch.rand(case.v_scale.shape, generator=g) + 2 - decades)
+    case.v_scale[case.pages[0, 1].long()] = 0
+    case.k_scale[case.pages[0, -1].long()] = 0
     if dtype == torch.float16:
         case.v_scale *= 0.1
-    got = case.call()
-    case.check(got)
-    case.v_scale[:] = 0
-    assert bool((case.call() == 0).all())
+    case.check(case.crowd(copies, max_new=new))
+    case.v_scale = torch.zeros_like(case.v_scale)
+    assert bool((case.crowd(copies, max_new=new) == 0).all())
+
+
+# rows (tokens x heads of a key/value head) of one workgroup and more, enough of them that the kernel of prompts takes them
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("dim,block", [(64, 16), (64, 32), (64, 128), (128, 16), (128, 64), (128, 32)])
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,copies", [([70, 33, 0, 200], [70, 33, 2, 40], 4, 2, 20), ([300], [129], 4, 2, 30), ([129], [1], 40, 1, 300),
+                                                              ([64, 1, 65], [64, 1, 1], 12, 2, 30)])
+def test_attention_of_many_prompts(code, dim, block, lengths, new, heads, kv_heads, copies):
+    case = Case(lengths, new, heads, kv_heads, dim, block, code, torch.float16 if code == E4M3 else torch.bfloat16, seed=block)
+    case.check(case.crowd(copies, max_new=max(new)))
+    if len(lengths) > 1:  # a page that is missing in the middle, NaN where nothing is, and a scale that is not finite behind what most rows see
+        case.pages[0, min(1, case.pages.shape[1] - 1)] = -1
+        last = int(case.pages[3 if len(lengths) > 3 else 2, -(-lengths[-1] // block) - 1])
+        bits(case.v)[last, :, lengths[-1] % block or block:] = 0x7f if code == E4M3 else 0x80
+        case.check(case.crowd(copies, max_new=max(new)))
+        if len(lengths) == 4 and block <= 32:  # the fourth sequence's new tokens are its positions 160 ... 199
+            clean = case.crowd(copies, max_new=max(new))
+            page, first = int(case.pages[3, 192 // block]), 192 - 160
+            case.v_scale[page], case.k_scale[page, 1] = math.nan, math.inf
+            spoilt = onebit.cache_attention(case.q.repeat(copies, 1, 1).cuda(), case.k.cuda(), case.v.cuda(), case.k_scale.cuda(), case.v_scale.cuda(),
+                                            case.pages.repeat(copies, 1).cuda(), torch.tensor(lengths * copies, dtype=torch.int32).cuda(),
+                                            starts=torch.cat([case.starts[:-1] + i * sum(new) for i in range(copies)] + [torch.tensor([copies * sum(new)])]).to(torch.int32).cuda(),
+                                            max_new=max(new))[:sum(new)]
+            seen = sum(new[:3]) + first
+            assert torch.equal(spoilt[:seen], clean[:seen]) and not bool(spoilt[seen:].isfinite().any())
 
 
 @pytest.mark.parametrize("new", [1, 64])
