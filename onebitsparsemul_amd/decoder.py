@@ -3,7 +3,7 @@ paged cache of 8-bit keys and values with the attention that reads it, and the n
 inference, as BinaryLinear_2_4: the results have no gradient. No counterpart in the reference, whose layers stop at the
 projection (onebit_sparse_mul/__init__.py:101-145).
 
-    python -m onebitsparsemul_amd.decoder        # a small decoder, token by token, against one pass over the whole prompt
+onebitsparsemul_amd.decode runs them together.
 """
 import math
 

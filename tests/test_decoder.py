@@ -611,3 +611,21 @@ def test_a_graph_of_a_decoding_step_replays():
         for mine, theirs in zip(outputs, step(eager)):
             assert torch.equal(mine, theirs)
     assert torch.equal(bits(cache.k), bits(eager.k)) and torch.equal(cache.v_scale, eager.v_scale)
+
+
+def test_a_decoder_in_pieces_is_the_decoder_in_one_pass():
+    """Two layers with their one-bit projections. Pieces that end with pages leave the same cache as one pass, up to what the activations' fp16
+    roundings (2^-11, of some ten operators in a row) turn in it: 1 % of the logits' norm at most. Single tokens round the pages that they grow into
+    again, each by at most a code's half step (2^-4 of a value) once the page's largest has grown."""
+    from onebitsparsemul_amd.decode import Decoder
+    ids = torch.randint(0, 4096, (3, 192), generator=generator(7)).cuda()
+    whole, pieces, single = (Decoder(2, 3, 192, block=32) for _ in range(3))
+    want = whole.step(ids.reshape(-1), 192, 192)
+    for begin, end in ((0, 64), (64, 96), (96, 192)):
+        got = pieces.step(ids[:, begin:end].reshape(-1), end - begin, end)
+    assert float((got - want).norm() / want.norm()) < 0.01
+    single.step(ids[:, :160].reshape(-1), 160, 160)
+    for t in range(160, 192):
+        last = single.step(ids[:, t], 1, t + 1)
+    assert float((last - want).norm() / want.norm()) < 2.0**-4
+    assert bool((single.lengths == 192).all())
