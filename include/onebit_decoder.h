@@ -7,7 +7,7 @@
  * All data pointers are DEVICE pointers, the structs themselves are HOST memory, read before the call returns. Work is
  * enqueued on `stream` (hipStream_t as void*, NULL = default stream) and the calls return without synchronising. They allocate
  * nothing, keep nothing between calls, and can be captured in a HIP graph. Status codes, dtype codes and
- * onebit_sparse_last_error() are those of onebit_sparse_tensor.h.
+ * onebit_sparse_last_error() are those of onebit_sparse_tensor.h; a call of more than 2^32 threads is refused as HIP refuses it.
  */
 #ifndef ONEBIT_DECODER_H_
 #define ONEBIT_DECODER_H_
@@ -30,7 +30,7 @@ typedef struct onebit_heads {
 
 /*
  * Keys and values of one layer. Codes: pages x kv_heads x block x head_dim, 16-byte aligned; a token's value is its code
- * times the scale of its page and head (pages x kv_heads, fp32). block: 16, 32, 64 or 128 tokens; head_dim: 64 or 128.
+ * times the scale of its page and head (pages x kv_heads, fp32, not negative). block: 16, 32, 64 or 128 tokens; head_dim: 64 or 128.
  */
 typedef struct onebit_cache {
   void *k, *v;
@@ -43,7 +43,8 @@ typedef struct onebit_cache {
  * The sequences of a call. Tokens [j * block, (j + 1) * block) of sequence s lie in page page_table[s * width + j]; an entry
  * outside of [0, pages) holds none (it is neither written nor attended to). lengths[s] counts the tokens of the sequence WITH
  * the call's new ones, which are its last: rows starts[s] ... starts[s + 1] - 1 of the call's token-major operands, or, with
- * starts NULL, tokens / count rows each. Lengths beyond width * block and starts outside of [0, tokens] are clamped.
+ * starts NULL, tokens / count rows each. Lengths beyond width * block (at most 2^30) and starts outside of [0, tokens] are clamped.
+ * Rows of no sequence are not read; what results hold there is not defined.
  */
 typedef struct onebit_sequences {
   const int *page_table; /* count x width */
@@ -51,7 +52,7 @@ typedef struct onebit_sequences {
   const int *starts;     /* count + 1, or NULL */
   int count, width;
   int tokens;     /* rows of the token-major operands */
-  int max_new;    /* no sequence has more new tokens */
+  int max_new;    /* no sequence has more new tokens (an append leaves out what is beyond) */
   int max_length; /* what the launch is planned for; longer sequences are right and slower. 0: width * block */
 } onebit_sequences;
 

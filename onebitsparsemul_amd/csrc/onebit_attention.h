@@ -83,7 +83,6 @@ struct Exponent {
   }
 };
 
-__device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 __device__ inline float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 
 // Eight values of a row of q: the largest magnitude, and as fp16 times `factor` (a power of two; not used on fp16)

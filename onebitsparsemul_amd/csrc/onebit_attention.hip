@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
         for (int j = 0; j < D / 16; ++j) sums[j] *= keep * v_keep;
       }
       const float base = most == -INFINITY ? 0.f : most, v_factor = power_of_two(14 - v_exponent.now);
-      h8_t p_high[kTiles / 2], p_low[kTiles / 2];  // together 22 bits of p: the eight rows that fp16 alone would cost are there anyway
+      h8_t p_high[kTiles / 2], p_low[kTiles / 2];  // together 22 bits of p: the products wait for the codes, a second one is hidden
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         const float factor = own_v[t] * v_factor;
@@ -383,7 +383,9 @@ void plan_attention(AttentionArgs& args, int compute_units) {
   args.rows = few ? kRows : many_rows(args.cache.head_dim);
   const long long units = workgroups(args.rows);
   // workgroups that the device holds
-  const long long slots = (few ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units, splits = std::max(1ll, slots / units);
+  const long long slots = (few ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units;
+  // (the join has a workgroup of up to 1024 threads to each row, and a launch less than 2^32 of them)
+  const long long splits = (long long)q.tokens * args.heads < 1 << 22 ? std::max(1ll, slots / units) : 1;
   // few rows: one step of each wavefront
   const long long least = few ? kWaves * 4096 / args.cache.head_dim : 8 * units <= compute_units && most >= 1024 ? 256 : 512;
   long long keys = std::max(least, ((most + splits - 1) / splits + least - 1) / least * least);

@@ -256,11 +256,11 @@ hipError_t launch_append_as(AppendArgs args, hipStream_t stream) {
   const onebit_sequences& q = args.sequences;
   const int most = q.max_new, in_page = std::min(most, args.cache.block) * units;
   args.slots = (most + args.cache.block - 2) / args.cache.block + 1;
-  const int page_tasks = args.slots * 2 * args.cache.kv_heads;
+  const long long page_tasks = 2ll * args.slots * args.cache.kv_heads;
   auto launch = [&](auto kernel, int threads) {
-    const long long turned = (long long)most * args.heads * units;
-    const dim3 grid(page_tasks + (unsigned)((turned + threads - 1) / threads), q.count);
-    return launch_kernel(kernel, grid, dim3(threads), 0, stream, args, page_tasks);
+    const long long turned = (long long)most * args.heads * units, tasks = page_tasks + (turned + threads - 1) / threads;
+    if (tasks * threads >= 1ll << 32) return hipErrorInvalidConfiguration;
+    return launch_kernel(kernel, dim3((unsigned)tasks, q.count), dim3(threads), 0, stream, args, (int)page_tasks);
   };
   if (in_page <= 64) return launch(append_kernel<TYPE, CODE, 64, 1>, 64);
   if (in_page <= 256) return launch(append_kernel<TYPE, CODE, 256, 1>, 256);

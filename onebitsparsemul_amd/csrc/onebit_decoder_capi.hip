@@ -36,7 +36,7 @@ int check_cache(const onebit_cache* c) {
 int check_sequences(const onebit_sequences* q, int block) {
   if (!q || !q->page_table || !q->lengths) return refuse("null pointer in the sequences");
   if (q->count < 1 || q->count > 65535 || q->width < 1) return refuse("1 to 65535 sequences and a page table of some width (got %d, %d)", q->count, q->width);
-  if ((long long)q->width * block >= 1ll << 31) return refuse("%d pages of %d tokens to a sequence exceed the int range", q->width, block);
+  if ((long long)q->width * block > 1ll << 30) return refuse("%d pages of %d tokens to a sequence exceed the int range that positions have: 2^30 tokens", q->width, block);
   if (q->tokens < 1 || q->max_new < 1 || q->max_length < 0) return refuse("tokens and max_new must be positive (got %d, %d)", q->tokens, q->max_new);
   if (!q->starts && q->tokens % q->count) return refuse("%d tokens do not divide into %d sequences: pass starts", q->tokens, q->count);
   return ONEBIT_OK;

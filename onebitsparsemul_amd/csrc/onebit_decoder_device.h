@@ -27,8 +27,6 @@ struct Stored<ONEBIT_DTYPE_F16> { typedef _Float16 type; };
 template <>
 struct Stored<ONEBIT_DTYPE_BF16> { typedef __bf16 type; };
 
-inline int bytes_of(int type) { return type == ONEBIT_DTYPE_F32 ? 4 : 2; }
-
 // N consecutive values (16-byte aligned where N is 8) as fp32, and back, rounded to nearest even
 template <int TYPE, int N>
 __device__ inline void load_values(const void* base, long long at, float (&x)[N]) {

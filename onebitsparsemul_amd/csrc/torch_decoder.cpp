@@ -4,6 +4,8 @@
 
 #include "onebit_decoder.h"
 
+#include <ATen/MemoryOverlap.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -94,6 +96,7 @@ torch::Tensor rotary(const torch::Tensor& x, const torch::Tensor& positions, con
   const Turning turning = turning_of(table, device);
   if (out.has_value()) {
     check_heads(*out, "out", device);
+    at::assert_no_internal_overlap(*out);
     TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->stride(2) == 1 && !out->is_neg(),
                       "out must have x's shape and type and whole heads");
   }
@@ -159,6 +162,7 @@ torch::Tensor cache_attention(const torch::Tensor& q, const torch::Tensor& k_cac
   const onebit_sequences sequences = sequences_of(pages, lengths, starts, tokens, max_new, max_length, device);
   if (out.has_value()) {
     check_heads(*out, "out", device);
+    at::assert_no_internal_overlap(*out);
     TORCH_CHECK_VALUE(out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && in_vectors(*out),
                       "out must have q's shape and type and be 16-byte aligned, with strides that are multiples of eight");
   }

@@ -73,11 +73,11 @@ def rotary(x, positions, table, interleaved=False, out=None):
 
 def cache_append(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, starts=None, q=None, rotary=None, interleaved=False, max_new=None):
     """Writes the new tokens' keys and values, (tokens, kv_heads, head_dim) each, into the 8-bit cache: codes (pages, kv_heads, block,
-    head_dim) of type float8_e4m3fn or int8 and scales (pages, kv_heads), a value being its code times the scale of its page and head.
+    head_dim) of type float8_e4m3fn or int8 and scales (pages, kv_heads), not negative, a value being its code times the scale of its page and head.
     pages (sequences, width) int32: the page of each `block` tokens of a sequence; lengths (sequences,) int32: tokens WITH the
     new ones; starts (sequences + 1,) int32: where a sequence's new tokens begin in k and v (None: equally many each); max_new: no
     sequence has more (host number; spares the launch a grid for all tokens in one sequence). With a rotary table keys are
-    turned by their positions, and so are the queries q; returns them turned (None without q). A page's scale only grows while
+    turned by their positions, and so are the queries q; returns them turned (None without q; rows of no sequence hold anything). A page's scale only grows while
     tokens are added to it; where it does, its older codes are rounded again. NaN and infinities make their page's scale such."""
     return _binding().cache_append(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, starts, q, rotary, interleaved, max_new)
 

@@ -59,7 +59,8 @@ def attention(lib, cache=(), sequences=(), heads=8, dtype=1, q=A, stride=1024, w
     (dict(cache=dict(v=A + 8)), "16-byte aligned"), (dict(cache=dict(block=48)), "block = 48"), (dict(cache=dict(head_dim=96)), "head_dim = 96"),
     (dict(cache=dict(pages=0)), "pages"), (dict(cache=dict(code=2)), "code must be"), (dict(sequences=dict(lengths=None)), "null pointer in the sequences"),
     (dict(sequences=dict(count=0)), "sequences"), (dict(sequences=dict(count=70000, tokens=70000)), "65535"), (dict(sequences=dict(tokens=0)), "positive"),
-    (dict(sequences=dict(tokens=5)), "do not divide"), (dict(sequences=dict(width=1 << 25)), "int range"), (dict(heads=7), "multiple of kv_heads"),
+    (dict(sequences=dict(tokens=5)), "do not divide"), (dict(sequences=dict(width=1 << 25)), "int range"),
+    (dict(sequences=dict(width=(1 << 24) + 1)), "2^30 tokens"), (dict(heads=7), "multiple of kv_heads"),
     (dict(heads=0), "multiple of kv_heads"), (dict(dtype=0), "dtype code"), (dict(dtype=3), "dtype code"), (dict(q=A + 2), "q must be 16-byte aligned"),
     (dict(q=None), "must not be null"), (dict(stride=1025), "multiples of eight"),
     (dict(sequences=dict(width=4096)), "needs a workspace of"), (dict(sequences=dict(width=4096), workspace=A + 4), "needs a workspace of"),
@@ -75,6 +76,9 @@ def test_workspace_follows_the_split(lib):
     assert lib.onebit_cache_attention_workspace(ctypes.byref(cache), ctypes.byref(short), 8) == 0
     bytes_ = lib.onebit_cache_attention_workspace(ctypes.byref(cache), ctypes.byref(long), 8)
     assert bytes_ > 0 and bytes_ % (4 * 8 * 130 * 4) == 0  # splits of 4 tokens x 8 heads x (128 sums, maximum, sum)
+    # rows that would be more than a launch of the join has threads for go unsplit
+    crowd = Sequences(**{**GOOD_SEQUENCES, "width": 4096, "tokens": 1 << 19, "max_new": 1, "starts": A})
+    assert lib.onebit_cache_attention_workspace(ctypes.byref(cache), ctypes.byref(crowd), 8) == 0 and _native.last_error() == ""
     assert lib.onebit_cache_attention_workspace(None, ctypes.byref(long), 8) == 0 and "cache" in _native.last_error()
 
 
@@ -178,6 +182,8 @@ def test_the_binding_refuses():
         (TypeError, "pages must be", lambda: cache.attend(q, pages.long(), lengths)), (ValueError, "one entry for each", lambda: cache.attend(q, pages, lengths[:2])),
         (ValueError, "starts must have", lambda: cache.attend(q, pages, lengths, starts=lengths)), (ValueError, "max_new", lambda: cache.attend(q, pages, lengths, max_new=0)),
         (RuntimeError, "multiple of kv_heads", lambda: cache.attend(q[:, :3], pages, lengths)), (ValueError, "out must have", lambda: cache.attend(q, pages, lengths, out=q[..., ::2])),
+        (RuntimeError, "single memory location", lambda: cache.attend(q, pages, lengths, out=q[:1].expand(3, 4, 64))),
+        (RuntimeError, "single memory location", lambda: onebit.rotary(x, lengths, table, out=x[:, :1].expand(3, 2, 64))),
         (RuntimeError, "do not divide", lambda: cache.attend(q[:2], pages, lengths)), (ValueError, "must live on", lambda: cache.attend(q, pages.cpu(), lengths)),
         (ValueError, "one shape and type", lambda: cache.append(x, x[:2], pages, lengths)), (ValueError, "for this cache", lambda: cache.append(q, q, pages, lengths)),
         (ValueError, "needs a rotary table", lambda: cache.append(x, x, pages, lengths, q=q)), (ValueError, "k's tokens", lambda: cache.append(x, x, pages, lengths, q=q.float(), rotary=table)),
