@@ -27,7 +27,7 @@ struct Stored<ONEBIT_DTYPE_F16> { typedef _Float16 type; };
 template <>
 struct Stored<ONEBIT_DTYPE_BF16> { typedef __bf16 type; };
 
-// N consecutive values (16-byte aligned where N is 8) as fp32, and back, rounded to nearest even
+// N consecutive values (16-byte aligned where N is 8) as fp32, and back, rounded to nearest even; FAR: past the caches
 template <int TYPE, int N>
 __device__ inline void load_values(const void* base, long long at, float (&x)[N]) {
   typedef typename Stored<TYPE>::type T;
@@ -40,7 +40,7 @@ __device__ inline void load_values(const void* base, long long at, float (&x)[N]
     for (int i = 0; i < N; ++i) x[i] = (float)v[i];
   }
 }
-template <int TYPE, int N>
+template <int TYPE, int N, bool FAR = false>
 __device__ inline void store_values(void* base, long long at, const float (&x)[N]) {
   typedef typename Stored<TYPE>::type T;
   typedef T vector __attribute__((ext_vector_type(N)));
@@ -50,7 +50,8 @@ __device__ inline void store_values(void* base, long long at, const float (&x)[N
     vector v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    *(vector*)((T*)base + at) = v;
+    if constexpr (FAR) __builtin_nontemporal_store(v, (vector*)((T*)base + at));
+    else *(vector*)((T*)base + at) = v;
   }
 }
 

@@ -48,12 +48,12 @@ __device__ inline void widen(const Raw& raw, int type, float (&x)[kVector]) {
     for (int i = 0; i < kVector; ++i) x[i] = __uint_as_float(i % 2 ? raw.low[i / 2] & 0xffff0000u : raw.low[i / 2] << 16);
   }
 }
-template <bool WHOLE>
+template <bool WHOLE, bool FAR>
 __device__ inline void store_row(void* base, int type, long long at, int count, const float (&x)[kVector]) {
   if (WHOLE) {
-    if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, kVector>(base, at, x);
-    else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, kVector>(base, at, x);
-    else store_values<ONEBIT_DTYPE_BF16, kVector>(base, at, x);
+    if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, kVector, FAR>(base, at, x);
+    else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, kVector, FAR>(base, at, x);
+    else store_values<ONEBIT_DTYPE_BF16, kVector, FAR>(base, at, x);
   } else {
 #pragma unroll
     for (int i = 0; i < kVector; ++i) {
@@ -108,8 +108,8 @@ __device__ inline void normalise(float (&x)[VECTORS][kVector], const onebit_norm
     for (int i = 0; i < kVector; ++i) x[v][i] *= factor;
 }
 
-// WHOLE: every vector is eight values at a multiple of 16 bytes.
-template <int VECTORS, bool WHOLE>
+// WHOLE: every vector is eight values at a multiple of 16 bytes. FAR: h goes past the caches.
+template <int VECTORS, bool WHOLE, bool FAR>
 __global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
   __shared__ float parts[16];
   const long long row = blockIdx.x;
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
     widen(residual[v], a.residual_dtype, other);
 #pragma unroll
     for (int i = 0; i < kVector; ++i) h[v][i] = (WHOLE || i < left[v]) ? a.residual_scale * other[i] + (a.x ? a.block_scale * h[v][i] : 0.f) : 0.f;
-    if (a.h_out) store_row<WHOLE>(a.h_out, a.residual_dtype, row * a.h_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
+    if (a.h_out) store_row<WHOLE, FAR>(a.h_out, a.residual_dtype, row * a.h_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
   }
   normalise(h, a, parts);
 #pragma unroll
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
 #pragma unroll
       for (int i = 0; i < kVector; ++i) h[v][i] += w[i];
     }
-    store_row<WHOLE>(a.y, a.y_dtype, row * a.y_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
+    store_row<WHOLE, false>(a.y, a.y_dtype, row * a.y_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
   }
 }
 
@@ -203,10 +203,18 @@ hipError_t launch_norm(const onebit_norm& a, hipStream_t stream) {
   // and waits for it: two vectors, half the wavefronts, and the next row under way (2048 x 8192 with a norm behind the block 51.0 us, with two 40.3).
   const int per_thread = units <= 1024 && (units < 512 || a.rows < 512) ? 1 : units <= 2048 ? 2 : 4;
   const int threads = ((units + per_thread - 1) / per_thread + 63) / 64 * 64;
+  // h is read again by the next norm, with at least a projection between: of a quarter of the 256 MB of the last cache on it is written past the caches,
+  // which leaves them to y (2048 x 8192, h fp32: 39.2 us for 46.3, and with the projections behind two such norms within 2 % either way;
+  // 8192 x 4096 fp16 with them 319 for 324; y too past them: 40.3, and 1 to 2 % lost in what reads it; h of 16 rows: 0.6 of 14.8 us lost).
+  const bool far = vectors && a.h_out && (long long)a.rows * a.hidden * (a.residual_dtype == ONEBIT_DTYPE_F32 ? 4 : 2) >= 64 << 20;
   auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3(a.rows), dim3(threads), 0, stream, a); };
-  if (per_thread == 1) return vectors ? launch(norm_kernel<1, true>) : launch(norm_kernel<1, false>);
-  if (per_thread == 2) return vectors ? launch(norm_kernel<2, true>) : launch(norm_kernel<2, false>);
-  return vectors ? launch(norm_kernel<4, true>) : launch(norm_kernel<4, false>);
+  auto launch_as = [&](auto count) {
+    constexpr int kVectors = decltype(count)::value;
+    return far ? launch(norm_kernel<kVectors, true, true>) : vectors ? launch(norm_kernel<kVectors, true, false>) : launch(norm_kernel<kVectors, false, false>);
+  };
+  if (per_thread == 1) return launch_as(std::integral_constant<int, 1>());
+  if (per_thread == 2) return launch_as(std::integral_constant<int, 2>());
+  return launch_as(std::integral_constant<int, 4>());
 }
 
 }  // namespace onebit

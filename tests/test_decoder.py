@@ -571,6 +571,23 @@ def test_block_norm_views_shapes_and_in_place():
     assert onebit.block_norm(x[:0], residual[:0], weight)[1].shape == (0, 5, 512)
 
 
+@pytest.mark.parametrize("rows,hidden", [(32768, 512), (2048, 8192), (1000, 24000)])
+def test_block_norm_of_many_rows_is_that_of_few(rows, hidden):
+    """A residual of 64 MB and more is stored in another way: the same values, in place too"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x = torch.randn((rows, hidden), generator=g, device="cuda").bfloat16()
+    residual = torch.randn((rows, hidden), generator=g, device="cuda")
+    weight = torch.randn(hidden, generator=g, device="cuda")
+    h, y = onebit.block_norm(x, residual, weight, post_weight=weight)
+    for first in range(0, rows - 512 + 1, rows // 2 - 256 if rows <= 2048 else 8192):
+        part = slice(first, first + 512)
+        few_h, few_y = onebit.block_norm(x[part], residual[part], weight, post_weight=weight)
+        assert torch.equal(h[part], few_h) and torch.equal(y[part], few_y)
+    _, again = onebit.block_norm(x, residual, weight, post_weight=weight, residual_out=residual)
+    assert torch.equal(residual, h) and torch.equal(again, y)
+
+
 # ---- together
 
 
