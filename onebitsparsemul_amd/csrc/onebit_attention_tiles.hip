@@ -1,8 +1,17 @@
 // Attention over the 8-bit cache (onebit_decoder.h) for many rows of q to a key/value head: prompts.
 //
-// A workgroup takes 256 rows (128 where heads are of 64; tokens x heads of the key/value head), 32 to a wavefront, and walks over the keys in tiles of 64. Each tile's
-// codes are read once, turned into fp16 by the wavefronts together, and lie in LDS twice (one tile in use, one being written): keys by rows of
-// dims, values by rows of keys, so that both matrix products (32x32x16, fp16) read their left operand with one 16-byte load a lane.
+// A workgroup takes 256 rows (128 where heads are of 64; tokens x heads of the key/value head), 32 to a wavefront, and walks over the keys in tiles
+// of 64. Each tile's codes are read once, turned into fp16 by the wavefronts together, and lie in LDS twice (one tile in use, one being written): keys
+// by rows of dims, values by rows of keys, so that both matrix products (32x32x16, fp16) read their left operand with one 16-byte load a lane.
+//
+// What bounds it: the matrix unit and the vector unit one after the other. Of a tile's 32 products a wavefront (1024 clocks) and some 200 vector
+// instructions (32 exponentials among them; 16 conversions and 8 byte permutations bring in its share of the next tile) the two wavefronts of a SIMD
+// overlap little: the matrix unit is busy in 36 % of the clocks, LDS in 27 %, and power takes 6 % (139 us on zeros). 4096 tokens, 32 heads of 128 on 8,
+// e4m3, bf16: 149 us = 920 TFLOP/s of the causal half, where a large bf16 matrix product of the library reaches 1330; 500 tokens behind 7500, 32 heads on 32,
+// int8, pages of 32: 97 us with 9 of the join = 650.
+// Why this tile: 128 rows (four wavefronts) read and convert each tile twice as often, 167 us; 64 rows to a wavefront do not fit its registers. Measured and
+// not kept: the wavefronts of a SIMD in turn, one multiplying while the other weighs, with a barrier at each change (148 us, the second call 100:
+// each is then bound by its own instructions' latencies); the loads two tiles ahead, 167; wave priorities, nothing.
 #include "onebit_attention.h"
 
 #include <type_traits>
@@ -14,11 +23,17 @@ typedef float f16x_t __attribute__((ext_vector_type(16)));
 constexpr int kTile = 64;  // keys
 constexpr int kSchedProduct = 0x8, kSchedRead = 0x100;  // kinds of instructions for the scheduler
 
-// Where the 16-byte piece `piece` of a row lies: moved within its row, so that eight neighbouring rows' pieces fall on different banks, and rows
-// eight apart do too (the values' writes). The piece takes part by exclusive or: other pieces of a row are one such operation away.
+// Where 16-byte pieces lie: moved within their rows by an exclusive or (other pieces of a row are one such operation away), so that the sixteen lanes that
+// LDS serves at a time fall on different banks: keys' rows (tokens) in reads of one piece of sixteen rows, and in writes of whole rows.
 template <int PIECES>
-__device__ inline int place(int row, int piece) {
-  return row * PIECES + (piece ^ (PIECES == 16 ? row & 15 : (row >> 1 & 3) ^ (row >> 3 & 7)));
+__device__ inline int key_place(int row, int piece) {
+  return row * PIECES + (piece ^ (PIECES == 16 ? row & 15 : row >> 1 & 7));
+}
+// The values' rows (dims, of eight pieces) are read as the keys', but written at every fourth row by neighbouring lanes: bits 0 and 2 of the row are exchanged.
+// 32 rows further on the piece moves by 2.
+__device__ inline int value_place(int row, int piece) {
+  const int r = (row & ~5) | (row >> 2 & 1) | (row & 1) << 2;
+  return r * 8 + (piece ^ (r >> 1 & 7) ^ (r >> 4 & 3));
 }
 // The same value, for which the compiler keeps no register with what a loop makes of it
 __device__ inline int made_here(int x) {
@@ -32,7 +47,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
   constexpr int kOwn = kTile / kWaves;  // keys a wavefront brings in
   constexpr int kKeyBytes = kOwn * D / 64, kValueBytes = D * kOwn / 256;
   typedef uint32_t key_words __attribute__((ext_vector_type(kKeyBytes / 4)));
-  typedef uint32_t value_words __attribute__((ext_vector_type(kValueBytes / 4)));
+  static_assert(kValueBytes == 4, "a lane takes four dims of four keys");
   __shared__ __align__(16) h8_t keys[2][kTile * D / 8];
   __shared__ __align__(16) h8_t values[2][kTile * D / 8];
   const onebit_cache& cache = args.cache;
@@ -109,7 +124,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
 
     // the wavefront's share of a tile: kOwn keys, in one page
     key_words raw_k;
-    value_words raw_v[4];
+    uint32_t raw_v[4];
     auto load = [&](int key) {
       const int own = key + wave * kOwn, entry = min((own >> block_bits) - window.first, 63);
       const int page = __builtin_amdgcn_readlane(window.page, entry);
@@ -120,7 +135,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
       const int first = lane / kLanes * 4;
       const uint8_t* const v = (const uint8_t*)cache.v + at + first * D + lane % kLanes * kValueBytes;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raw_v[i] = *(const value_words*)(v + i * D);
+      for (int i = 0; i < 4; ++i) raw_v[i] = *(const uint32_t*)(v + i * D);
       if (valid < kOwn) {  // codes of keys that are not there may be NaN, which a p of 0 would not hide
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -130,35 +145,32 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
     auto put = [&](auto buffer) {
       constexpr int to = decltype(buffer)::value;
       constexpr int kKeyLanes = D / kKeyBytes, kLanes = D / kValueBytes;
-      const int key_at = made_here(place<D / 8>(wave * kOwn + lane / kKeyLanes, lane % kKeyLanes * (kKeyBytes / 8)));
+      const int key_at = made_here(key_place<D / 8>(wave * kOwn + lane / kKeyLanes, lane % kKeyLanes * (kKeyBytes / 8)));
 #pragma unroll
       for (int i = 0; i < kKeyBytes / 8; ++i) keys[to][key_at ^ i] = codes_to_f16<CODE>(raw_k[2 * i], raw_k[2 * i + 1]);
       // four keys are half a piece of each dim's row; pieces are in the order in which the products want them
       const int group = (wave * kOwn + lane / kLanes * 4) / 4, half = group >> 1 & 1;
-      const int value_at = made_here(place<8>(lane % kLanes * kValueBytes, (group >> 2) * 2 + (group & 1)));
+      const int value_at = made_here(value_place(lane % kLanes * kValueBytes, (group >> 2) * 2 + (group & 1)));
+uint32_t by_dim[4];
+      transpose_bytes(raw_v[0], raw_v[1], raw_v[2], raw_v[3], by_dim);
 #pragma unroll
-      for (int w = 0; w < kValueBytes / 4; ++w) {
-        uint32_t by_dim[4];
-        transpose_bytes(raw_v[0][w], raw_v[1][w], raw_v[2][w], raw_v[3][w], by_dim);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h2_t a, b;
-          codes_to_f16<CODE>(by_dim[i], a, b);
-          ((h4_t*)&values[to][(value_at ^ (4 * w + i) >> 1) + (4 * w + i) * 8])[half] = h4_t{a.x, a.y, b.x, b.y};
-        }
+      for (int i = 0; i < 4; ++i) {  // the row's bits 0 and 1 in value_place()
+        h2_t a, b;
+        codes_to_f16<CODE>(by_dim[i], a, b);
+        ((h4_t*)&values[to][(value_at ^ (i >> 1 | (i & 1) << 1)) + ((i & 2) + (i & 1) * 4) * 8])[half] = h4_t{a.x, a.y, b.x, b.y};
       }
     };
 
     auto multiply = [&](auto buffer, int key) {
       constexpr int kFrom = decltype(buffer)::value;
       f16x_t scores[2] = {};
-      const int own_key = made_here(place<D / 8>(r, h)), own_value = made_here(place<8>(r, h));
+      const int own_key = made_here(key_place<D / 8>(r, h)), own_value = made_here(value_place(r, h));
       constexpr int kAhead = 6;  // LDS reads in front of the first product: their latency is that of several
 #pragma unroll
       for (int c = 0; c < D / 16; ++c)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-          scores[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[kFrom][32 * (D / 8) * half + (own_key ^ 2 * c ^ (D == 64 ? 4 * half : 0))], q[c], scores[half], 0, 0, 0);
+          scores[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[kFrom][32 * (D / 8) * half + (own_key ^ 2 * c)], q[c], scores[half], 0, 0, 0);
       __builtin_amdgcn_sched_group_barrier(kSchedRead, kAhead, 0);
 #pragma unroll
       for (int i = 0; i < D / 8 - kAhead; ++i) {
@@ -229,8 +241,8 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
         for (int j = 0; j < D / 32; ++j) sums[j] *= keep * v_keep;
       }
       const float base = most == -INFINITY ? 0.f : most;
-      // rows 32 j + r of the values, pieces 2 i + h: place() moves a row's pieces by 4 with every 32 rows
-      auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 4 * (j & 1))]; };
+      // rows 32 j + r of the values, pieces 2 i + h
+      auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 2 * (j & 1))]; };
       const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
       float sum = 0.f;
       // p of 16 keys, with v_scale as a part of the exponent
