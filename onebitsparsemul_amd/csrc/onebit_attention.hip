@@ -1,5 +1,13 @@
 // Attention over the 8-bit cache (onebit_decoder.h) for a few rows of q to a key/value head: sixteen rows (tokens x heads of the key/value
 // head) to a workgroup, whose wavefronts share its keys out and each keep a running maximum, sum and output of their own.
+//
+// What bounds it: memory where sequences are long, and the chain of loads in front (lengths and pages, scales, codes) where they are not. One token behind
+// 131072, 32 heads of 128 on 8, int8: 54 us for 269 MB = 4.9 TB/s (a large copy reaches 5.1), with the join 59. Sixteen sequences of 500 to 4096
+// tokens: 19 us for 69 MB = 3.6 TB/s, the join 3 to 4; the matrix unit is busy in 5 % of the clocks, wavefronts wait for loads in half of theirs. One token
+// behind 1000, heads of 64: 5.5 us and the join 2 to 3, nearly all of it that chain and the two launches.
+// Why this split: sixteen rows are the columns of a matrix instruction; columns that few heads leave empty cost nothing beside the loads. Four wavefronts, each
+// with the next step's codes asked for as soon as this step's registers are free, keep enough bytes under way with three workgroups to a compute unit
+// (one step at a time and one wavefront: 78 us for the long sequence, 38 for the sixteen).
 #include "onebit_attention.h"
 
 #include <algorithm>
@@ -370,16 +378,20 @@ hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
 // Rows of q to a workgroup, and how its keys are split over workgroups where a call has fewer of them than the device holds at once.
 //
 // few_rows_kernel reads the keys for every 16 rows again but starts and ends quickly and fills the device with few rows; many_rows_kernel does
-// with a quarter of the work. Both sides of the rule, head_dim 64 | 128: one prompt of 512 tokens (8 heads on 4: 256 workgroups) 6.8 | 8.7 us with the
-// first, 13.4 | 21.5 with the second; 8 prompts of 128 (32 heads on 8: 2048 workgroups) 14.8 | 19.7 and 7.8 | 13.3; 64 tokens behind 20000 (32 heads on 8: 128
-// workgroups, but 2.5 million keys for them) 47 | 69 and 34 | 41.
+// with a quarter of the work. Both sides of the rule, few | many, us: one prompt of 512, 8 heads of 64 on 4 (256 workgroups) 6.8 | 13.7; one of 1024, 8 of 128 on 4
+// (512) 17.9 | 26.3; one of 512, 32 of 128 on 8 (1024) 19.5 | 23.0; eight of 128, 16 of 64 on 16 (1024, but of 64 keys) 10.2 | 7.4; two of 512, 32 of 64 on 8 (2048)
+// 21.2 | 14.4; 64 tokens behind 1936 in four sequences, 16 of 128 on 16 (256, 65 million values) 30.1 | 22.0; five of 37 to 512, 8 of 64 on 4 (1280, of which
+// 756 have rows) 12.4 | 14.7.
 // A split costs its join, some 3 us: few rows go unsplit up to three steps (500 keys, heads of 64: 6.5 us, 7.8 in two splits), four where the device is full.
 void plan_attention(AttentionArgs& args, int compute_units) {
   const onebit_sequences& q = args.sequences;
   const long long rows = (long long)q.max_new * args.group, room = (long long)q.width * args.cache.block;
   const long long most = std::max(1ll, q.max_length > 0 ? std::min(room, (long long)q.max_length) : room);
   auto workgroups = [&](int of) { return (rows + of - 1) / of * args.cache.kv_heads * q.count; };
-  const bool few = rows <= 32 || (workgroups(kRows) <= 3ll * compute_units && workgroups(kRows) * most * args.cache.head_dim <= 148000ll * compute_units);
+  // that have rows, and the keys that one sees: half of its own tokens are behind it
+  const long long busy = std::min(workgroups(kRows), ((long long)q.tokens * args.group / kRows + q.count) * args.cache.kv_heads);
+  const long long keys_seen = most - std::min<long long>(q.max_new, most) / 2;
+  const bool few = rows <= 32 || (busy <= (keys_seen >= 256 ? 4ll : 3ll) * compute_units && busy * keys_seen * args.cache.head_dim <= 148000ll * compute_units);
   args.rows = few ? kRows : many_rows(args.cache.head_dim);
   const long long units = workgroups(args.rows);
   // workgroups that the device holds

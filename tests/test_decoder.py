@@ -177,7 +177,7 @@ def test_attention_ignores_what_a_row_does_not_see(new):
         assert torch.equal(got[:new + 18], clean[:new + 18]) and not bool(torch.isfinite(got[new + 18:]).any())
 
 
-@pytest.mark.parametrize("length,new,copies", [(400, 1, 1), (400, 48, 1), (400, 400, 1), (400, 130, 24), (130, 130, 24)])
+@pytest.mark.parametrize("length,new,copies", [(400, 1, 1), (400, 48, 1), (400, 400, 1), (400, 130, 24), (400, 130, 36), (130, 130, 24)])
 @pytest.mark.parametrize("block", [16, 32, 64])
 @pytest.mark.parametrize("decades", [3, 13])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -200,7 +200,7 @@ def test_attention_with_scales_far_apart(length, new, copies, block, decades, dt
 @pytest.mark.parametrize("code", [E4M3, INT8])
 @pytest.mark.parametrize("dim,block", [(64, 16), (64, 32), (64, 128), (128, 16), (128, 64), (128, 32)])
 @pytest.mark.parametrize("lengths,new,heads,kv_heads,copies", [([70, 33, 0, 200], [70, 33, 2, 40], 4, 2, 20), ([300], [129], 4, 2, 30), ([129], [1], 40, 1, 300),
-                                                              ([64, 1, 65], [64, 1, 1], 12, 2, 30)])
+                                                              ([64, 1, 65], [64, 1, 1], 12, 2, 30), ([300], [129], 4, 2, 40), ([129], [1], 40, 1, 400)])
 def test_attention_of_many_prompts(code, dim, block, lengths, new, heads, kv_heads, copies):
     case = Case(lengths, new, heads, kv_heads, dim, block, code, torch.float16 if code == E4M3 else torch.bfloat16, seed=block)
     case.check(case.crowd(copies, max_new=max(new)))
