@@ -15,14 +15,14 @@
 namespace onebit {
 namespace {
 
-constexpr int kRows = 16, kWaves = 4;
+constexpr int kRows = 16, kWaves = 4;  // wavefronts of a workgroup: kWaves, or twice as many
 
-template <int D, int CODE>
-__global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs args, int row_tiles) {
+template <int D, int CODE, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, WAVES == kWaves ? 3 : 2) void few_rows_kernel(AttentionArgs args, int row_tiles) {
   // a step: as many tiles of 16 keys as 2 KiB of keys are, each two of them the K of an fp16 matrix instruction
   constexpr int kTiles = 256 / D, kChunk = 16 * kTiles;
   constexpr int kStride = D + 4;  // floats of a row of sums in LDS
-  __shared__ __align__(16) float shared[kWaves * kRows * (kStride + 2)];
+  __shared__ __align__(16) float shared[WAVES * kRows * (kStride + 2)];
   typedef uint32_t value_words __attribute__((ext_vector_type(D / 64)));
   const onebit_cache& cache = args.cache;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
     const int total = max(seq.length - seq.fresh + last_token + 1, 0);
     const int all_see = tile * kRows + kRows <= rows ? max(seq.length - seq.fresh + own_first.token + 1, 0) : 0;
     const int high = split == args.splits - 1 ? total : min(total, low + args.keys_per_split);
-    const int chunks = max(high - low + kChunk - 1, 0) / kChunk, per_wave = (chunks + kWaves - 1) / kWaves;
+    const int chunks = max(high - low + kChunk - 1, 0) / kChunk, per_wave = (chunks + WAVES - 1) / WAVES;
     const int first = low + min(wave * per_wave, chunks) * kChunk, end = min(low + min((wave + 1) * per_wave, chunks) * kChunk, high);
 
     u4_t raw[D / 64][2] = {};
@@ -225,14 +225,14 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
     }
 
     // the wavefronts' sums in the largest of their maxima, one behind the other, then added in their order
-    float* const tops = shared + kWaves * kRows * kStride;
-    float* const totals = tops + kWaves * kRows;
+    float* const tops = shared + WAVES * kRows * kStride;
+    float* const totals = tops + WAVES * kRows;
     total_p = sum_over_16(total_p);
     if (g == 0) tops[wave * kRows + r] = most;
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w * kRows + r]);
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w * kRows + r]);
     // (NaN goes on: a maximum that is none has no keys, or a NaN in its sum)
     const float share = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(most - top), v_factor = power_of_two(v_exponent.now - 14);
     if (row < rows) {
@@ -246,12 +246,12 @@ __global__ __launch_bounds__(kWaves * 64, 3) void few_rows_kernel(AttentionArgs 
     }
     __syncthreads();
     const int here = min(rows - tile * kRows, kRows);
-    for (int item = threadIdx.x; item < here * (D / 4); item += kWaves * 64) {
+    for (int item = threadIdx.x; item < here * (D / 4); item += WAVES * 64) {
       const int column = item / (D / 4), dim = item % (D / 4) * 4;
       float sum = 0.f, top = -INFINITY;
       f4_t out = {};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         sum += totals[w * kRows + column];
         top = fmaxf(top, tops[w * kRows + column]);
         out += *(const f4_t*)(shared + (w * kRows + column) * kStride + dim);
@@ -358,7 +358,8 @@ hipError_t launch_few_rows(const AttentionArgs& args, hipStream_t stream) {
   const onebit_sequences& q = args.sequences;
   const int row_tiles = (int)(((long long)q.max_new * args.group + kRows - 1) / kRows);
   const dim3 grid(row_tiles * args.splits, args.cache.kv_heads, q.count);
-  return launch_kernel(few_rows_kernel<D, CODE>, grid, dim3(64 * kWaves), 0, stream, args, row_tiles);
+  if (args.wide) return launch_kernel(few_rows_kernel<D, CODE, 2 * kWaves>, grid, dim3(128 * kWaves), 0, stream, args, row_tiles);
+  return launch_kernel(few_rows_kernel<D, CODE, kWaves>, grid, dim3(64 * kWaves), 0, stream, args, row_tiles);
 }
 template <int D>
 hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
@@ -382,7 +383,10 @@ hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
 // (512) 17.9 | 26.3; one of 512, 32 of 128 on 8 (1024) 19.5 | 23.0; eight of 128, 16 of 64 on 16 (1024, but of 64 keys) 10.2 | 7.4; two of 512, 32 of 64 on 8 (2048)
 // 21.2 | 14.4; 64 tokens behind 1936 in four sequences, 16 of 128 on 16 (256, 65 million values) 30.1 | 22.0; five of 37 to 512, 8 of 64 on 4 (1280, of which
 // 756 have rows) 12.4 | 14.7.
-// A split costs its join, some 3 us: few rows go unsplit up to three steps (500 keys, heads of 64: 6.5 us, 7.8 in two splits), four where the device is full.
+// A split costs its join, some 3 us: few rows go unsplit up to three steps (500 keys, heads of 64: 6.5 us, 7.8 in two splits), four where a quarter of the device
+// has work (16 sequences of 1000 on 8 heads of 64: 9.9 us, 10.8 in splits; 4 sequences on 4: 9.0, 8.5). Where a compute unit has no second workgroup to wait
+// for and the steps are even, twice as many wavefronts take half of them each: 500 keys, heads of 64 6.7 us for 7.2, 64 sequences on 4 of them 7.7 for 8.3,
+// 1000 keys 11.6 for 12.8; three steps gain nothing (8.9), and 512 workgroups of 500 keys take 14.5 for 11.5.
 void plan_attention(AttentionArgs& args, int compute_units) {
   const onebit_sequences& q = args.sequences;
   const long long rows = (long long)q.max_new * args.group, room = (long long)q.width * args.cache.block;
@@ -401,7 +405,8 @@ void plan_attention(AttentionArgs& args, int compute_units) {
   // few rows: one step of each wavefront
   const long long least = few ? kWaves * 4096 / args.cache.head_dim : 8 * units <= compute_units && most >= 1024 ? 256 : 512;
   long long keys = std::max(least, ((most + splits - 1) / splits + least - 1) / least * least);
-  if (few && most <= (units >= compute_units ? 4 : 3) * least) keys = most;
+  if (few && most <= (4 * units > compute_units ? 4 : 3) * least) keys = most;
+  args.wide = few && keys >= most && units <= compute_units && (most + least - 1) / least % 2 == 0;
   args.splits = (int)((most + keys - 1) / keys);
   args.keys_per_split = (int)keys;
 }

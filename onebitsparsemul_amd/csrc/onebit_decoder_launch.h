@@ -35,6 +35,7 @@ struct AttentionArgs {
   uint32_t group_inverse;  // 2^32 / group, rounded up
   int dtype;
   float scale;
+  int wide;  // few_rows_kernel with twice as many wavefronts
   int rows;  // of q to a workgroup: 16 (few_rows_kernel) or many_rows() (many_rows_kernel)
   // keys split over workgroups: split i takes keys [i * keys_per_split, ...) of its sequence; workspace: splits x tokens x heads rows of
   // head_dim fp32 sums, then as many pairs (running maximum, sum); splits == 1: none
