@@ -79,7 +79,7 @@ int onebit_cache_append(const onebit_cache *cache, const onebit_sequences *seque
 
 /*
  * out = softmax(scale q k^T) v: the i-th of a sequence's n new tokens attends to its first length - n + i + 1 tokens, head h through
- * key/value head h / (heads / kv_heads). A row that attends to nothing is 0. q and out: fp16 or bf16 (dtype), 16-byte aligned rows.
+ * key/value head h / (heads / kv_heads). A row that attends to nothing is 0. scale may be negative. q and out: fp16 or bf16 (dtype), 16-byte aligned rows.
  * workspace: onebit_cache_attention_workspace() bytes, 16-byte aligned (NULL where that is 0).
  */
 size_t onebit_cache_attention_workspace(const onebit_cache *cache, const onebit_sequences *sequences, int heads);

@@ -88,6 +88,11 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) raw[c] = *(const u4_t*)(at + 16 * c);
       }
+      if (args.scale < 0.f) {  // the sign into q: multiply() takes maxima of products and multiplies them by row_factor afterwards
+        row_factor = -row_factor;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) raw[c] ^= 0x80008000u;
+      }
       float factor = 1.f;
       if (args.dtype == ONEBIT_DTYPE_BF16) {  // rows as q 2^(8 - e), e the exponent of their largest value
         uint32_t most = 0;

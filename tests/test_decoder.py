@@ -246,6 +246,17 @@ def test_attention_with_large_scores(new):
     case.check(case.call(scale=2.0), scale=2.0)
 
 
+# (copies of the sequence, new tokens): few rows, and enough of them that the kernel of prompts takes them
+@pytest.mark.parametrize("new,copies", [(1, 1), (24, 1), (200, 24)])
+@pytest.mark.parametrize("dim,block,code,dtype", [(64, 16, E4M3, torch.float16), (64, 128, INT8, torch.bfloat16), (128, 32, E4M3, torch.bfloat16),
+                                                  (128, 64, INT8, torch.float16)])
+@pytest.mark.parametrize("scale", [-0.5, -0.125, 0.0])
+def test_attention_with_a_scale_that_is_not_positive(new, copies, dim, block, code, dtype, scale):
+    """The largest exponent is then that of the least product; with a scale of 0 every key counts the same"""
+    case = Case([500], [new], 4, 2, dim, block, code, dtype, seed=dim + new)
+    case.check(case.crowd(copies, max_new=new, scale=scale), scale=scale)
+
+
 def test_attention_views_streams_and_results_in_place():
     case = Case([130, 90], [20, 1], 8, 2, 128, 64, E4M3, torch.bfloat16)
     plain = case.call()
