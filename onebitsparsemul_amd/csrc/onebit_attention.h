@@ -62,6 +62,7 @@ __device__ inline float sum_over_16(float x) {
 }
 
 __device__ inline float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+__device__ inline float power_or_zero(int e) { return e < -126 ? 0.f : power_of_two(e); }
 // Exponent of a normal magnitude (a NaN and infinities: 128)
 __device__ inline int exponent_of(uint32_t magnitude_bits) { return (int)(magnitude_bits >> 23) - 127; }
 
@@ -70,16 +71,17 @@ __device__ inline float usable_scale(float scale) {
   return magnitude(scale) >= 0x7f800000u ? 0x1p-100f : fminf(fmaxf(scale, 0x1p-100f), 0x1p110f);
 }
 // The exponent that the sums stand in: that of the keys' v_scale at hand, followed where it grows or falls by more than a few, for fp16 to keep the
-// bits of small p beside it. Never further below the largest so far than fp32 has room for.
+// bits of small p beside it. Never further below the largest so far than fp32 has room for. It is one for all rows, also for those that do not see the
+// largest: their sums stand as far below it as fp32 reaches.
 struct Exponent {
   int now = -100, largest = -100;
   // The power of two that the sums take on.
   __device__ float follow(int power) {
     if (power <= now && power >= now - 6) return 1.f;
     largest = max(largest, power);
-    const int next = max(power, largest - 60), down = max(now - next, -126);
+    const int next = max(power, largest - 60), down = now - next;
     now = next;
-    return power_of_two(down);
+    return power_or_zero(down);
   }
 };
 

@@ -144,6 +144,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == kWaves ? 3 : 2) void few_rows_
       int there[kTiles], there_all = 0;
       float k_factor[kTiles], own_v[kTiles];
       int power = -1000;
+      // of the least v_scale, above -99; what is as good as 0, or not finite and so reaches the sums by itself, wraps round and is none
+      uint32_t least = ~0u;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         there[t] = valid[t];
@@ -151,6 +153,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == kWaves ? 3 : 2) void few_rows_
         k_factor[t] = row_factor * k_scale[t];
         own_v[t] = v_scale[t];
         power = max(power, powers[t]);
+        least = min(least, (uint32_t)(powers[t] + 99));
       }
       const bool more = key + kChunk < end;
       if (more) {
@@ -185,6 +188,45 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == kWaves ? 3 : 2) void few_rows_
         for (int j = 0; j < D / 16; ++j) sums[j] *= keep * v_keep;
       }
       const float base = most == -INFINITY ? 0.f : most, v_factor = power_of_two(14 - v_exponent.now);
+      // the values of 32 keys, four dims at a time, as the left operands of D / 16 products
+      auto multiply_values = [&](int c, auto read, auto product) {
+#pragma unroll
+        for (int w = 0; w < D / 64; ++w) {
+          uint32_t near[4], far[4];
+          const value_words* const v = raw_v + 8 * c;
+          transpose_bytes(read(v[0][w]), read(v[1][w]), read(v[2][w]), read(v[3][w]), near);
+          transpose_bytes(read(v[4][w]), read(v[5][w]), read(v[6][w]), read(v[7][w]), far);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) product(sums[4 * w + i], codes_to_f16<CODE>(near[i], far[i]));
+        }
+      };
+      if (least < (uint32_t)max(v_exponent.now - 6 + 99, 0)) {
+        // Pages of one step whose scales are far apart: p of the smaller ones would lose its bits beside the largest, which not all rows need see. By
+        // themselves, in their own power, and then no more.
+        auto apart = [](uint32_t word) {  // for which the compiler does not keep what the products below need too
+          asm("" : "+v"(word));
+          return word;
+        };
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const int own_power = exponent_of(magnitude(usable_scale(own_v[t])));
+          if (own_power <= -100 || own_power >= v_exponent.now - 6) continue;
+          const float factor = own_v[t] * power_of_two(14 - own_power), down = power_or_zero(own_power - v_exponent.now);
+          h8_t high = {}, low = {};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float weighted = __builtin_amdgcn_exp2f(scores[t][i] - base) * factor;
+            high[t % 2 * 4 + i] = (_Float16)weighted;
+            low[t % 2 * 4 + i] = (_Float16)(weighted - (float)high[t % 2 * 4 + i]);
+          }
+          multiply_values(t / 2, apart, [&](f4_t& sum, h8_t codes) {
+            f4_t own = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, high, f4_t{}, 0, 0, 0);
+            own = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, low, own, 0, 0, 0);
+            sum += own * down;
+          });
+          own_v[t] = 0.f;
+        }
+      }
       h8_t p_high[kTiles / 2], p_low[kTiles / 2];  // together 22 bits of p: the products wait for the codes, a second one is hidden
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
@@ -208,19 +250,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == kWaves ? 3 : 2) void few_rows_
       }
 #pragma unroll
       for (int c = 0; c < kTiles / 2; ++c)
-#pragma unroll
-        for (int w = 0; w < D / 64; ++w) {  // four dims at a time
-          uint32_t near[4], far[4];
-          const value_words* const v = raw_v + 8 * c;
-          transpose_bytes(v[0][w], v[1][w], v[2][w], v[3][w], near);
-          transpose_bytes(v[4][w], v[5][w], v[6][w], v[7][w], far);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const h8_t codes = codes_to_f16<CODE>(near[i], far[i]);
-            sums[4 * w + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, p_high[c], sums[4 * w + i], 0, 0, 0);
-            sums[4 * w + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, p_low[c], sums[4 * w + i], 0, 0, 0);
-          }
-        }
+        multiply_values(c, [](uint32_t word) { return word; }, [&](f4_t& sum, h8_t codes) {
+          sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, p_high[c], sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, p_low[c], sum, 0, 0, 0);
+        });
       if (more) load_values();
     }
 

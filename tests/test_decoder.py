@@ -257,6 +257,27 @@ def test_attention_with_a_scale_that_is_not_positive(new, copies, dim, block, co
     case.check(case.crowd(copies, max_new=new, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("new", [16, 20, 40])
+@pytest.mark.parametrize("dim,block,code", [(64, 16, E4M3), (64, 32, INT8), (64, 64, E4M3), (128, 16, INT8), (128, 32, E4M3), (128, 64, INT8)])
+@pytest.mark.parametrize("apart", [30, 70, -30, -70])
+def test_attention_is_blind_to_the_scales_of_later_pages(new, dim, block, code, apart):
+    """Every other page has values 2^apart times as large, and the first new tokens see half of the first page alone, where others of the same tile of rows
+    see the second: what a row does not see costs it no bits"""
+    case = Case([block // 2 + new], [new], 2, 2, dim, block, code, torch.bfloat16, seed=block)
+    case.v_scale[case.pages[0, 1::2].long()] *= 2.0**apart
+    case.check(case.call())
+
+
+def test_attention_beside_pages_beyond_the_range_of_a_sum():
+    """Values 2^150 apart: the small ones of rows that see no others may count as 0, but as nothing else"""
+    case = Case([24], [16], 2, 2, 64, 16, E4M3, torch.bfloat16)
+    case.v_scale[case.pages[0, 0].long()] *= 2.0**-90
+    case.v_scale[case.pages[0, 1].long()] *= 2.0**60
+    got, want = case.call(), case.want()[0]
+    case.check(got, rows=slice(8, None))
+    assert bool(((got.double().cpu() - want).abs() <= want.abs() * (1 + 2.0**-7))[:8].all())
+
+
 def test_attention_views_streams_and_results_in_place():
     case = Case([130, 90], [20, 1], 8, 2, 128, 64, E4M3, torch.bfloat16)
     plain = case.call()
