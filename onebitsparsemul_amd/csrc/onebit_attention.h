@@ -74,14 +74,15 @@ __device__ inline float usable_scale(float scale) {
 // bits of small p beside it. Never further below the largest so far than fp32 has room for. It is one for all rows, also for those that do not see the
 // largest: their sums stand as far below it as fp32 reaches.
 struct Exponent {
-  int now = -100, largest = -100;
+  int now = -100, largest = -100;  // -100: nothing yet but what is as good as 0
   // The power of two that the sums take on.
   __device__ float follow(int power) {
     if (power <= now && power >= now - 6) return 1.f;
     largest = max(largest, power);
-    const int next = max(power, largest - 60), down = now - next;
+    const int next = max(power, max(largest - 60, -99));
+    const float factor = now == -100 ? 0.f : power_or_zero(now - next);
     now = next;
-    return power_or_zero(down);
+    return factor;
   }
 };
 

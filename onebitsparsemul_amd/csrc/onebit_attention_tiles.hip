@@ -75,7 +75,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
     // the row of this lane's column
     const int row = wave_row + r;
     const Rows own_row = behind(own_first, wave * 32 + r, args);
-    const long long token = seq.start + own_row.token;
+    const int token = seq.start + own_row.token;
     const int query_head = head * args.group + own_row.head;
     const int seen = row < rows ? max(before + own_row.token, 0) : 0;
 
@@ -250,9 +250,9 @@ uint32_t by_dim[4];
       auto value = [&](int i, int j) { return values[kFrom][32 * 8 * j + (own_value ^ 2 * i ^ 2 * (j & 1))]; };
       const h2_t ones = {(_Float16)1.f, (_Float16)1.f};
       float sum = 0.f;
-      // p of 16 keys, with v_scale as a part of the exponent
-      auto weigh = [&](int i, float log) {
-        const float shift = log + (float)(8 - v_exponent.now) - base;
+      // p of 16 keys, with v_scale as a part of the exponent, beside 2^(exponent - 8)
+      auto weigh = [&](int i, float log, int exponent) {
+        const float shift = log + (float)(8 - exponent) - base;
         h8_t p;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -267,35 +267,38 @@ uint32_t by_dim[4];
       int least = powers[0];
 #pragma unroll
       for (int i = 1; i < (ONE_PAGE ? 1 : 4); ++i) least = min(least, powers[i]);
+      float v_total[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_total[i] = lane_value(v_inverse, entry[i]);
       if (least < v_exponent.now - 6) {
-        // Pages of one tile whose scales are far apart (p of the smaller ones would lose its bits beside the largest), or a scale too small for the sums
-        // to follow, which counts as the smallest that they can: nothing beside the largest. By themselves, and then no more.
+        // Pages of one tile whose scales are far apart (p of the smaller ones would lose its bits beside the largest, which not all rows need see), or a scale
+        // too small for the sums to follow. By themselves, in their own power, and then no more; a scale that is as good as 0 adds nothing.
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (powers[i] >= power - 6 && powers[i] >= v_exponent.now - 6) continue;
-          const float own_keep = v_exponent.follow(powers[i]);
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) sums[j] *= own_keep;
-          const bool negligible = powers[i] < v_exponent.now - 6;
-          const h8_t p = weigh(i, negligible ? (float)v_exponent.now : lane_value(v_log, entry[i]));
-          total_p += sum * (negligible ? 0x1p-8f : lane_value(v_inverse, entry[i]) * power_of_two(v_exponent.now - 8));
+          if (powers[i] >= v_exponent.now - 6) continue;
+          const float down = powers[i] > -100 ? power_or_zero(powers[i] - v_exponent.now) : 0.f;
+          const h8_t p = weigh(i, lane_value(v_log, entry[i]), powers[i]);
+          total_p += sum * (lane_value(v_inverse, entry[i]) * power_of_two(powers[i] - 8));
           sum = 0.f;
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) sums[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p, sums[j], 0, 0, 0);
+          for (int j = 0; j < D / 32; ++j) {
+            sums[j] += __builtin_amdgcn_mfma_f32_32x32x16_f16(value(i, j), p, f16x_t{}, 0, 0, 0) * down;
+            // one after the other; without it the build of e4m3 codes, heads of 64 and pages from 64 on takes 169 registers, and two workgroups to a compute
+            // unit for three: 64 prompts of 256 44.5 us for 37.3 (smaller pages are better off without: int8 168 registers for 169)
+            if (ONE_PAGE) __builtin_amdgcn_sched_barrier(0);
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) scores[i / 2][i % 2 * 8 + e] = -INFINITY;
           factor[i] = 1.f;
+          v_total[i] = 0.f;  // (beside the large exponent it need not be finite)
         }
-        const float own_keep = v_exponent.follow(power);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) sums[j] *= own_keep;
       }
       h8_t p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = weigh(i, lane_value(v_log, entry[i]));
+        p[i] = weigh(i, lane_value(v_log, entry[i]), v_exponent.now);
         if (!ONE_PAGE || i == 3) {
-          total_p += sum * (lane_value(v_inverse, entry[i]) * power_of_two(v_exponent.now - 8));
+          total_p += sum * (v_total[i] * power_of_two(v_exponent.now - 8));
           sum = 0.f;
         }
       }
@@ -345,7 +348,7 @@ uint32_t by_dim[4];
     const float sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]), v_factor = v_exponent.largest > -100 ? power_of_two(v_exponent.now - 8) : 0.f;
     if (row < rows) {
       if (args.splits > 1) {
-        const long long at = split * all_rows + token * args.heads + query_head;
+        const long long at = split * all_rows + (long long)token * args.heads + query_head;
         if (sum != 0.f) {
 #pragma unroll
           for (int j = 0; j < D / 32; ++j)

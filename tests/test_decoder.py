@@ -268,6 +268,19 @@ def test_attention_is_blind_to_the_scales_of_later_pages(new, dim, block, code, 
     case.check(case.call())
 
 
+@pytest.mark.parametrize("dim,block,code", [(64, 16, E4M3), (64, 32, INT8), (64, 64, E4M3), (128, 16, INT8), (128, 32, E4M3), (128, 64, INT8)])
+@pytest.mark.parametrize("apart", [30, 70, -30, -70])
+def test_attention_of_prompts_is_blind_to_the_scales_of_later_pages(dim, block, code, apart):
+    """The same where many rows make a tile, and first pages whose codes count as 0"""
+    case = Case([block // 2 + 64], [64], 2, 2, dim, block, code, torch.bfloat16, seed=block)
+    case.v_scale[case.pages[0, 1::2].long()] *= 2.0**apart
+    case.check(case.crowd(200, max_new=64))
+    case.v_scale[case.pages[0, 0].long()] = 0
+    got = case.crowd(200, max_new=64)
+    case.check(got)
+    assert bool((got[:block // 2] == 0).all())
+
+
 def test_attention_beside_pages_beyond_the_range_of_a_sum():
     """Values 2^150 apart: the small ones of rows that see no others may count as 0, but as nothing else"""
     case = Case([24], [16], 2, 2, 64, 16, E4M3, torch.bfloat16)
