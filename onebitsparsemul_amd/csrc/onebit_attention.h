@@ -66,9 +66,10 @@ __device__ inline float power_or_zero(int e) { return e < -126 ? 0.f : power_of_
 // Exponent of a normal magnitude (a NaN and infinities: 128)
 __device__ inline int exponent_of(uint32_t magnitude_bits) { return (int)(magnitude_bits >> 23) - 127; }
 
-// What takes a v_scale's part in exponents: one below 2^-100 is as good as 0, one that is not finite is dealt with apart.
+// What takes a v_scale's part in exponents: one below 2^-100 is as good as 0, one that is not finite is dealt with apart. The largest finite value makes
+// scales below 2^122 (over 127); an exponent of theirs has room for its neighbours here, and for its negative.
 __device__ inline float usable_scale(float scale) {
-  return magnitude(scale) >= 0x7f800000u ? 0x1p-100f : fminf(fmaxf(scale, 0x1p-100f), 0x1p110f);
+  return magnitude(scale) >= 0x7f800000u ? 0x1p-100f : fminf(fmaxf(scale, 0x1p-100f), 0x1.fffffep121f);
 }
 // The exponent that the sums stand in: that of the keys' v_scale at hand, followed where it grows or falls by more than a few, for fp16 to keep the
 // bits of small p beside it. Never further below the largest so far than fp32 has room for. It is one for all rows, also for those that do not see the

@@ -291,6 +291,15 @@ def test_attention_beside_pages_beyond_the_range_of_a_sum():
     assert bool(((got.double().cpu() - want).abs() <= want.abs() * (1 + 2.0**-7))[:8].all())
 
 
+@pytest.mark.parametrize("new,copies", [(16, 1), (64, 200)])
+@pytest.mark.parametrize("dim,block,code", [(64, 16, E4M3), (64, 64, INT8), (128, 32, E4M3), (128, 64, INT8)])
+def test_attention_of_the_largest_values(new, copies, dim, block, code):
+    """Values up to some 2^123, of which an append makes scales up to 2^121: their sums over the keys are within fp32 here"""
+    case = Case([8 + new], [new], 2, 2, dim, block, code, torch.bfloat16, seed=block)
+    case.v_scale *= 2.0**(119 if code == E4M3 else 117)
+    case.check(case.crowd(copies, max_new=new))
+
+
 def test_attention_views_streams_and_results_in_place():
     case = Case([130, 90], [20, 1], 8, 2, 128, 64, E4M3, torch.bfloat16)
     plain = case.call()
