@@ -8,6 +8,7 @@
  * enqueued on `stream` (hipStream_t as void*, NULL = default stream) and the calls return without synchronising. They allocate
  * nothing, keep nothing between calls, and can be captured in a HIP graph. Status codes, dtype codes and
  * onebit_sparse_last_error() are those of onebit_sparse_tensor.h; a call of more than 2^32 threads is refused as HIP refuses it.
+ * Results lie apart from the operands unless a function says that the two may be the same memory.
  */
 #ifndef ONEBIT_DECODER_H_
 #define ONEBIT_DECODER_H_
@@ -82,7 +83,7 @@ int onebit_cache_append(const onebit_cache *cache, const onebit_sequences *seque
 /*
  * out = softmax(scale q k^T) v: the i-th of a sequence's n new tokens attends to its first length - n + i + 1 tokens, head h through
  * key/value head h / (heads / kv_heads). A row that attends to nothing is 0. scale may be negative. q and out: fp16 or bf16 (dtype), 16-byte aligned rows.
- * workspace: onebit_cache_attention_workspace() bytes, 16-byte aligned (NULL where that is 0).
+ * q and out may be the same memory (with equal strides). workspace: onebit_cache_attention_workspace() bytes, 16-byte aligned (NULL where that is 0).
  */
 size_t onebit_cache_attention_workspace(const onebit_cache *cache, const onebit_sequences *sequences, int heads);
 int onebit_cache_attention(const onebit_cache *cache, const onebit_sequences *sequences, const onebit_heads *q, const onebit_heads *out,
@@ -92,7 +93,7 @@ int onebit_cache_attention(const onebit_cache *cache, const onebit_sequences *se
  * The norms around a block: h = residual_scale * residual + block_scale * gate * post(x), y = pre(h), with one pass over the rows.
  * post is left out where post_weight is NULL, the gate where it is NULL, and with x NULL h is residual_scale * residual. kind 0:
  * h / sqrt(mean(h^2) + eps) * weight + bias, kind 1: (h - mean(h)) / sqrt(var(h) + eps) * weight + bias (a bias NULL: none). All in fp32 from
- * the unrounded h; h and y are rounded once. h_out may be residual, or NULL (h is not wanted). Rows are hidden consecutive
+ * the unrounded h; h and y are rounded once. h_out may be residual or x (with equal strides and types), or NULL (h is not wanted). Rows are hidden consecutive
  * values; strides in elements. gate: gate_row_stride between rows, gate_column_stride 0 or 1. hidden: at most 32768.
  */
 typedef struct onebit_norm {

@@ -1,5 +1,6 @@
 // Torch side of onebit_decoder.h: checks of the operands, results, workspace and the current stream. Operands that the kernels
-// do not read where they lie (rows inside a head that are no whole 16-byte units, a negated view) are copied first.
+// do not read where they lie (rows inside a head that are no whole 16-byte units, a negated view, elements on which a result given by the caller is
+// written in another order) are copied first.
 #include "torch_binding.h"
 
 #include "onebit_decoder.h"
@@ -8,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace {
 
@@ -20,6 +22,50 @@ void check_table(const torch::Tensor& t, const char* name, c10::ScalarType type,
   check_gpu(t, name, device);
   TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
   TORCH_CHECK_VALUE(t.dim() == dims && t.is_contiguous() && !t.is_neg(), name, " must be contiguous with ", dims, " dimensions, got shape ", t.sizes());
+}
+
+// The bytes from a tensor's first element to its last
+std::pair<const char*, const char*> extent(const torch::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const char* const first = (const char*)t.data_ptr();
+  return {first, first + (last + 1) * t.element_size()};
+}
+// Whether sum of x_i step_i = distance for some x_i from -below_i to above_i; true also where there are many to try. Steps from the largest on.
+struct Step {
+  int64_t step, below, above;
+};
+bool reaches(const std::vector<Step>& steps, size_t from, int64_t distance) {
+  if (from == steps.size()) return distance == 0;
+  int64_t low = 0, high = 0;  // of the others
+  for (size_t i = from + 1; i < steps.size(); ++i) low -= steps[i].step * steps[i].below, high += steps[i].step * steps[i].above;
+  const Step s = steps[from];
+  int tries = 0;
+  for (int64_t x = std::max(-s.below, (distance - high) / s.step - 1); x <= std::min(s.above, (distance - low) / s.step + 1); ++x)
+    if (++tries > 8 || reaches(steps, from + 1, distance - x * s.step)) return true;
+  return false;
+}
+// Whether two tensors may have memory in common: exactly for views that go through it in the same steps, else by their extents.
+bool may_meet(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto one = extent(a), other = extent(b);
+  if (one.second <= other.first || other.second <= one.first) return false;
+  const int64_t distance = other.first - one.first, size = a.element_size();
+  if (a.dim() != b.dim() || b.element_size() != size || distance % size) return true;
+  std::vector<Step> steps;
+  for (int64_t i = 0; i < a.dim(); ++i) {
+    if (a.size(i) > 1 && b.size(i) > 1 && a.stride(i) != b.stride(i)) return true;
+    const int64_t step = a.size(i) > 1 ? a.stride(i) : b.stride(i);
+    if (step != 0 && (a.size(i) > 1 || b.size(i) > 1)) steps.push_back({step, b.size(i) - 1, a.size(i) - 1});
+  }
+  std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.step > y.step; });
+  return reaches(steps, 0, distance / size);
+}
+// An operand that is read while `out` is written: as it is where the two are apart or the same element by element, else a copy.
+torch::Tensor beside(const torch::Tensor& in, const torch::Tensor& out) {
+  bool same = in.data_ptr() == out.data_ptr() && in.scalar_type() == out.scalar_type() && in.sizes() == out.sizes();
+  for (int64_t i = 0; same && i < in.dim(); ++i) same = in.size(i) <= 1 || in.stride(i) == out.stride(i);
+  return same || !may_meet(in, out) ? in : in.clone(at::MemoryFormat::Contiguous);
 }
 
 bool in_vectors(const torch::Tensor& t) {
@@ -104,10 +150,12 @@ torch::Tensor rotary(const torch::Tensor& x, const torch::Tensor& positions, con
   torch::Tensor y = out.has_value() ? *out : empty_result(x.sizes(), x.scalar_type(), device);
   if (x.numel() == 0) return y;
   TORCH_CHECK_VALUE(tokens < (1ll << 31) && heads < (1ll << 31) && dim < (1ll << 31), "x exceeds the int range");
-  const torch::Tensor in = x.stride(2) == 1 && !x.is_neg() ? x : x.resolve_neg().clone(at::MemoryFormat::Contiguous);
+  auto read = [&](const torch::Tensor& t) { return out.has_value() ? beside(t, y) : t; };
+  const torch::Tensor in = read(x.stride(2) == 1 && !x.is_neg() ? x : x.resolve_neg().clone(at::MemoryFormat::Contiguous));
+  const torch::Tensor places = read(positions), angles = read(table);
   const onebit_heads from = heads_of(in), to = heads_of(y);
-  check_status(onebit_rotary(&from, &to, dtype_code(x.scalar_type()), (int)tokens, (int)heads, (int)dim, positions.data_ptr(),
-                             positions.scalar_type() == torch::kInt64, turning.table, turning.rows, turning.rotary_dim, interleaved, current_stream(device)));
+  check_status(onebit_rotary(&from, &to, dtype_code(x.scalar_type()), (int)tokens, (int)heads, (int)dim, places.data_ptr(),
+                             places.scalar_type() == torch::kInt64, (const float*)angles.data_ptr(), turning.rows, turning.rotary_dim, interleaved, current_stream(device)));
   return y;
 }
 
@@ -169,7 +217,7 @@ torch::Tensor cache_attention(const torch::Tensor& q, const torch::Tensor& k_cac
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
   torch::Tensor y = out.has_value() ? *out : empty_result(q.sizes(), q.scalar_type(), device);
   if (q.numel() == 0) return y;
-  const torch::Tensor in = readable_heads(q);
+  const torch::Tensor in = out.has_value() ? beside(readable_heads(q), y) : readable_heads(q);
   const onebit_heads from = heads_of(in), to = heads_of(y);
   const size_t bytes = onebit_cache_attention_workspace(&cache, &sequences, (int)heads);
   torch::Tensor workspace;  // of the current stream, as the kernels that use it: free again with this call
@@ -225,7 +273,9 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
   const bool writes = x.has_value() || residual_scale != 1.0 || (residual_out.has_value() && residual_out->data_ptr() != residual.data_ptr());
   torch::Tensor h = residual_out.has_value() ? *residual_out : writes ? empty_result(residual.sizes(), residual.scalar_type(), device) : residual;
   if (residual.numel() == 0) return {h, y};
-  const torch::Tensor residual_rows = rows_of(residual, hidden), x_rows = x.has_value() ? rows_of(*x, hidden) : residual_rows;
+  const bool given = residual_out.has_value();
+  auto read = [&](const torch::Tensor& t) { return given ? beside(t, h) : t; };
+  const torch::Tensor residual_rows = rows_of(read(residual), hidden), x_rows = x.has_value() ? rows_of(read(*x), hidden) : residual_rows;
   TORCH_CHECK_VALUE(residual_rows.size(0) < (1ll << 31) && hidden < (1ll << 31), "too many rows");
   onebit_norm n = {};
   torch::Tensor gate_rows;
@@ -237,6 +287,7 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
                       "gate must have shape (hidden,), (..., 1) or (..., hidden), or one value, got ", gate->sizes());
     gate_rows = gate->numel() == 1 ? gate->reshape({1, 1}) : gate->dim() == 1 ? gate->reshape({1, hidden}) : gate->reshape({-1, last});
     if (gate_rows.is_neg() || (gate_rows.size(1) > 1 && gate_rows.stride(1) != 1 && gate_rows.stride(1) != 0)) gate_rows = gate_rows.resolve_neg().clone(at::MemoryFormat::Contiguous);
+    gate_rows = read(gate_rows);
     n.gate = gate_rows.data_ptr();
     n.gate_row_stride = gate_rows.size(0) > 1 ? gate_rows.stride(0) : 0;
     n.gate_column_stride = gate_rows.size(1) > 1 ? (int)gate_rows.stride(1) : 0;
@@ -246,10 +297,13 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
   n.residual = residual_rows.data_ptr();
   n.h_out = writes ? h.data_ptr() : nullptr;
   n.y = y.data_ptr();
-  n.weight = weight.data_ptr();
-  n.bias = bias.has_value() ? bias->data_ptr() : nullptr;
-  n.post_weight = post_weight.has_value() ? post_weight->data_ptr() : nullptr;
-  n.post_bias = post_bias.has_value() ? post_bias->data_ptr() : nullptr;
+  const torch::Tensor vectors[] = {read(weight), bias.has_value() ? read(*bias) : torch::Tensor(), post_weight.has_value() ? read(*post_weight) : torch::Tensor(),
+                                   post_bias.has_value() ? read(*post_bias) : torch::Tensor()};
+  auto address = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  n.weight = address(vectors[0]);
+  n.bias = address(vectors[1]);
+  n.post_weight = address(vectors[2]);
+  n.post_bias = address(vectors[3]);
   n.x_stride = x_rows.size(0) > 1 ? x_rows.stride(0) : 0;
   n.residual_stride = residual_rows.size(0) > 1 ? residual_rows.stride(0) : 0;
   n.h_stride = n.y_stride = residual_rows.size(0) > 1 ? hidden : 0;

@@ -67,7 +67,7 @@ def rotary_table(positions, rotary_dim, base=10000.0, scaling=None, device="cuda
 def rotary(x, positions, table, interleaved=False, out=None):
     """Rotary positions on x (tokens, heads, head_dim): the first table.shape[1] elements of each head are turned in pairs, half
     a part apart or interleaved, the others copied. positions (tokens,): int32 or int64; one outside of the table gives NaN. x may
-    be strided; out may be x."""
+    be strided; out may be x. Where it lies on the operands in another way, they are copied first."""
     return _binding().rotary(x, positions, table, interleaved, out)
 
 
@@ -86,7 +86,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, start
     """softmax(scale q k^T) v of the new tokens' queries (tokens, heads, head_dim), float16 or bfloat16, over the cache, causal: the last of
     a sequence's new tokens sees all its `lengths` tokens. heads is a multiple of kv_heads. Other arguments as of cache_append; scale:
     1 / sqrt(head_dim) unless given; max_length: no sequence is longer (host number: what the launch is planned for). A row that
-    sees nothing is 0."""
+    sees nothing is 0. out may be q, as rotary's may be x."""
     return _binding().cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, starts, scale, max_new, max_length, out)
 
 
@@ -95,7 +95,7 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
     """(h, y): h = residual_scale residual + block_scale gate post(x), the residual behind a block with output x, and y = norm(h), the
     input of the next. post: a norm with post_weight (and post_bias), where given; gate: (hidden,), (..., 1), (..., hidden) or one value.
     kind "rms" or "layer". In fp32 throughout; h has the residual's type, y x's (or out_dtype). x None: y = norm(residual). residual_out
-    may be the residual itself."""
+    may be the residual or x itself, as rotary's out may be x."""
     return _binding().block_norm(x, residual, weight, bias, post_weight, post_bias, gate, residual_scale, block_scale, eps, kind, out_dtype, residual_out)
 
 

@@ -414,6 +414,81 @@ def test_rotary_outside_of_the_table_and_of_nothing():
     assert torch.equal(onebit.rotary(strided, torch.arange(4).cuda(), table), onebit.rotary(strided.contiguous(), torch.arange(4).cuda(), table))
 
 
+# ---- results on the memory of operands
+
+
+def same_as_apart(call, memory, operands, result):
+    """call(operands, out): the result on memory that operands lie on is that of copies of them; operands and result are taken from `memory`"""
+    source = memory.clone()
+    want = call([take(source).clone() for take in operands], None)
+    out = result(memory)
+    got = call([take(memory) for take in operands], out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("part", [128, 64, 10])
+def test_rotary_onto_its_operands_memory(part):
+    tokens, heads, dim = 600, 8, 128
+    g = generator(part)
+    table, positions = onebit.rotary_table(700, part), torch.randint(0, 700, (600,), generator=g).cuda()
+    memory = torch.randn((tokens + 1, heads + 1, dim), generator=g).half().cuda()
+    turn = lambda x, out: onebit.rotary(x[0], positions, table, out=out)  # noqa: E731
+    same_as_apart(turn, memory.clone(), [lambda m: m[1:, :heads]], lambda m: m[1:, 1:])     # a head further on
+    same_as_apart(turn, memory.clone(), [lambda m: m[1:, 1:]], lambda m: m[1:, :heads])
+    same_as_apart(turn, memory.clone(), [lambda m: m[:-1, :heads]], lambda m: m[1:, :heads])  # a token further on
+    square = torch.randn((tokens, tokens // 40, dim), generator=g).half().cuda().view(-1)
+    same_as_apart(turn, square, [lambda m: m.view(tokens // 40, tokens, dim).transpose(0, 1)], lambda m: m.view(tokens, tokens // 40, dim))  # other strides
+    wide = memory.view(-1)[:tokens * heads * dim]
+    same_as_apart(lambda x, out: onebit.rotary(x[0].expand(tokens, heads, dim), positions, table, out=out), wide.clone(),
+                  [lambda m: m[dim * heads * 300:dim * heads * 300 + dim]], lambda m: m.view(tokens, heads, dim))  # one head for all
+    # apart, though between one another: read in place, and left alone
+    pair = torch.randn((tokens, 2 * heads, dim), generator=g).half().cuda()
+    before = pair.clone()
+    same_as_apart(turn, pair, [lambda m: m[:, :heads]], lambda m: m[:, heads:])
+    assert torch.equal(pair[:, :heads], before[:, :heads])
+    ids = torch.randn((tokens, heads, dim), generator=g).cuda()
+    ids.view(torch.int32).view(-1)[:tokens] = positions.int()
+    same_as_apart(lambda o, out: onebit.rotary(ids, o[0].view(torch.int32), table, out=out), ids.clone(), [lambda m: m.view(-1)[:tokens]], lambda m: m)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_onto_its_queries_memory(new):
+    case = Case([300] * 4, [new] * 4, 8, 2, 64, 32, E4M3, torch.float16)
+    memory = torch.randn((4 * new + 1, 9, 64), generator=generator(new)).half().cuda()
+    attend = lambda q, out: case.call(q=q[0], out=out, max_new=new)  # noqa: E731
+    same_as_apart(attend, memory.clone(), [lambda m: m[1:, :8]], lambda m: m[1:, 1:])
+    same_as_apart(attend, memory.clone(), [lambda m: m[:-1, 1:]], lambda m: m[1:, 1:])
+    same_as_apart(attend, memory.clone(), [lambda m: m[1:, 1:]], lambda m: m[1:, 1:])  # the very same
+
+
+@pytest.mark.parametrize("hidden", [512, 4096, 9000])
+def test_block_norm_onto_its_operands_memory(hidden):
+    rows = 300
+    g = generator(hidden)
+    memory = torch.randn((rows + 1, hidden), generator=g).half().cuda()
+    other, weight = torch.randn((rows, hidden), generator=g).half().cuda(), torch.randn(hidden, generator=g).half().cuda()
+
+    def check(operands, result, call):
+        same_as_apart(lambda o, out: call(o, out)[0], memory.clone(), operands, result)
+        now, source = memory.clone(), memory.clone()
+        assert torch.equal(call([take(now) for take in operands], result(now))[1], call([take(source).clone() for take in operands], None)[1])
+
+    first, second = (lambda m: m[:-1]), (lambda m: m[1:])
+    norm = lambda x, residual, out, **options: onebit.block_norm(x, residual, options.pop("weight", weight), residual_out=out, **options)  # noqa: E731
+    check([first], second, lambda o, out: norm(other, o[0], out))             # a residual a row further up
+    check([first], second, lambda o, out: norm(o[0], other, out))             # a block's output
+    check([first, second], second, lambda o, out: norm(o[0], o[1], out))
+    check([second], second, lambda o, out: norm(o[0], other, out))            # the very same
+    check([lambda m: m[1:, :1]], second, lambda o, out: norm(other, other, out, gate=o[0]))  # a column of it
+    for row in (3, 200):
+        take = [lambda m, row=row: m[row]]
+        check(take, second, lambda o, out: norm(other, other, out, weight=o[0]))
+        check(take, second, lambda o, out: norm(other, other, out, bias=o[0]))
+        check(take, second, lambda o, out: norm(other, other, out, post_weight=o[0]))
+        check(take, second, lambda o, out: norm(other, other, out, gate=o[0]))
+    check([lambda m: m.view(-1)[:hidden * rows].view(hidden, rows).t()], first, lambda o, out: norm(other, o[0], out))  # other strides
+
+
 # ---- the cache's write side
 
 
