@@ -61,11 +61,16 @@ bool may_meet(const torch::Tensor& a, const torch::Tensor& b) {
   std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.step > y.step; });
   return reaches(steps, 0, distance / size);
 }
+// Whether two tensors are the same element by element
+bool are_same(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
 // An operand that is read while `out` is written: as it is where the two are apart or the same element by element, else a copy.
 torch::Tensor beside(const torch::Tensor& in, const torch::Tensor& out) {
-  bool same = in.data_ptr() == out.data_ptr() && in.scalar_type() == out.scalar_type() && in.sizes() == out.sizes();
-  for (int64_t i = 0; same && i < in.dim(); ++i) same = in.size(i) <= 1 || in.stride(i) == out.stride(i);
-  return same || !may_meet(in, out) ? in : in.clone(at::MemoryFormat::Contiguous);
+  return are_same(in, out) || !may_meet(in, out) ? in : in.clone(at::MemoryFormat::Contiguous);
 }
 
 bool in_vectors(const torch::Tensor& t) {
@@ -270,7 +275,7 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
   torch::Tensor y = empty_result(residual.sizes(), y_type, device);
   // without a block the residual is only normed, unless it is scaled or wanted elsewhere
-  const bool writes = x.has_value() || residual_scale != 1.0 || (residual_out.has_value() && residual_out->data_ptr() != residual.data_ptr());
+  const bool writes = x.has_value() || residual_scale != 1.0 || (residual_out.has_value() && (!are_same(residual, *residual_out) || residual.is_neg()));
   torch::Tensor h = residual_out.has_value() ? *residual_out : writes ? empty_result(residual.sizes(), residual.scalar_type(), device) : residual;
   if (residual.numel() == 0) return {h, y};
   const bool given = residual_out.has_value();

@@ -489,6 +489,21 @@ def test_block_norm_onto_its_operands_memory(hidden):
     check([lambda m: m.view(-1)[:hidden * rows].view(hidden, rows).t()], first, lambda o, out: norm(other, o[0], out))  # other strides
 
 
+def test_block_norm_of_a_residual_in_other_strides_than_its_result():
+    """Without a block and with the scale 1 the residual is only to be moved: it is, also where both begin at one address"""
+    memory = torch.randn((256, 256), generator=generator(1)).half().cuda()
+    weight = torch.ones(256, dtype=torch.float16, device="cuda")
+    for residual in (lambda m: m.t(), lambda m: m[:1].expand(256, 256), lambda m: m.view(128, 2, 256)[:, 0]):
+        now, source = memory.clone(), memory.clone()
+        x = residual(now)
+        out = now[:x.shape[0]]
+        h, y = onebit.block_norm(None, x, weight, residual_out=out)
+        want = residual(source).contiguous()
+        assert h.data_ptr() == now.data_ptr() and torch.equal(out, want) and torch.equal(y, onebit.block_norm(None, want, weight)[1])
+    kept = memory.clone()
+    assert onebit.block_norm(None, kept, weight, residual_out=kept)[0].data_ptr() == kept.data_ptr() and torch.equal(kept, memory)
+
+
 # ---- the cache's write side
 
 
