@@ -55,7 +55,7 @@ typedef struct onebit_sequences {
   const int *starts;     /* count + 1, or NULL */
   int count, width;
   int tokens;     /* rows of the token-major operands */
-  int max_new;    /* no sequence has more new tokens (an append leaves out what is beyond) */
+  int max_new;    /* no sequence has more new tokens (an append writes no keys and values of those beyond; attention does all, slower) */
   int max_length; /* what the launch is planned for; longer sequences are right and slower. 0: width * block */
 } onebit_sequences;
 

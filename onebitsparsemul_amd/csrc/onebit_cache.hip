@@ -146,13 +146,14 @@ __device__ inline void append_page(const AppendArgs& args, const Sequence& seq, 
   __shared__ uint32_t most[THREADS / 64];
   const onebit_cache& cache = args.cache;
   const int first = seq.length - seq.fresh;  // position of the first new token; before the sequence where there are too many
+  const int end = first + min(seq.fresh, args.sequences.max_new);  // what is beyond is left out
   const int j = max(first, 0) / cache.block + slot, begin = j * cache.block;
-  if (begin >= seq.length) return;
+  if (begin >= end) return;
   const int page = args.sequences.page_table[(long long)s * args.sequences.width + j];
   if (page < 0 || page >= cache.pages) return;
   const int units = cache.head_dim / (2 * kUnit), tokens_per_pass = THREADS / units;
   const int low_position = max(max(first, 0), begin);
-  const int count = min(min(seq.length, begin + cache.block) - low_position, PASSES * tokens_per_pass);
+  const int count = min(end, begin + cache.block) - low_position;  // above 0, at most PASSES * tokens_per_pass
   const onebit_heads& x = values ? args.v : args.k;
   const long long place = (long long)page * cache.kv_heads + head;
   float* const scale_at = (values ? cache.v_scale : cache.k_scale) + place;

@@ -573,6 +573,34 @@ def test_append(code, dtype, dim, block, part, interleaved):
             assert got is None
 
 
+@pytest.mark.parametrize("most", [1, 3, 8, 9, 20, 64, 100, 1 << 31])
+@pytest.mark.parametrize("dim,block,code", [(64, 64, E4M3), (128, 16, INT8), (64, 128, INT8)])
+def test_append_leaves_out_tokens_beyond_max_new(most, dim, block, code):
+    """Sequences with more new tokens than the call says: the first of them are written, to the bit, and nothing else; queries are turned all"""
+    kv_heads, heads, new, first = 2, 4, [70, 1, 33, 150], [5, 90, 0, 61]
+    g = generator(block)
+    cache = onebit.QuantizedCache(60, kv_heads, dim, block=block, dtype=code)
+    for codes in (cache.k, cache.v):
+        bits(codes).copy_(torch.randint(0, 100, codes.shape, generator=g, dtype=torch.uint8))
+    cache.k_scale.fill_(0.25)
+    cache.v_scale.fill_(0.125)
+    mirror = [t.cpu().clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    pages = torch.randperm(60, generator=g).view(4, 15).to(torch.int32)
+    table = onebit.rotary_table(240, dim, device="cpu")
+    q, k, v = (torch.randn((sum(new), n, dim), generator=g).half() for n in (heads, kv_heads, kv_heads))
+    starts = torch.tensor([sum(new[:i]) for i in range(5)], dtype=torch.int32)
+    lengths = [a + b for a, b in zip(first, new)]
+    got = cache.append(k.cuda(), v.cuda(), pages.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), starts=starts.cuda(), q=q.cuda(), rotary=table.cuda(),
+                       max_new=most)
+    left = [min(n, most) for n in new]
+    rows = torch.cat([torch.arange(int(s), int(s) + n) for s, n in zip(starts, left)])
+    appended(*mirror, k[rows], v[rows], pages, [a + b for a, b in zip(first, left)], left, code, table, False)
+    for mine, theirs in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), mirror):
+        assert torch.equal(bits(mine.cpu()), bits(theirs))
+    positions = torch.cat([torch.arange(a, a + n) for a, n in zip(first, new)])
+    assert torch.equal(got.cpu(), turned(q.float(), table[positions], False).to(q.dtype))
+
+
 def test_append_is_as_near_as_its_codes():
     """Against 64 bits: within half a step of the code"""
     for code, relative, absolute in ((E4M3, 2.0**-4, 2.0**-10), (INT8, 0.0, 0.5)):
