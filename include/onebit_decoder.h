@@ -74,7 +74,7 @@ int onebit_rotary(const onebit_heads *x, const onebit_heads *out, int dtype, int
  * larger of the scale that its older tokens have and the new tokens' largest magnitude / 448 or 127; codes are value / scale' rounded
  * to nearest even, and where scale' grew, the older codes become (code * scale) / scale'. All in fp32. A page that starts with a
  * new token forgets its old scale. A NaN or an infinity among the new values makes the scale NaN or infinite and the codes 0, so that
- * what attends to the page is NaN. No two sequences may write into one page.
+ * what attends to the page is NaN. No two sequences may write into one page, and keys and values (with their scales) share no memory.
  */
 int onebit_cache_append(const onebit_cache *cache, const onebit_sequences *sequences, const onebit_heads *k, const onebit_heads *v,
                         const onebit_heads *q, const onebit_heads *q_out, int heads, int dtype, const float *table, int table_rows,

@@ -174,6 +174,7 @@ OptionalTensor cache_append(const torch::Tensor& k, const torch::Tensor& v, cons
   check_heads(k, "k", device);
   check_heads(v, "v", device);
   const onebit_cache cache = cache_of(k_cache, v_cache, k_scale, v_scale, device);
+  TORCH_CHECK_VALUE(!may_meet(k_cache, v_cache) && !may_meet(k_scale, v_scale), "an append writes keys and values: their codes and scales must not share memory");
   TORCH_CHECK_VALUE(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v must have one shape and type");
   TORCH_CHECK_VALUE(k.size(1) == cache.kv_heads && k.size(2) == cache.head_dim, "k and v must have shape (tokens, ", cache.kv_heads, ", ", cache.head_dim,
                     ") for this cache, got ", k.sizes());

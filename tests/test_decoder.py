@@ -601,6 +601,23 @@ def test_append_leaves_out_tokens_beyond_max_new(most, dim, block, code):
     assert torch.equal(got.cpu(), turned(q.float(), table[positions], False).to(q.dtype))
 
 
+def test_append_refuses_keys_and_values_in_one_memory():
+    """Attention takes them"""
+    cache = onebit.QuantizedCache(4, 2, 64, block=16)
+    x = torch.randn((5, 2, 64), generator=generator(1)).half().cuda()
+    pages, lengths = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda")
+    for v, v_scale in ((cache.k, cache.v_scale), (cache.v, cache.k_scale)):
+        with pytest.raises(ValueError, match="share memory"):
+            onebit.cache_append(x, x, cache.k, v, cache.k_scale, v_scale, pages, lengths)
+    both = torch.zeros((8, 2, 16, 64), dtype=E4M3, device="cuda")
+    scales = torch.zeros((8, 2), device="cuda")
+    onebit.cache_append(x, x, both[:4], both[4:], scales[:4], scales[4:], pages, lengths)
+    cache.append(x, x, pages, lengths)
+    assert torch.equal(bits(both)[:4], bits(cache.k)) and torch.equal(bits(both)[4:], bits(cache.v)) and torch.equal(scales[4:], cache.v_scale)
+    want = cache.attend(x, pages, lengths)
+    assert torch.equal(onebit.cache_attention(x, cache.k, cache.k, cache.k_scale, cache.k_scale, pages, lengths), want)
+
+
 def test_append_is_as_near_as_its_codes():
     """Against 64 bits: within half a step of the code"""
     for code, relative, absolute in ((E4M3, 2.0**-4, 2.0**-10), (INT8, 0.0, 0.5)):
