@@ -196,6 +196,26 @@ def test_attention_with_scales_far_apart(length, new, copies, block, decades, dt
     assert bool((case.crowd(copies, max_new=new) == 0).all())
 
 
+@pytest.mark.parametrize("dim,code", [(64, E4M3), (128, INT8)])
+@pytest.mark.parametrize("lengths,new,copies,most", [([200, 77], [70, 33], 1, 1), ([200, 77], [70, 33], 1, 9), ([150], [150], 1, 20),
+                                                     ([300], [300], 130, 20), ([300, 40], [300, 7], 130, 70), ([420], [410], 130, 129)])
+def test_attention_of_more_rows_than_planned(dim, code, lengths, new, copies, most):
+    """Sequences with more new tokens than the launch was planned for: its workgroups take their other rows one tile behind the other, few rows of them and many"""
+    case = Case(lengths, new, 4, 2, dim, 16, code, torch.float16, seed=most)
+    case.check(case.crowd(copies, max_new=most))
+
+
+@pytest.mark.parametrize("dim,block,code", [(64, 16, E4M3), (128, 16, INT8), (64, 32, INT8)])
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,copies", [([5000, 4113, 2100], [1, 1, 1], 8, 4, 70), ([9000], [3], 4, 4, 200), ([5000], [2], 1, 1, 1),
+                                                               ([2500, 1100], [130, 33], 4, 2, 90), ([2500], [130], 4, 2, 24), ([1025], [130], 4, 2, 90)])
+def test_attention_over_more_pages_than_lanes(dim, block, code, lengths, new, heads, kv_heads, copies):
+    """A wavefront knows 64 pages of its sequence at a time and reads on in the table where its keys go beyond; small pages, in one split and in several"""
+    case = Case(lengths, new, heads, kv_heads, dim, block, code, torch.float16, seed=lengths[0])
+    if len(lengths) > 1:
+        case.pages[0, 66], case.pages[0, 64] = -1, 1 << 30  # two that are not there
+    case.check(case.crowd(copies, max_new=max(new), max_length=max(lengths)))
+
+
 # rows (tokens x heads of a key/value head) of one workgroup and more, enough of them that the kernel of prompts takes them
 @pytest.mark.parametrize("code", [E4M3, INT8])
 @pytest.mark.parametrize("dim,block", [(64, 16), (64, 32), (64, 128), (128, 16), (128, 64), (128, 32)])
