@@ -32,6 +32,7 @@ typedef struct onebit_heads {
 /*
  * Keys and values of one layer. Codes: pages x kv_heads x block x head_dim, 16-byte aligned; a token's value is its code
  * times the scale of its page and head (pages x kv_heads, fp32, not negative). block: 16, 32, 64 or 128 tokens; head_dim: 64 or 128.
+ * Codes of a sequence's tokens are not NaN (an append writes none): attention would carry one to rows that do not see its token.
  * Attention takes a v_scale below 2^-99 as good as 0; a row that sees no values but some 2^-100 of those that rows beside it see may take them as 0 too. The
  * largest v_scale is 2^122, and sums of values over a sequence's keys are fp32: what exceeds it is infinite.
  */

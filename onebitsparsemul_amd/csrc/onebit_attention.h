@@ -2,9 +2,10 @@
 //
 // Mathematics: out = sum_j p_j v_j / sum_j p_j with p_j = exp2(t_j - m), t_j = log2(e) scale k_scale q . k_code_j and m the largest t so far, in
 // one pass over the keys; where m grows, what is summed so far is multiplied by exp2(m_old - m). Codes are exact in fp16, and so
-// is q (bf16 rows as q 2^-e), so that the products of the matrix instructions are exact and their sums fp32. p_j takes its key's
-// v_scale by its power of two beside that of the keys around it, and some powers on top, so that fp16 keeps the bits of small p_j; the sums follow
-// that power exactly.
+// is q (bf16 rows as q 2^-e; what lies below 2^-33 of a row's largest value is lost), so that the products of the matrix instructions are exact and their sums
+// fp32. p_j takes its key's v_scale by its power of two beside that of the keys around it, and some powers on top, so that fp16 keeps the bits of small p_j; the
+// sums follow that power exactly. What p_j v_scale comes to below 2^-32 of the largest (2^-38 where rows are few)
+// counts as 0.
 //
 // Scores are computed as K Q^T: a lane then holds scores of one row of q (matrix column) and of the keys that the next product,
 // V^T P^T, wants from it as its own operand: p goes from one matrix instruction to the next without leaving its register.
@@ -137,7 +138,7 @@ struct Rows {
 };
 __device__ inline Rows first_row(int row, int group) { return row == 0 ? Rows{0, 0} : Rows{row / group, row % group}; }
 __device__ inline Rows behind(Rows first, int step, const AttentionArgs& args) {
-  // exact: numbers below group + 128, whose product with group is below 2^32
+  // exact: numbers below group + 256, whose product with group (at most 32768) is below 2^32
   const uint32_t n = first.head + step, tokens = args.group == 1 ? n : __umulhi(n, args.group_inverse);
   return {first.token + (int)tokens, (int)(n - tokens * args.group)};
 }

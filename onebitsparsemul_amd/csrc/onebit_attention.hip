@@ -3,7 +3,7 @@
 //
 // What bounds it: memory where sequences are long, and the chain of loads in front (lengths and pages, scales, codes) where they are not. One token behind
 // 131072, 32 heads of 128 on 8, int8: 54 us for 269 MB = 4.9 TB/s (a large copy reaches 5.1), with the join 59. Sixteen sequences of 500 to 4096
-// tokens: 19 us for 69 MB = 3.6 TB/s, the join 3 to 4; the matrix unit is busy in 5 % of the clocks, wavefronts wait for loads in half of theirs. One token
+// tokens: 19 to 20 us for 69 MB = 3.5 TB/s, the join 3 to 4; the matrix unit is busy in 5 % of the clocks, wavefronts wait for loads in half of theirs. One token
 // behind 1000, heads of 64: 5.5 us and the join 2 to 3, nearly all of it that chain and the two launches.
 // Why this split: sixteen rows are the columns of a matrix instruction; columns that few heads leave empty cost nothing beside the loads. Four wavefronts, each
 // with the next step's codes asked for as soon as this step's registers are free, keep enough bytes under way with three workgroups to a compute unit
@@ -412,7 +412,8 @@ hipError_t launch_as(const AttentionArgs& args, hipStream_t stream) {
 // Rows of q to a workgroup, and how its keys are split over workgroups where a call has fewer of them than the device holds at once.
 //
 // few_rows_kernel reads the keys for every 16 rows again but starts and ends quickly and fills the device with few rows; many_rows_kernel does
-// with a quarter of the work. Both sides of the rule, few | many, us: one prompt of 512, 8 heads of 64 on 4 (256 workgroups) 6.8 | 13.7; one of 1024, 8 of 128 on 4
+// with a quarter of the work. The rule's numbers stand between what was measured, no quantity of the device among them, and calls near them may be better off
+// on the other side. Both sides, few | many, us: one prompt of 512, 8 heads of 64 on 4 (256 workgroups) 6.8 | 13.7; one of 1024, 8 of 128 on 4
 // (512) 17.9 | 26.3; one of 512, 32 of 128 on 8 (1024) 19.5 | 23.0; eight of 128, 16 of 64 on 16 (1024, but of 64 keys) 10.2 | 7.4; two of 512, 32 of 64 on 8 (2048)
 // 21.2 | 14.4; 64 tokens behind 1936 in four sequences, 16 of 128 on 16 (256, 65 million values) 30.1 | 22.0; five of 37 to 512, 8 of 64 on 4 (1280, of which
 // 756 have rows) 12.4 | 14.7.
@@ -431,7 +432,7 @@ void plan_attention(AttentionArgs& args, int compute_units) {
   const bool few = rows <= 32 || (busy <= (keys_seen >= 256 ? 4ll : 3ll) * compute_units && busy * keys_seen * args.cache.head_dim <= 148000ll * compute_units);
   args.rows = few ? kRows : many_rows(args.cache.head_dim);
   const long long units = workgroups(args.rows);
-  // workgroups that the device holds
+  // workgroups that splits are made for (of many_rows_kernel's for heads of 64 the device would hold a third to a compute unit)
   const long long slots = (few ? 3ll : args.rows == 128 ? 2ll : 1ll) * compute_units;
   // (the join has a workgroup of up to 1024 threads to each row, and a launch less than 2^32 of them)
   const long long splits = (long long)q.tokens * args.heads < 1 << 22 ? std::max(1ll, slots / units) : 1;

@@ -6,12 +6,15 @@
 //
 // What bounds it: the matrix unit and the vector unit one after the other. Of a tile's 32 products a wavefront (1024 clocks) and some 200 vector
 // instructions (32 exponentials among them; 16 conversions and 8 byte permutations bring in its share of the next tile) the two wavefronts of a SIMD
-// overlap little: the matrix unit is busy in 36 % of the clocks, LDS in 27 %, and power takes 6 % (139 us on zeros). 4096 tokens, 32 heads of 128 on 8,
-// e4m3, bf16: 149 us = 920 TFLOP/s of the causal half, where a large bf16 matrix product of the library reaches 1330; 500 tokens behind 7500, 32 heads on 32,
-// int8, pages of 32: 97 us with 9 of the join = 650.
-// Why this tile: 128 rows (four wavefronts) read and convert each tile twice as often, 167 us; 64 rows to a wavefront do not fit its registers. Measured and
-// not kept: the wavefronts of a SIMD in turn, one multiplying while the other weighs, with a barrier at each change (148 us, the second call 100:
-// each is then bound by its own instructions' latencies); the loads two tiles ahead, 167; wave priorities, nothing.
+// overlap little: the matrix unit is busy in 37 % of the clocks, LDS in 27 %, and power takes 6 % (zeros: 139 us for 149 on one card). 4096 tokens, 32 heads of
+// 128 on 8, e4m3, bf16: 152 us (149 to 156 on different cards) = 900 TFLOP/s of the causal half, where a large bf16 matrix product of the library reaches 1330;
+// 500 tokens behind 7500, 32 heads on 32, int8, pages of 32: 98 us with 9 of the join = 650.
+// Why this tile: 128 rows (four wavefronts) read and convert each tile twice as often, 167 us for 149; 64 rows to a wavefront do not fit its registers.
+// Measured and not kept: the wavefronts of a SIMD in turn, one multiplying while the other weighs, with a barrier at each change (148 us for 149, the second
+// call 100 for 97: each is then bound by its own instructions' latencies); the loads two tiles ahead, 167; wave priorities, nothing.
+// p goes into the second product as one fp16: a second for the bits below, as where rows are few, would be half as many matrix instructions again, and the sum
+// of p is taken from the same rounded values. That costs up to 2^-11 of sum p |v| (the second call above stands 2.9e-4 from 64 bits, with p in fp32 2.1e-4: the
+// result's own rounding).
 #include "onebit_attention.h"
 
 #include <type_traits>
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(many_rows(D) * 2, 2) void many_rows_kernel(Attentio
       // four keys are half a piece of each dim's row; pieces are in the order in which the products want them
       const int group = (wave * kOwn + lane / kLanes * 4) / 4, half = group >> 1 & 1;
       const int value_at = made_here(value_place(lane % kLanes * kValueBytes, (group >> 2) * 2 + (group & 1)));
-uint32_t by_dim[4];
+      uint32_t by_dim[4];
       transpose_bytes(raw_v[0], raw_v[1], raw_v[2], raw_v[3], by_dim);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // the row's bits 0 and 1 in value_place()

@@ -140,7 +140,9 @@ constexpr int kUnit = 8;  // P of the cache's kernel
 
 // Keys or values of one page and head, in registers from the first read to the codes: THREADS x PASSES units. The scale is that of all the page's new tokens,
 // so a workgroup takes a page and head whole and no value is read twice. 2048 tokens, 32 heads of 128 on 8, fp16: 10.6 us for 47 MB = 4.4 TB/s (8192 tokens in
-// four sequences 41 us, 4.6). Sixteen sequences' single tokens: 4.5 us, the launch and the chain lengths, page, scale, codes.
+// four sequences 41 us, 4.6); int8 codes take 2 % more. Sixteen sequences' single tokens: 4.4 us, the launch and the chain lengths, page, scale, codes; 14 us where
+// scales grow: the codes of a page's older tokens, up to 63 here, then go through the workgroup four to a thread, one round behind the other. With tokens of one
+// distribution that is so for some 15 of the 256 pages and heads of such a call.
 template <int TYPE, int CODE, int THREADS, int PASSES>
 __device__ inline void append_page(const AppendArgs& args, const Sequence& seq, int s, int slot, int head, bool values) {
   __shared__ uint32_t most[THREADS / 64];

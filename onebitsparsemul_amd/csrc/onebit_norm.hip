@@ -207,6 +207,8 @@ hipError_t launch_norm(const onebit_norm& a, hipStream_t stream) {
   // h is read again by the next norm, with at least a projection between: of a quarter of the 256 MB of the last cache on it is written past the caches,
   // which leaves them to y (2048 x 8192, h fp32: 39.2 us for 46.3, and with the projections behind two such norms within 2 % either way;
   // 8192 x 4096 fp16 with them 319 for 324; y too past them: 40.3, and 1 to 2 % lost in what reads it; h of 16 rows: 0.6 of 14.8 us lost).
+  // By itself, past the caches | through them: h of 16 MB 10.8 | 11.9 us (512 x 8192 fp32), 32 MB 19.4 | 17.6 (1024 x 8192) and 23.9 | 27.4 (4096 x 4096 fp16),
+  // 48 MB 31.1 | 32.0, 64 MB 38.1 | 45.9 and 52.0 | 51.4 (8192 x 4096 fp16), 94 MB 58.2 | 60.8: below the quarter either way, and what reads h next finds it.
   const bool far = vectors && a.h_out && (long long)a.rows * a.hidden * (a.residual_dtype == ONEBIT_DTYPE_F32 ? 4 : 2) >= 64 << 20;
   auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3(a.rows), dim3(threads), 0, stream, a); };
   auto launch_as = [&](auto count) {

@@ -56,7 +56,7 @@ def rotary_table(positions, rotary_dim, base=10000.0, scaling=None, device="cuda
         def pair_of(turns):  # the (fractional) index of the pair that turns so often in the original positions
             return rotary_dim * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(base))
         first = max(math.floor(pair_of(scaling.get("fast", 32))), 0)
-        last = min(math.ceil(pair_of(scaling.get("slow", 1))), rotary_dim - 1)
+        last = min(math.ceil(pair_of(scaling.get("slow", 1))), rotary_dim - 1)  # (pairs end at rotary_dim / 2 - 1: the bound that models are trained with)
         stretched = ((index / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
         rates = rates * (1 - stretched) + rates / factor * stretched
         magnitude = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
