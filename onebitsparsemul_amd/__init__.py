@@ -11,6 +11,7 @@ import torch.nn as nn
 
 from . import _native
 from .decoder import QuantizedCache, block_norm, cache_append, cache_attention, rotary, rotary_table
+from .head import BlockLinear, block_linear, block_norm_codes, quantize_rows, quantize_weight, sample
 from ._semi_structured_conversions import (
     mask_creator,
     sparse_semi_structured_from_dense_cutlass,
@@ -22,6 +23,7 @@ __all__ = [
     "py_binary_gemm", "BinaryLinear_2_4", "PreparedWeight", "mask_creator", "sparse_semi_structured_from_dense_cutlass",
     "sparse_semi_structured_to_dense_cutlass", "set_weight_cache", "clear_weight_cache",
     "QuantizedCache", "block_norm", "cache_append", "cache_attention", "rotary", "rotary_table",
+    "BlockLinear", "block_linear", "block_norm_codes", "quantize_rows", "quantize_weight", "sample",
 ]
 
 

@@ -42,7 +42,8 @@ def build_library():
     objs, cmds = [], []
     for src in ("onebit_gemm.hip", "onebit_gemm_tokens.hip", "onebit_skinny.hip", "onebit_skinny_tokens.hip",
                 "onebit_wide.hip", "onebit_wide_tokens.hip", "onebit_format.hip", "onebit_capi.hip", "onebit_diag.hip",
-                "onebit_cache.hip", "onebit_attention.hip", "onebit_attention_tiles.hip", "onebit_norm.hip", "onebit_decoder_capi.hip"):
+                "onebit_cache.hip", "onebit_attention.hip", "onebit_attention_tiles.hip", "onebit_norm.hip", "onebit_decoder_capi.hip",
+                "onebit_codes.hip", "onebit_block.hip", "onebit_sample.hip", "onebit_head_capi.hip"):
         obj = os.path.join(CSRC, src.replace(".hip", ".o"))
         cmds.append([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
         objs.append(obj)
@@ -73,7 +74,7 @@ def build_binding():
     flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    objs = [os.path.join(CSRC, name + ".o") for name in ("torch_binding", "torch_decoder")]
+    objs = [os.path.join(CSRC, name + ".o") for name in ("torch_binding", "torch_decoder", "torch_head")]
     _run_side_by_side([["g++", *flags, *inc, "-c", obj[:-2] + ".cpp", "-o", obj] for obj in objs])
     cmd = ["g++", "-shared", *objs, "-o", out,
            "-L", PKG, "-lonebitmul", "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",

@@ -17,27 +17,6 @@ namespace onebit {
 
 constexpr float kLog2E = 1.44269504088896340736f;
 
-// Four codes of a word as fp16, exact. e4m3 by the conversion instruction; int8: the byte plus 128 as the low byte of 1024 + n, minus 1152.
-template <int CODE>
-__device__ inline void codes_to_f16(uint32_t word, h2_t& low, h2_t& high) {
-  if constexpr (CODE == ONEBIT_CODE_E4M3) {
-    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false));
-    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true));
-  } else {
-    const uint32_t shifted = word ^ 0x80808080u;
-    const h2_t offset = {(_Float16)1152.f, (_Float16)1152.f};
-    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04010400u)) - offset;
-    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04030402u)) - offset;
-  }
-}
-template <int CODE>
-__device__ inline h8_t codes_to_f16(uint32_t first, uint32_t second) {
-  h2_t a, b, c, d;
-  codes_to_f16<CODE>(first, a, b);
-  codes_to_f16<CODE>(second, c, d);
-  return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
 // Words of four tokens' codes at four dims -> words of four dims' codes of the four tokens
 __device__ inline void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&out)[4]) {
   const uint32_t ab_low = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_high = __builtin_amdgcn_perm(b, a, 0x07030602u);

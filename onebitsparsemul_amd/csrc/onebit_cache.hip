@@ -108,24 +108,6 @@ hipError_t launch_rotary_type(const RotaryArgs& args, hipStream_t stream) {
 // ---- the write side of the cache
 
 template <int CODE>
-__device__ inline float most_code() { return CODE == ONEBIT_CODE_INT8 ? kMostInt8 : kMostE4M3; }
-
-// value / scale as a code; four of them in a word. `inside`: the scale is finite and not 0.
-template <int CODE>
-__device__ inline uint32_t encode4(const float* x, float scale, bool inside) {
-  float q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = inside ? fminf(fmaxf(x[i] / scale, -most_code<CODE>()), most_code<CODE>()) : 0.f;
-  if (CODE == ONEBIT_CODE_INT8) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) word |= ((uint32_t)(int)rintf(q[i]) & 0xff) << (8 * i);
-    return word;
-  }
-  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], low, true);
-}
-template <int CODE>
 __device__ inline void decode4(uint32_t word, float* x) {
   if (CODE == ONEBIT_CODE_INT8) {
 #pragma unroll

@@ -1,28 +1,15 @@
 // C ABI of onebit_decoder.h: argument validation and launches. Host code only.
+#include "onebit_decoder_checks.h"
 #include "onebit_decoder_launch.h"
 
 #include <algorithm>
-#include <cstdarg>
-#include <cstdio>
 
 namespace {
 
-int fail(int code, const char* fmt, ...) {
-  char text[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(text, sizeof text, fmt, ap);
-  va_end(ap);
-  return onebit::report(code, text);
-}
-template <class... Values>
-int refuse(const char* fmt, Values... values) { return fail(ONEBIT_ERR_ARGUMENT, fmt, values...); }
-int launched(hipError_t status, const char* what) {
-  return status == hipSuccess ? ONEBIT_OK : fail(ONEBIT_ERR_HIP, "HIP error '%s' from %s", hipGetErrorString(status), what);
-}
-
-bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-bool is_type(int dtype) { return dtype == ONEBIT_DTYPE_F32 || dtype == ONEBIT_DTYPE_F16 || dtype == ONEBIT_DTYPE_BF16; }
+using onebit::aligned;
+using onebit::is_type;
+using onebit::launched;
+using onebit::refuse;
 
 int check_cache(const onebit_cache* c) {
   if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return refuse("null pointer in the cache");
@@ -53,8 +40,17 @@ int check_table(const float* table, int rows, int rotary_dim, int head_dim) {
   if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim) return refuse("rotary_dim = %d must be even, from 2 to head_dim = %d", rotary_dim, head_dim);
   return ONEBIT_OK;
 }
-#define CHECKED(call) \
-  if (const int code_ = (call)) return code_
+// (y apart)
+int check_norm(const onebit_norm& n) {
+  if (n.rows < 1 || n.hidden < 1 || n.hidden > 32768) return refuse("rows must be positive and hidden 1 to 32768 (got %d, %d)", n.rows, n.hidden);
+  if (n.kind != 0 && n.kind != 1) return refuse("kind must be 0 (rms) or 1 (layer), got %d", n.kind);
+  if ((n.x && !is_type(n.x_dtype)) || !is_type(n.residual_dtype) || !is_type(n.weight_dtype) || (n.gate && !is_type(n.gate_dtype)))
+    return refuse("dtype codes must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+  if (!n.x && (n.post_weight || n.gate)) return refuse("a norm behind the block and a gate need the block's output x");
+  if (n.post_bias && !n.post_weight) return refuse("post_bias needs post_weight");
+  if (n.gate && n.gate_column_stride != 0 && n.gate_column_stride != 1) return refuse("gate_column_stride must be 0 or 1 (got %d)", n.gate_column_stride);
+  return ONEBIT_OK;
+}
 
 onebit_sequences planned(const onebit_sequences& q) {
   onebit_sequences r = q;
@@ -144,14 +140,17 @@ int onebit_cache_attention(const onebit_cache* cache, const onebit_sequences* se
 int onebit_block_norm(const onebit_norm* n, void* stream) {
   onebit::report(ONEBIT_OK, "");
   if (!n || !n->residual || !n->y || !n->weight) return refuse("residual, y and weight must not be null");
-  if (n->rows < 1 || n->hidden < 1 || n->hidden > 32768) return refuse("rows must be positive and hidden 1 to 32768 (got %d, %d)", n->rows, n->hidden);
-  if (n->kind != 0 && n->kind != 1) return refuse("kind must be 0 (rms) or 1 (layer), got %d", n->kind);
-  if ((n->x && !is_type(n->x_dtype)) || !is_type(n->residual_dtype) || !is_type(n->y_dtype) || !is_type(n->weight_dtype) || (n->gate && !is_type(n->gate_dtype)))
-    return refuse("dtype codes must be 0 (fp32), 1 (fp16) or 2 (bf16)");
-  if (!n->x && (n->post_weight || n->gate)) return refuse("a norm behind the block and a gate need the block's output x");
-  if (n->post_bias && !n->post_weight) return refuse("post_bias needs post_weight");
-  if (n->gate && n->gate_column_stride != 0 && n->gate_column_stride != 1) return refuse("gate_column_stride must be 0 or 1 (got %d)", n->gate_column_stride);
-  return launched(onebit::launch_norm(*n, (hipStream_t)stream), "onebit_block_norm");
+  if (!is_type(n->y_dtype)) return refuse("dtype codes must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+  CHECKED(check_norm(*n));
+  return launched(onebit::launch_norm(*n, nullptr, (hipStream_t)stream), "onebit_block_norm");
+}
+
+int onebit_block_norm_codes(const onebit_norm* n, const onebit_codes* out, void* stream) {
+  onebit::report(ONEBIT_OK, "");
+  if (!n || !n->residual || !n->weight) return refuse("residual and weight must not be null");
+  CHECKED(check_norm(*n));
+  CHECKED(onebit::check_codes(out, "the result"));
+  return launched(onebit::launch_norm(*n, out, (hipStream_t)stream), "onebit_block_norm_codes");
 }
 
 }  // extern "C"

@@ -60,20 +60,68 @@ constexpr float kMostE4M3 = 448.f, kMostInt8 = 127.f;
 // Magnitudes as integers: their order is that of the floats, and NaN is the largest, so that a maximum does not lose it.
 __device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Over the 64 lanes, the same in each: neighbours, pairs, halves of a row of 16 and rows by cross-lane moves, then rows and halves by swaps.
+template <int CODE>
+__device__ inline float most_code() { return CODE == ONEBIT_CODE_INT8 ? kMostInt8 : kMostE4M3; }
+
+// value / scale as a code; four of them in a word. `inside`: the scale is finite and not 0.
+template <int CODE>
+__device__ inline uint32_t encode4(const float* x, float scale, bool inside) {
+  float q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = inside ? fminf(fmaxf(x[i] / scale, -most_code<CODE>()), most_code<CODE>()) : 0.f;
+  if (CODE == ONEBIT_CODE_INT8) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) word |= ((uint32_t)(int)rintf(q[i]) & 0xff) << (8 * i);
+    return word;
+  }
+  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], low, true);
+}
+
+// Four codes of a word as fp16, exact. e4m3 by the conversion instruction; int8: the byte plus 128 as the low byte of 1024 + n, minus 1152.
+template <int CODE>
+__device__ inline void codes_to_f16(uint32_t word, h2_t& low, h2_t& high) {
+  if constexpr (CODE == ONEBIT_CODE_E4M3) {
+    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false));
+    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true));
+  } else {
+    const uint32_t shifted = word ^ 0x80808080u;
+    const h2_t offset = {(_Float16)1152.f, (_Float16)1152.f};
+    low = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04010400u)) - offset;
+    high = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04030402u)) - offset;
+  }
+}
+template <int CODE>
+__device__ inline h8_t codes_to_f16(uint32_t first, uint32_t second) {
+  h2_t a, b, c, d;
+  codes_to_f16<CODE>(first, a, b);
+  codes_to_f16<CODE>(second, c, d);
+  return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Over 16 neighbouring lanes, the same in each: neighbours, pairs, halves of the 16 and of the eights by cross-lane moves. All lanes take part.
 template <class Value, class Combine>
-__device__ inline Value over_wave(Value x, Combine combine) {
+__device__ inline Value over_row(Value x, Combine combine) {
   auto moved = [&](auto pattern) {
     return __builtin_bit_cast(Value, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(pattern)::value, 0xf, 0xf, true));
   };
   x = combine(x, moved(std::integral_constant<int, 0xb1>()));   // lane ^ 1
   x = combine(x, moved(std::integral_constant<int, 0x4e>()));   // lane ^ 2
   x = combine(x, moved(std::integral_constant<int, 0x141>()));  // the other four of eight
-  x = combine(x, moved(std::integral_constant<int, 0x140>()));  // the other eight of sixteen
+  return combine(x, moved(std::integral_constant<int, 0x140>()));  // the other eight of sixteen
+}
+// Over the 64 lanes, the same in each: rows of 16, then rows and halves by swaps.
+template <class Value, class Combine>
+__device__ inline Value over_wave(Value x, Combine combine) {
+  x = over_row(x, combine);
   auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
   x = combine(__builtin_bit_cast(Value, (uint32_t)r[0]), __builtin_bit_cast(Value, (uint32_t)r[1]));
   r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
   return combine(__builtin_bit_cast(Value, (uint32_t)r[0]), __builtin_bit_cast(Value, (uint32_t)r[1]));
+}
+__device__ inline uint32_t row_max(uint32_t x) {
+  return over_row(x, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 __device__ inline uint32_t wave_max(uint32_t x) {
   return over_wave(x, [](uint32_t a, uint32_t b) { return max(a, b); });

@@ -2,6 +2,7 @@
 // onebit_decoder.h, checked.
 #pragma once
 #include "onebit_decoder.h"
+#include "onebit_head.h"
 #include "onebit_launch.h"
 
 namespace onebit {
@@ -50,6 +51,6 @@ size_t attention_workspace(const AttentionArgs& args);
 hipError_t launch_attention(const AttentionArgs& args, hipStream_t stream);
 hipError_t launch_many_rows(const AttentionArgs& args, hipStream_t stream);  // without the pass that joins splits
 
-hipError_t launch_norm(const onebit_norm& args, hipStream_t stream);
+hipError_t launch_norm(const onebit_norm& args, const onebit_codes* codes, hipStream_t stream);  // codes: where y goes as such, or NULL
 
 }  // namespace onebit

@@ -1,7 +1,7 @@
 // The norms around a block (onebit_decoder.h): one workgroup for each row, the row in registers from its one read to its one write.
 // Bound by memory: 2048 x 8192, norm on both sides, residuals in fp32, 39.2 us for 201 MB = 5.1 TB/s, as a large copy. Small calls by the launch and one round
 // of loads, so every operand of a row is requested before the first is used: 16 x 4096 3.3 us.
-#include "onebit_decoder_device.h"
+#include "onebit_codes.h"
 #include "onebit_decoder_launch.h"
 
 namespace onebit {
@@ -109,9 +109,10 @@ __device__ inline void normalise(float (&x)[VECTORS][kVector], const onebit_norm
     for (int i = 0; i < kVector; ++i) x[v][i] *= factor;
 }
 
-// WHOLE: every vector is eight values at a multiple of 16 bytes. FAR: h goes past the caches.
-template <int VECTORS, bool WHOLE, bool FAR>
-__global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
+// WHOLE: every vector is eight values at a multiple of 16 bytes. FAR: h goes past the caches. CODES: y leaves as 8-bit codes; 16 neighbouring threads, which
+// are in one wavefront, hold the 128 values of a scale, and threads behind the row's end the zeros of its last group.
+template <int VECTORS, bool WHOLE, bool FAR, bool CODES>
+__device__ inline void norm_row(const onebit_norm& a, const onebit_codes& codes) {
   __shared__ float parts[16];
   const long long row = blockIdx.x;
   const int stride = blockDim.x * kVector;
@@ -177,29 +178,40 @@ __global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
   normalise(h, a, parts);
 #pragma unroll
   for (int v = 0; v < VECTORS; ++v) {
-    if (left[v] <= 0) continue;
+    if (left[v] <= 0 && !CODES) continue;
     float w[kVector];
-    widen(EAGER ? weight : load_weight(a.weight, v), a.weight_dtype, w);
+    if (left[v] > 0) {
+      widen(EAGER ? weight : load_weight(a.weight, v), a.weight_dtype, w);
 #pragma unroll
-    for (int i = 0; i < kVector; ++i) h[v][i] *= w[i];
-    if (a.bias) {
-      widen(EAGER ? bias : load_weight(a.bias, v), a.weight_dtype, w);
+      for (int i = 0; i < kVector; ++i) h[v][i] *= w[i];
+      if (a.bias) {
+        widen(EAGER ? bias : load_weight(a.bias, v), a.weight_dtype, w);
 #pragma unroll
-      for (int i = 0; i < kVector; ++i) h[v][i] += w[i];
+        for (int i = 0; i < kVector; ++i) h[v][i] += w[i];
+      }
     }
-    store_row<WHOLE, false>(a.y, a.y_dtype, row * a.y_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
+    if (CODES) store_codes(codes, row, threadIdx.x * kVector + v * stride, threadIdx.x * kVector + v * stride < padded_columns(a.hidden), h[v]);
+    else store_row<WHOLE, false>(a.y, a.y_dtype, row * a.y_stride + threadIdx.x * kVector + v * stride, left[v], h[v]);
   }
+}
+template <int VECTORS, bool WHOLE, bool FAR>
+__global__ __launch_bounds__(1024) void norm_kernel(onebit_norm a) {
+  norm_row<VECTORS, WHOLE, FAR, false>(a, {});
+}
+template <int VECTORS, bool WHOLE, bool FAR>
+__global__ __launch_bounds__(1024) void norm_codes_kernel(onebit_norm a, onebit_codes codes) {
+  norm_row<VECTORS, WHOLE, FAR, true>(a, codes);
 }
 
 bool whole(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % kVector == 0; }
 
 }  // namespace
 
-hipError_t launch_norm(const onebit_norm& a, hipStream_t stream) {
+hipError_t launch_norm(const onebit_norm& a, const onebit_codes* codes, hipStream_t stream) {
   const bool vectors = a.hidden % kVector == 0 && whole(a.x, a.x ? a.x_stride : 0) && whole(a.residual, a.residual_stride) &&
-                       whole(a.h_out, a.h_out ? a.h_stride : 0) && whole(a.y, a.y_stride) && whole(a.weight, 0) && whole(a.bias, 0) &&
+                       whole(a.h_out, a.h_out ? a.h_stride : 0) && (codes || whole(a.y, a.y_stride)) && whole(a.weight, 0) && whole(a.bias, 0) &&
                        whole(a.post_weight, 0) && whole(a.post_bias, 0) && (!a.gate_column_stride || whole(a.gate, a.gate_row_stride));
-  const int units = (a.hidden + kVector - 1) / kVector;
+  const int units = ((codes ? padded_columns(a.hidden) : a.hidden) + kVector - 1) / kVector;
   // One vector to a thread is the shortest way for few rows (16 x 4096 3.6 us, with two 4.4). Of many long rows a compute unit then holds one at a time
   // and waits for it: two vectors, half the wavefronts, and the next row under way (2048 x 8192 with a norm behind the block 51.0 us, with two 40.3).
   const int per_thread = units <= 1024 && (units < 512 || a.rows < 512) ? 1 : units <= 2048 ? 2 : 4;
@@ -210,10 +222,14 @@ hipError_t launch_norm(const onebit_norm& a, hipStream_t stream) {
   // By itself, past the caches | through them: h of 16 MB 10.8 | 11.9 us (512 x 8192 fp32), 32 MB 19.4 | 17.6 (1024 x 8192) and 23.9 | 27.4 (4096 x 4096 fp16),
   // 48 MB 31.1 | 32.0, 64 MB 38.1 | 45.9 and 52.0 | 51.4 (8192 x 4096 fp16), 94 MB 58.2 | 60.8: below the quarter either way, and what reads h next finds it.
   const bool far = vectors && a.h_out && (long long)a.rows * a.hidden * (a.residual_dtype == ONEBIT_DTYPE_F32 ? 4 : 2) >= 64 << 20;
-  auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3(a.rows), dim3(threads), 0, stream, a); };
+  auto launch = [&](auto kernel, auto codes_kernel) {
+    return codes ? launch_kernel(codes_kernel, dim3(a.rows), dim3(threads), 0, stream, a, *codes) : launch_kernel(kernel, dim3(a.rows), dim3(threads), 0, stream, a);
+  };
   auto launch_as = [&](auto count) {
     constexpr int kVectors = decltype(count)::value;
-    return far ? launch(norm_kernel<kVectors, true, true>) : vectors ? launch(norm_kernel<kVectors, true, false>) : launch(norm_kernel<kVectors, false, false>);
+    return far       ? launch(norm_kernel<kVectors, true, true>, norm_codes_kernel<kVectors, true, true>)
+           : vectors ? launch(norm_kernel<kVectors, true, false>, norm_codes_kernel<kVectors, true, false>)
+                     : launch(norm_kernel<kVectors, false, false>, norm_codes_kernel<kVectors, false, false>);
   };
   if (per_thread == 1) return launch_as(std::integral_constant<int, 1>());
   if (per_thread == 2) return launch_as(std::integral_constant<int, 2>());

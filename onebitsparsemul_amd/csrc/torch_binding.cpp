@@ -311,4 +311,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prepare", &prepare, NoGil());
   m.def("pack_weight", &pack_weight, NoGil());
   bind_decoder(m);
+  bind_head(m);
 }

@@ -30,5 +30,6 @@ inline torch::Tensor empty_result(at::IntArrayRef sizes, c10::ScalarType type, c
   return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
 }
 
-// torch_decoder.cpp
+// torch_decoder.cpp, torch_head.cpp
 void bind_decoder(pybind11::module_& m);
+void bind_head(pybind11::module_& m);

@@ -1,9 +1,9 @@
 // Torch side of onebit_decoder.h: checks of the operands, results, workspace and the current stream. Operands that the kernels
 // do not read where they lie (rows inside a head that are no whole 16-byte units, a negated view, elements on which a result given by the caller is
 // written in another order) are copied first.
-#include "torch_binding.h"
+#include "torch_operands.h"
 
-#include "onebit_decoder.h"
+#include "onebit_head.h"
 
 #include <ATen/MemoryOverlap.h>
 
@@ -13,54 +13,6 @@
 
 namespace {
 
-void check_gpu(const torch::Tensor& t, const char* name, const c10::Device& device) {
-  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == device, name, " must live on ", device, ", got ", t.device());
-}
-
-// A contiguous vector or matrix of the call's plan, as it is
-void check_table(const torch::Tensor& t, const char* name, c10::ScalarType type, int64_t dims, const c10::Device& device) {
-  check_gpu(t, name, device);
-  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-  TORCH_CHECK_VALUE(t.dim() == dims && t.is_contiguous() && !t.is_neg(), name, " must be contiguous with ", dims, " dimensions, got shape ", t.sizes());
-}
-
-// The bytes from a tensor's first element to its last
-std::pair<const char*, const char*> extent(const torch::Tensor& t) {
-  int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-  const char* const first = (const char*)t.data_ptr();
-  return {first, first + (last + 1) * t.element_size()};
-}
-// Whether sum of x_i step_i = distance for some x_i from -below_i to above_i; true also where there are many to try. Steps from the largest on.
-struct Step {
-  int64_t step, below, above;
-};
-bool reaches(const std::vector<Step>& steps, size_t from, int64_t distance) {
-  if (from == steps.size()) return distance == 0;
-  int64_t low = 0, high = 0;  // of the others
-  for (size_t i = from + 1; i < steps.size(); ++i) low -= steps[i].step * steps[i].below, high += steps[i].step * steps[i].above;
-  const Step s = steps[from];
-  int tries = 0;
-  for (int64_t x = std::max(-s.below, (distance - high) / s.step - 1); x <= std::min(s.above, (distance - low) / s.step + 1); ++x)
-    if (++tries > 8 || reaches(steps, from + 1, distance - x * s.step)) return true;
-  return false;
-}
-// Whether two tensors may have memory in common: exactly for views that go through it in the same steps, else by their extents.
-bool may_meet(const torch::Tensor& a, const torch::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto one = extent(a), other = extent(b);
-  if (one.second <= other.first || other.second <= one.first) return false;
-  const int64_t distance = other.first - one.first, size = a.element_size();
-  if (a.dim() != b.dim() || b.element_size() != size || distance % size) return true;
-  std::vector<Step> steps;
-  for (int64_t i = 0; i < a.dim(); ++i) {
-    if (a.size(i) > 1 && b.size(i) > 1 && a.stride(i) != b.stride(i)) return true;
-    const int64_t step = a.size(i) > 1 ? a.stride(i) : b.stride(i);
-    if (step != 0 && (a.size(i) > 1 || b.size(i) > 1)) steps.push_back({step, b.size(i) - 1, a.size(i) - 1});
-  }
-  std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.step > y.step; });
-  return reaches(steps, 0, distance / size);
-}
 // Whether two tensors are the same element by element
 bool are_same(const torch::Tensor& a, const torch::Tensor& b) {
   if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
@@ -234,16 +186,12 @@ torch::Tensor cache_attention(const torch::Tensor& q, const torch::Tensor& k_cac
   return y;
 }
 
-// (rows, hidden) from (..., hidden), a view or a copy
-torch::Tensor rows_of(const torch::Tensor& t, int64_t hidden) {
-  torch::Tensor r = t.dim() == 2 ? t : t.reshape({-1, hidden});
-  return (r.stride(1) == 1 || hidden == 1) && !r.is_neg() ? r : r.resolve_neg().clone(at::MemoryFormat::Contiguous);
-}
-
-std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, const torch::Tensor& residual, const torch::Tensor& weight,
-                                                    const OptionalTensor& bias, const OptionalTensor& post_weight, const OptionalTensor& post_bias,
-                                                    const OptionalTensor& gate, double residual_scale, double block_scale, double eps,
-                                                    const std::string& kind, std::optional<c10::ScalarType> out_dtype, const OptionalTensor& residual_out) {
+// (h, y, scales): y as codes, or in its type and no scales
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> normed(const OptionalTensor& x, const torch::Tensor& residual, const torch::Tensor& weight,
+                                                               const OptionalTensor& bias, const OptionalTensor& post_weight, const OptionalTensor& post_bias,
+                                                               const OptionalTensor& gate, double residual_scale, double block_scale, double eps,
+                                                               const std::string& kind, std::optional<c10::ScalarType> out_dtype,
+                                                               const OptionalTensor& residual_out, bool as_codes) {
   at::AutoDispatchBelowADInplaceOrView guard_dispatch;
   const c10::Device device = residual.device();
   TORCH_CHECK_VALUE(residual.is_cuda() && residual.dim() >= 1, "residual must live on the GPU with shape (..., hidden)");
@@ -274,11 +222,13 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
                           residual_out->is_contiguous() && !residual_out->is_neg(),
                       "residual_out must be contiguous with the residual's shape and type");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
-  torch::Tensor y = empty_result(residual.sizes(), y_type, device);
+  torch::Tensor y, scales;
+  if (as_codes) std::tie(y, scales) = empty_codes(residual.sizes(), device);
+  else y = empty_result(residual.sizes(), y_type, device);
   // without a block the residual is only normed, unless it is scaled or wanted elsewhere
   const bool writes = x.has_value() || residual_scale != 1.0 || (residual_out.has_value() && (!are_same(residual, *residual_out) || residual.is_neg()));
   torch::Tensor h = residual_out.has_value() ? *residual_out : writes ? empty_result(residual.sizes(), residual.scalar_type(), device) : residual;
-  if (residual.numel() == 0) return {h, y};
+  if (residual.numel() == 0) return {h, y, scales};
   const bool given = residual_out.has_value();
   auto read = [&](const torch::Tensor& t) { return given ? beside(t, h) : t; };
   const torch::Tensor residual_rows = rows_of(read(residual), hidden), x_rows = x.has_value() ? rows_of(read(*x), hidden) : residual_rows;
@@ -323,8 +273,29 @@ std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, con
   n.residual_scale = (float)residual_scale;
   n.block_scale = (float)block_scale;
   n.eps = (float)eps;
-  check_status(onebit_block_norm(&n, current_stream(device)));
+  if (as_codes) {
+    const onebit_codes codes = codes_of(y, scales);
+    check_status(onebit_block_norm_codes(&n, &codes, current_stream(device)));
+  } else {
+    check_status(onebit_block_norm(&n, current_stream(device)));
+  }
+  return {h, y, scales};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> block_norm(const OptionalTensor& x, const torch::Tensor& residual, const torch::Tensor& weight,
+                                                    const OptionalTensor& bias, const OptionalTensor& post_weight, const OptionalTensor& post_bias,
+                                                    const OptionalTensor& gate, double residual_scale, double block_scale, double eps,
+                                                    const std::string& kind, std::optional<c10::ScalarType> out_dtype, const OptionalTensor& residual_out) {
+  auto [h, y, scales] = normed(x, residual, weight, bias, post_weight, post_bias, gate, residual_scale, block_scale, eps, kind, out_dtype, residual_out, false);
   return {h, y};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> block_norm_codes(const OptionalTensor& x, const torch::Tensor& residual, const torch::Tensor& weight,
+                                                                         const OptionalTensor& bias, const OptionalTensor& post_weight,
+                                                                         const OptionalTensor& post_bias, const OptionalTensor& gate, double residual_scale,
+                                                                         double block_scale, double eps, const std::string& kind,
+                                                                         const OptionalTensor& residual_out) {
+  return normed(x, residual, weight, bias, post_weight, post_bias, gate, residual_scale, block_scale, eps, kind, std::nullopt, residual_out, true);
 }
 
 }  // namespace
@@ -335,4 +306,5 @@ void bind_decoder(pybind11::module_& m) {
   m.def("cache_append", &cache_append, NoGil());
   m.def("cache_attention", &cache_attention, NoGil());
   m.def("block_norm", &block_norm, NoGil());
+  m.def("block_norm_codes", &block_norm_codes, NoGil());
 }

@@ -1,0 +1,483 @@
+"""From the last layer to the next tokens against plain implementations in 64 bits.
+
+u is the unit roundoff of a result's type (fp16 2^-11, bf16 2^-8, fp32 2^-24). Codes are those of the definition in fp32, to the bit, where they come from given values. Products
+of codes are exact in fp32; a sum over a group of 128, over the groups and with the scales takes at most 128 + 3 groups + 2 fp32 operations, each off by less than
+2^-23 (a matrix unit that cuts off included) of the sum of all magnitudes. Tokens are whole: equal to those of sums in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import onebitsparsemul_amd as onebit
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}
+E4M3 = torch.float8_e4m3fn
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def generator(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def padded(columns):
+    return -(-columns // 128) * 128
+
+
+def want_codes(x):
+    """The definition in fp32, on the host"""
+    x = x.float().cpu()
+    columns = x.shape[-1]
+    x = torch.nn.functional.pad(x.reshape(-1, columns), (0, padded(columns) - columns)).view(-1, padded(columns) // 128, 128)
+    largest = x.abs().amax(-1)
+    scale = largest / 448
+    fine = ((scale > 0) & torch.isfinite(scale))[..., None]
+    codes = torch.where(fine, x / torch.where(fine, scale[..., None], 1.0), 0.0).clamp(-448, 448).to(E4M3)
+    return codes.flatten(1), scale
+
+
+def same(a, b):
+    """Equal to the bit, NaN with NaN; codes 0 of either sign"""
+    a, b = a.cpu().float(), b.cpu().float()
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+# ---- codes
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,columns", [(1, 1), (1, 7), (3, 127), (2, 128), (5, 129), (17, 512), (33, 1000), (4, 1408), (7, 5001), (300, 8192)])
+def test_rows_as_codes(dtype, rows, columns):
+    g = generator(columns)
+    x = (torch.randn((rows, columns), generator=g) * torch.exp(3 * torch.randn((rows, columns), generator=g))).to(dtype)
+    codes, scales = onebit.quantize_rows(x.cuda())
+    assert codes.dtype == E4M3 and codes.shape == (rows, padded(columns)) and scales.shape == (rows, padded(columns) // 128)
+    want, scale = want_codes(x)
+    assert same(codes, want) and same(scales, scale)
+
+
+def test_rows_of_zeros_of_little_and_of_what_is_not_finite():
+    x = torch.randn((8, 300), generator=generator(1))
+    x[0] = 0
+    x[1, 128:256] = 0
+    x[2, 5], x[3, 200], x[4, 299], x[5, 1] = math.nan, math.inf, -math.inf, -math.nan
+    x[6] *= 1e-42  # subnormal, and a scale that is 0 or a few of the least
+    x[7] *= 1e37
+    codes, scales = onebit.quantize_rows(x.cuda())
+    want, scale = want_codes(x)
+    assert same(codes, want) and same(scales, scale)
+    assert bool(torch.isnan(scales[2, 0])) and bool(torch.isinf(scales[3, 1])) and float(scales[0].abs().sum()) == 0
+    y = onebit.block_linear(codes, scales, *onebit.quantize_weight(torch.randn((40, 300)).cuda()), out_dtype=torch.float32)
+    assert bool(torch.isnan(y[2:6]).all()) and bool(torch.isfinite(y[[0, 1, 6]]).all()) and bool((y[0] == 0).all())
+
+
+def test_rows_that_are_strided_shaped_or_none():
+    x = torch.randn((6, 5, 700), generator=generator(2)).half().cuda()
+    base = onebit.quantize_rows(x)
+    assert base[0].shape == (6, 5, 768) and base[1].shape == (6, 5, 6)
+    for view in (x[:, 2], x[..., 3:131], x[..., ::2], x.transpose(0, 1), x[1:4, :, 1:], x.expand(6, 5, 700), x[:, :, :1], torch._neg_view(x)):
+        codes, scales = onebit.quantize_rows(view)
+        want, scale = want_codes(view)
+        assert same(codes.flatten(0, -2), want) and same(scales.flatten(0, -2), scale)
+    assert onebit.quantize_rows(x[0, 0])[0].shape == (768,) and onebit.quantize_rows(x[:0])[1].shape == (0, 5, 6)
+    assert onebit.quantize_rows(x[..., :0])[0].shape == (6, 5, 0)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("rows,hidden,dtype,residual", [(1, 512, torch.float16, torch.float16), (16, 4096, torch.bfloat16, torch.float32), (3, 1000, torch.float32, torch.float32),
+                                                        (5, 77, torch.float16, torch.float32), (600, 8192, torch.bfloat16, torch.bfloat16), (2, 20000, torch.float16, torch.float16),
+                                                        (2, 32768, torch.float32, torch.float32), (2, 16500, torch.float16, torch.float32), (700, 5000, torch.float16, torch.float16)])
+def test_norms_as_codes(kind, post, rows, hidden, dtype, residual):
+    """The codes of block_norm's fp32 result, to the bit, and its h"""
+    g = generator(hidden + rows)
+    make = lambda shape, t, std=1.0: (torch.randn(shape, generator=g) * std).to(t).cuda()  # noqa: E731
+    x, r, weight = make((rows, hidden), dtype, 2), make((rows, hidden), residual, 3), make((hidden,), dtype)
+    options = dict(bias=make((hidden,), dtype), post_weight=make((hidden,), dtype) if post else None, gate=make((rows, 1), dtype), residual_scale=0.7, block_scale=0.3, kind=kind)
+    h, codes, scales = onebit.block_norm_codes(x, r, weight, **options)
+    want_h, y = onebit.block_norm(x, r, weight, out_dtype=torch.float32, **options)
+    assert torch.equal(h, want_h)
+    want, scale = want_codes(y)
+    assert same(codes, want) and same(scales, scale)
+
+
+def test_norms_as_codes_in_place_without_a_block_and_of_what_is_not_finite():
+    g = generator(4)
+    x, r = (torch.randn((2, 9, 640), generator=g).half().cuda() for _ in range(2))
+    weight = torch.randn(640, generator=g).half().cuda()
+    h, codes, scales = onebit.block_norm_codes(None, r, weight)
+    assert h is not x and torch.equal(h, r) and codes.shape == (2, 9, 640) and scales.shape == (2, 9, 5)
+    want, scale = want_codes(onebit.block_norm(None, r, weight, out_dtype=torch.float32)[1])
+    assert same(codes.flatten(0, 1), want) and same(scales.flatten(0, 1), scale)
+    want = onebit.block_norm_codes(x, r, weight)
+    in_place = r.clone()
+    got = onebit.block_norm_codes(x, in_place, weight, residual_out=in_place)
+    assert torch.equal(got[0], want[0]) and torch.equal(in_place, want[0]) and same(got[1], want[1]) and torch.equal(got[2], want[2])
+    x[0, 3, 100] = math.nan
+    _, codes, scales = onebit.block_norm_codes(x, r, weight)
+    assert bool(torch.isnan(scales[0, 3]).all()) and bool((codes[0, 3].float() == 0).all()) and int(torch.isnan(scales).sum()) == 5
+    # a row of the fused projection's output, as the last tokens of sequences are
+    last = onebit.block_norm_codes(x[:, -1], r[:, -1], weight)
+    assert same(last[1], want[1][:, -1]) and torch.equal(last[0], want[0][:, -1])
+    assert onebit.block_norm_codes(x[:, :0], r[:, :0], weight)[1].shape == (2, 0, 640)
+
+
+# ---- products
+
+
+def random_codes(rows, columns, g, group_rows=1):
+    codes = (torch.randn((rows, columns), generator=g) * 100).clamp(-448, 448).to(E4M3)
+    scales = torch.exp(torch.randn((-(-rows // group_rows), columns // 128), generator=g)) * 0.01
+    return codes, scales
+
+
+def check_product(tokens, rows, columns, dtype=torch.float32, bias=False, seed=0, **options):
+    g = generator(seed + tokens + rows + columns)
+    (x, xs), (w, ws) = random_codes(tokens, columns, g), random_codes(rows, columns, g, 128)
+    b = torch.randn(rows, generator=g).to(dtype) if bias else None
+    cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
+    y = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda(), bias=cuda(b), out_dtype=dtype, **options)
+    xd = (x.float().double().view(tokens, -1, 128) * xs.double()[..., None]).view(tokens, -1).cuda()
+    wd = (w.float().double().view(rows, -1, 128) * ws.double().repeat_interleave(128, 0)[:rows, :, None]).view(rows, -1).cuda()
+    want, size = xd @ wd.T.contiguous(), xd.abs() @ wd.abs().T.contiguous()
+    if bias:
+        want, size = want + b.double().cuda(), size + b.double().abs().cuda()
+    error = (y.double() - want).abs()
+    bound = U[dtype] * (1 + 2.0**-10) * want.abs() + (130 + 3 * (columns // 128)) * 2.0**-23 * size
+    if dtype == torch.float16:
+        bound = bound + 2.0**-25
+    assert y.dtype == dtype and y.shape == (tokens, rows) and bool(torch.isfinite(y).all())
+    assert bool((error <= bound).all()), float((error / bound).max())
+    return y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 100, 127, 128, 129, 200, 256, 257, 500])
+def test_products_by_tokens(tokens, dtype):
+    check_product(tokens, 300, 640, dtype, bias=tokens % 2 == 0)
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 16, 20, 64, 90, 300])
+@pytest.mark.parametrize("rows", [1, 3, 15, 16, 17, 64, 100, 127, 128, 129, 255, 257, 1000, 4099])
+def test_products_by_rows(tokens, rows):
+    check_product(tokens, rows, 256, torch.float16 if rows % 2 else torch.float32, bias=rows % 3 == 0)
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 37, 64, 150, 513])
+@pytest.mark.parametrize("columns", [128, 256, 384, 1408, 4096, 5120, 11008, 28672])
+def test_products_by_columns(tokens, columns):
+    check_product(tokens, 200, columns, torch.bfloat16 if columns % 256 else torch.float32, bias=True)
+
+
+@pytest.mark.parametrize("tokens,rows,columns", [(2048, 4096, 1024), (1000, 11008, 512), (16, 32000, 2048), (1, 131072, 256), (64, 50000, 512), (4096, 300, 2048), (700, 3000, 4096)])
+def test_large_products(tokens, rows, columns):
+    check_product(tokens, rows, columns, torch.float16)
+
+
+@pytest.mark.parametrize("tokens,rows,columns", [(1, 64, 512), (16, 200, 1024), (40, 130, 2048), (64, 1000, 512), (129, 515, 640), (600, 700, 1152), (2000, 4000, 384)])
+def test_products_of_whole_numbers_are_exact(tokens, rows, columns):
+    """Codes -8 ... 8 with scales that are powers of two: sums are whole numbers below 2^24 of one unit: to the bit, whatever the order"""
+    g = generator(tokens)
+    x, w = (torch.randint(-8, 9, (n, columns), generator=g).float() for n in (tokens, rows))
+    xs = 2.0 ** torch.randint(0, 2, (tokens, columns // 128), generator=g)
+    ws = 2.0 ** torch.randint(0, 2, (-(-rows // 128), columns // 128), generator=g)
+    y = onebit.block_linear(x.to(E4M3).cuda(), xs.cuda(), w.to(E4M3).cuda(), ws.cuda(), out_dtype=torch.float32)
+    xd = x.double() * xs.double().repeat_interleave(128, 1)
+    wd = w.double() * ws.double().repeat_interleave(128, 0)[:rows].repeat_interleave(128, 1)
+    assert torch.equal(y.double().cpu(), xd @ wd.T)
+
+
+def test_products_of_views_into_given_results():
+    g = generator(3)
+    (x, xs), (w, ws) = random_codes(24, 1024, g), random_codes(333, 1024, g, 128)
+    x, xs, w, ws = x.cuda(), xs.cuda(), w.cuda(), ws.cuda()
+    want = onebit.block_linear(x, xs, w, ws)
+    as_bytes = x.view(torch.uint8)
+    wide = torch.full((24, 1040), 0x7f, dtype=torch.uint8, device="cuda")
+    wide[:, 16:] = as_bytes
+    odd = torch.full((24, 1031), 0x7f, dtype=torch.uint8, device="cuda")
+    odd[:, 7:] = as_bytes
+    for view in (wide[:, 16:], odd[:, 7:], as_bytes.T.contiguous().T, as_bytes.view(4, 6, 1024)):
+        scales = xs.view(4, 6, 8) if view.dim() == 3 else xs.T.contiguous().T
+        got = onebit.block_linear(view.view(E4M3) if view.is_contiguous() else view.view(E4M3), scales, w, ws)
+        assert torch.equal(got.view(24, 333), want)
+    for shape, stride, offset in (((24, 333), (333, 1), 0), ((24, 333), (340, 1), 3), ((24, 333), (336, 1), 8), ((24, 333), (1, 24), 0)):
+        room = torch.full((24 * 400,), 9.0, dtype=torch.float16, device="cuda")
+        out = room.as_strided(shape, stride, offset)
+        if stride[1] != 1:
+            with pytest.raises(ValueError, match="whole rows"):
+                onebit.block_linear(x, xs, w, ws, out=out)
+            continue
+        assert onebit.block_linear(x, xs, w, ws, out=out) is not None and torch.equal(out, want)
+        out.fill_(9.0)
+        assert bool((room == 9).all())  # nothing beside
+    # weights whose rows lie apart, a part of a weight's rows
+    apart = torch.zeros((333, 1056), dtype=torch.uint8, device="cuda")
+    apart[:, 32:] = w.view(torch.uint8)
+    assert torch.equal(onebit.block_linear(x, xs, apart[:, 32:].view(E4M3), ws), want)
+    assert torch.equal(onebit.block_linear(x, xs, w[128:300], ws[1:3]), want[:, 128:300])
+    # none
+    assert onebit.block_linear(x[:0], xs[:0], w, ws).shape == (0, 333) and onebit.block_linear(x, xs, w[:0], ws[:0]).shape == (24, 0)
+    assert onebit.block_linear(x[0], xs[0], w, ws).shape == (333,) and torch.equal(onebit.block_linear(x[0], xs[0], w, ws), onebit.block_linear(x[:1], xs[:1], w, ws)[0])
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 30, 64, 65, 300])
+def test_what_is_not_finite_stays_in_its_token(tokens):
+    g = generator(8)
+    (x, xs), (w, ws) = random_codes(tokens, 512, g), random_codes(200, 512, g, 128)
+    clean = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
+    xs[tokens // 2, 1] = math.nan
+    x.view(torch.uint8)[tokens // 2, 128:256] = 0
+    got = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
+    others = [t for t in range(tokens) if t != tokens // 2]
+    assert bool(torch.isnan(got[tokens // 2]).all()) and torch.equal(got[others], clean[others])
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16, 17, 64, 200])
+def test_a_token_of_a_batch_is_that_token_alone_on_codes(tokens):
+    """Up to the order of fp32 sums"""
+    g = generator(tokens)
+    (x, xs), (w, ws) = random_codes(tokens, 1024, g), random_codes(500, 1024, g, 128)
+    x, xs, w, ws = x.cuda(), xs.cuda(), w.cuda(), ws.cuda()
+    together = onebit.block_linear(x, xs, w, ws, out_dtype=torch.float32)
+    alone = torch.cat([onebit.block_linear(x[t:t + 1], xs[t:t + 1], w, ws, out_dtype=torch.float32) for t in range(0, tokens, 7)])
+    assert float((together[::7] - alone).norm() / alone.norm()) < 1e-5
+
+
+def test_layers():
+    g = generator(6)
+    weight, bias = torch.randn((520, 700), generator=g), torch.randn(520, generator=g)
+    layer = onebit.BlockLinear(weight.cuda(), bias=bias.cuda())
+    x = torch.randn((3, 11, 700), generator=g).half().cuda()
+    y = layer(x)
+    codes, scales = onebit.quantize_rows(x)
+    assert y.dtype == torch.float16 and y.shape == (3, 11, 520) and torch.equal(y, layer((codes, scales)))
+    assert torch.equal(y, onebit.block_linear(codes, scales, layer.codes, layer.scales, bias=layer.bias))
+    # codes of x and of the weight are off by half a step each, 2^-4: of all values at most that, and both of them
+    size = x.double().abs() @ weight.double().abs().T.cuda()
+    assert bool(((y.double() - (x.double() @ weight.double().T.cuda() + bias.double().cuda())).abs() <= 0.14 * size + 0.01).all())
+    assert onebit.BlockLinear(weight.cuda(), out_dtype=torch.float32)(x).dtype == torch.float32 and layer(x.float()).dtype == torch.float32
+
+
+# ---- tokens
+
+
+def plain_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """From the definition, row by row in 64 bits"""
+    logits, uniform, out = logits.double().cpu(), uniform.double().cpu(), []
+    for r in range(logits.shape[0]):
+        t, k, p, m = (float(v[r]) if isinstance(v, torch.Tensor) else float(torch.tensor(float(v))) for v in (temperature, top_k, top_p, min_p))
+        row = logits[r]
+        if bool(row.isnan().any()) or float(row.max()) == -math.inf:
+            out.append(-1)
+            continue
+        order = torch.sort(row, descending=True, stable=True).indices
+        if not t > 0:
+            out.append(int(order[0]))
+            continue
+        top = row[order[0]]
+        w = torch.where(row == top, 1.0, torch.exp((row - top) / t))[order]
+        if k > 0:
+            w = w[:int(k)]
+        if p < 1:
+            in_front = torch.cat([w.new_zeros(1), w.cumsum(0)[:-1]])
+            w = w[:max(1, int((in_front < p * w.sum()).sum()))]
+        w = w[:max(1, int((w >= m).sum()))]
+        kept, place = order[:len(w)].sort()
+        w = w[place]
+        running = w.cumsum(0)
+        u = float(uniform[r]) if float(uniform[r]) > 0 else 0.0
+        at = int((running <= u * running[-1]).sum())
+        out.append(int(kept[min(at, int((w > 2.0**-43).nonzero()[-1]))]))  # (weights below half of 2^-42 are 0)
+    return out
+
+
+def check_tokens(logits, uniform, **options):
+    cuda = lambda v: v.cuda() if isinstance(v, torch.Tensor) else v  # noqa: E731
+    got = onebit.sample(logits.cuda(), uniform.cuda(), **{k: cuda(v) for k, v in options.items()})
+    assert got.dtype == torch.int64 and got.shape == logits.shape[:-1]
+    want = plain_tokens(logits, uniform, **options)
+    assert got.tolist() == want, [(r, a, b) for r, (a, b) in enumerate(zip(got.tolist(), want)) if a != b][:5]
+    return got
+
+
+def random_logits(rows, vocabulary, g, dtype, spread=3.0):
+    return (torch.randn((rows, vocabulary), generator=g) * spread).to(dtype)
+
+
+FILTERS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=5), dict(top_k=50, temperature=1.3), dict(top_p=0.9), dict(top_p=0.3, temperature=0.5), dict(min_p=0.05),
+           dict(top_k=40, top_p=0.95, min_p=0.02, temperature=0.8), dict(temperature=0.0), dict(top_k=10**6), dict(top_p=0.0), dict(min_p=1.0), dict(min_p=2.0),
+           dict(top_p=0.999, temperature=2.0), dict(top_k=1000, top_p=0.99), dict(temperature=100.0), dict(temperature=1e-6, top_p=0.9)]
+
+
+@pytest.mark.parametrize("options", FILTERS, ids=str)
+@pytest.mark.parametrize("vocabulary", [1, 2, 63, 64, 65, 1000, 4096, 32000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens(options, vocabulary, dtype):
+    g = generator(vocabulary)
+    check_tokens(random_logits(7, vocabulary, g, dtype), torch.rand(7, generator=g), **options)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary", [(1, 131072), (40, 50257), (300, 1500), (3, 131071), (2, 1 << 20)])
+def test_tokens_with_parameters_of_their_own(rows, vocabulary, dtype):
+    g = generator(rows)
+    logits = random_logits(rows, vocabulary, g, dtype)
+    share = lambda: torch.rand(rows, generator=g)  # noqa: E731
+    pick = lambda *values: torch.tensor(values)[torch.randint(0, len(values), (rows,), generator=g)]  # noqa: E731
+    for _ in range(2):
+        check_tokens(logits, share(), temperature=pick(0.0, 0.5, 1.0, 3.0), top_k=pick(0, 1, 30, 2000, 1 << 30).int(), top_p=pick(0.2, 0.9, 0.999, 1.0), min_p=pick(0.0, 0.01, 0.3))
+        check_tokens(logits, share(), temperature=share() + 0.5, top_p=share())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_equal_logits_go_by_index(dtype):
+    """All equal, and few values: borders that fall on whole masses, ties that a filter takes in part"""
+    g = generator(1)
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.999999])
+    for value in (0.0, -0.0, 5.0, -60000.0):
+        flat = torch.full((5, 1000), value).to(dtype)
+        for options in (dict(), dict(top_k=7), dict(top_p=0.5), dict(top_k=64, top_p=0.25), dict(min_p=1.0), dict(temperature=0.0), dict(top_k=999)):
+            check_tokens(flat, u, **options)
+    signs = torch.where(torch.rand((5, 3000), generator=g) < 0.5, 0.0, -0.0).to(dtype)
+    check_tokens(signs, u, top_k=1500)
+    check_tokens(signs, u, temperature=0.0)
+    few = torch.randint(0, 4, (5, 20000), generator=g).to(dtype)
+    for options in (dict(), dict(top_k=100), dict(top_k=4990), dict(top_k=7000), dict(top_p=0.31), dict(top_k=9000, top_p=0.8), dict(min_p=0.2, top_p=0.9), dict(top_p=0.7, temperature=0.25)):
+        check_tokens(few, u, **options)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_hidden_tokens(dtype):
+    g = generator(2)
+    logits = random_logits(9, 5000, g, dtype)
+    logits[0, :] = -math.inf
+    logits[1, :] = -math.inf
+    logits[1, 4321] = -3.0
+    logits[2, torch.rand(5000, generator=g) < 0.99] = -math.inf
+    logits[3, 17] = math.nan
+    logits[4, 4999] = -math.nan
+    logits[5, [3, 400, 4000]] = math.inf
+    logits[6, 0] = math.inf
+    logits[7, :] = math.nan
+    logits[8, 1:] = -math.inf
+    least = torch.finfo(dtype).min
+    for options in FILTERS:
+        for u in (0.0, 0.4, 0.999):
+            check_tokens(logits, torch.full((9,), u), **options)
+    logits = torch.where(torch.rand((9, 5000), generator=g) < 0.9, least, random_logits(9, 5000, g, torch.float32)).to(dtype)  # a mask of the type's lowest value
+    logits[0, :] = least
+    for options in FILTERS:
+        check_tokens(logits, torch.rand(9, generator=g), **options)
+
+
+def test_random_numbers_at_and_beyond_their_ends():
+    logits = random_logits(6, 700, generator(3), torch.float32)
+    logits[:, -1] = -math.inf
+    logits[:, -2] = -200.0  # a weight that rounds to 0
+    u = torch.tensor([0.0, 1.0, 1.5, -1.0, math.inf, 1 - 2.0**-24])
+    first, second = check_tokens(logits, u), check_tokens(logits, u, top_k=10)
+    nan = onebit.sample(logits.cuda(), torch.full((6,), math.nan, device="cuda"))
+    assert torch.equal(nan, onebit.sample(logits.cuda(), torch.zeros(6, device="cuda"))) and first.shape == second.shape
+
+
+@pytest.mark.parametrize("place", ["front", "end", "sorted", "falling"])
+def test_the_largest_logits_side_by_side(place):
+    """What a filter keeps lies in one stretch of the row"""
+    g = generator(4)
+    logits = random_logits(4, 40000, g, torch.float32, 1.0)
+    if place in ("sorted", "falling"):
+        logits = logits.sort(-1, descending=place == "falling").values
+    else:
+        logits[:, slice(0, 3000) if place == "front" else slice(-3000, None)] += 12.0
+    for options in (dict(top_k=50), dict(top_k=2500), dict(top_p=0.9), dict(min_p=0.01), dict(top_k=3500, top_p=0.999)):
+        check_tokens(logits, torch.rand(4, generator=g), **options)
+
+
+def test_logits_that_are_strided_shaped_or_none():
+    g = generator(5)
+    logits, u = random_logits(12, 1001, g, torch.float16).view(3, 4, 1001).cuda(), torch.rand((3, 4), generator=g).cuda()
+    want = onebit.sample(logits, u, top_k=20)
+    assert want.shape == (3, 4)
+    room = torch.full((12, 1100), math.nan, dtype=torch.float16, device="cuda")
+    for first in (0, 1, 3, 8):
+        room[:, first:first + 1001] = logits.view(12, 1001)
+        assert torch.equal(onebit.sample(room[:, first:first + 1001], u.view(12), top_k=20), want.view(12))
+        room.fill_(math.nan)
+    assert torch.equal(onebit.sample(logits.transpose(0, 1), u.T.contiguous(), top_k=20), want.T)
+    assert torch.equal(onebit.sample(logits.flip(-1).flip(-1), u, top_k=20), want)
+    spread = torch.empty((3, 4, 2002), dtype=torch.float16, device="cuda")
+    spread[..., ::2] = logits
+    assert torch.equal(onebit.sample(spread[..., ::2], u, top_k=20), want) and torch.equal(onebit.sample(torch._neg_view(-logits), u, top_k=20), want)
+    one = onebit.sample(logits[0, 0], u[0, 0], top_k=20)
+    assert one.shape == () and int(one) == int(want[0, 0])
+    assert torch.equal(onebit.sample(logits[:1, :1].expand(3, 4, 1001), u, top_k=20), torch.stack([onebit.sample(logits[0, 0], v, top_k=20) for v in u.view(-1)]).view(3, 4))
+    assert onebit.sample(logits[:0], u[:0]).shape == (0, 4)
+
+
+def test_shares_of_many_draws():
+    """65536 evenly spaced numbers: a token has its share of them, to one of them at each end"""
+    logits = random_logits(1, 50, generator(6), torch.float32, 1.5)
+    u = (torch.arange(65536) + 0.5) / 65536
+    tokens = onebit.sample(logits.expand(65536, 50).cuda(), u.cuda(), temperature=0.9)
+    share = torch.bincount(tokens.cpu(), minlength=50).double() / 65536
+    assert float((share - torch.softmax(logits[0].double() / float(torch.tensor(0.9)), 0)).abs().max()) <= 2 / 65536
+
+
+# ---- together
+
+
+def head_step(x, residual, weight, layer, u, **options):
+    h, codes, scales = onebit.block_norm_codes(x, residual, weight)
+    logits = layer((codes, scales))
+    return h, codes, scales, logits, onebit.sample(logits, u, **options)
+
+
+@pytest.mark.parametrize("count", [1, 5, 16, 70])
+def test_a_graph_of_the_last_steps_replays(count):
+    """Captured once, replayed with a program's eager work and synchronizations in between; each replay is the eager result"""
+    g = generator(count)
+    layer = onebit.BlockLinear(torch.randn((3000, 512), generator=g).cuda())
+    weight = torch.ones(512, dtype=torch.float16, device="cuda")
+    x, residual = (torch.zeros((count, 512), dtype=torch.float16, device="cuda") for _ in range(2))
+    u = torch.zeros(count, device="cuda")
+    options = dict(temperature=torch.full((count,), 0.8, device="cuda"), top_k=40, top_p=0.95, min_p=0.01)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        head_step(x, residual, weight, layer, u, **options)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            outputs = head_step(x, residual, weight, layer, u, **options)
+    torch.cuda.synchronize()
+    for _ in range(12):
+        x.copy_(torch.randn(x.shape, generator=g).half())
+        residual.copy_(torch.randn(x.shape, generator=g).half())
+        u.copy_(torch.rand(count, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for mine, theirs in zip(outputs, head_step(x, residual, weight, layer, u, **options)):
+            assert same(mine, theirs)
+        torch.zeros(1000, device="cuda").sum().item()
+
+
+def test_two_streams_at_once():
+    g = generator(9)
+    layer = onebit.BlockLinear(torch.randn((2000, 1024), generator=g).cuda())
+    weight = torch.ones(1024, dtype=torch.float16, device="cuda")
+    inputs = [(torch.randn((n, 1024), generator=g).half().cuda(), torch.randn((n, 1024), generator=g).half().cuda(), torch.rand(n, generator=g).cuda()) for n in (1, 16, 40, 300)]
+    want = [head_step(x, r, weight, layer, u, top_p=0.9) for x, r, u in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[] for _ in inputs]
+    for _ in range(5):
+        for i, (x, r, u) in enumerate(inputs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(head_step(x, r, weight, layer, u, top_p=0.9))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        for result in results:
+            assert all(same(a, b) for a, b in zip(result, want[i]))
