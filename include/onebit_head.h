@@ -41,11 +41,12 @@ int onebit_quantize_rows(const void *x, int dtype, long long x_stride, int rows,
 int onebit_block_norm_codes(const onebit_norm *norm, const onebit_codes *out, void *stream);
 
 /*
- * y[t][m] = sum over groups g of x.scales[t][g] * weight.scales[m / 128][g] * (sum over the group's columns k of x[t][k] * weight[m][k])
- * + bias[m]: tokens x rows values, fp32, fp16 or bf16 (y_dtype), y_stride between tokens. Products of codes are exact, their sums over a group and
- * everything behind them fp32, y is rounded once. weight: `rows` rows of codes, scales for each 128 rows and columns (ceil(rows / 128) rows of
- * them). columns: a multiple of 128. bias: `rows` values (bias_dtype), or NULL. workspace: onebit_block_linear_workspace() bytes,
- * 16-byte aligned (NULL where that is 0). Codes are not NaN but in rows whose results may be.
+ * y[t][m] = sum over groups g of (x.scales[t][g] * weight.scales[m / 128][g]) * (sum over the group's columns k of x[t][k] * weight[m][k])
+ * + bias[m]: tokens x rows values, fp32, fp16 or bf16 (y_dtype), y_stride between tokens. Products of codes are exact, their sums and everything behind
+ * them fp32, y is rounded once; but for fp16 and bf16 results of more than 16 tokens the products of eight neighbouring columns are cut off
+ * at 2^-13 of the largest of them, as the 8-bit matrix instruction does (1.5e-5 of y over normal values). weight: `rows` rows of codes, scales for each 128 rows and
+ * columns (ceil(rows / 128) rows of them). columns: a multiple of 128. bias: `rows` values (bias_dtype), or NULL. workspace:
+ * onebit_block_linear_workspace() bytes, 16-byte aligned (NULL where that is 0). A NaN among a token's codes or scales reaches that token's results alone.
  */
 typedef struct onebit_block_product {
   onebit_codes x, weight;

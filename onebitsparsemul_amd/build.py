@@ -43,7 +43,7 @@ def build_library():
     for src in ("onebit_gemm.hip", "onebit_gemm_tokens.hip", "onebit_skinny.hip", "onebit_skinny_tokens.hip",
                 "onebit_wide.hip", "onebit_wide_tokens.hip", "onebit_format.hip", "onebit_capi.hip", "onebit_diag.hip",
                 "onebit_cache.hip", "onebit_attention.hip", "onebit_attention_tiles.hip", "onebit_norm.hip", "onebit_decoder_capi.hip",
-                "onebit_codes.hip", "onebit_block.hip", "onebit_sample.hip", "onebit_head_capi.hip"):
+                "onebit_codes.hip", "onebit_block.hip", "onebit_block_tiles.hip", "onebit_sample.hip", "onebit_head_capi.hip"):
         obj = os.path.join(CSRC, src.replace(".hip", ".o"))
         cmds.append([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
         objs.append(obj)

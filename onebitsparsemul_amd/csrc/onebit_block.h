@@ -1,0 +1,87 @@
+// What the products of 8-bit codes share (internal to libonebitmul): operands of the matrix instructions, results.
+#pragma once
+#include "onebit_codes.h"
+#include "onebit_head_launch.h"
+
+namespace onebit {
+
+__device__ inline float value_at(const void* base, int type, long long at) {
+  if (type == ONEBIT_DTYPE_F32) return ((const float*)base)[at];
+  return type == ONEBIT_DTYPE_F16 ? (float)((const _Float16*)base)[at] : (float)((const __bf16*)base)[at];
+}
+
+typedef int i8_t __attribute__((ext_vector_type(8)));
+
+// A lane's 32 codes of a group, and the products of 16 x 128 with 128 x 16 of them
+template <bool NARROW>
+struct Operand {
+  h8_t v[4];
+  Operand() = default;
+  __device__ Operand(const u4_t& a, const u4_t& b)
+      : v{codes_to_f16<ONEBIT_CODE_E4M3>(a.x, a.y), codes_to_f16<ONEBIT_CODE_E4M3>(a.z, a.w), codes_to_f16<ONEBIT_CODE_E4M3>(b.x, b.y), codes_to_f16<ONEBIT_CODE_E4M3>(b.z, b.w)} {}
+  __device__ f4_t operator*(const Operand& other) const {
+    f4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], other.v[k], sum, 0, 0, 0);
+    return sum;
+  }
+};
+template <>
+struct Operand<true> {
+  i8_t v;
+  Operand() = default;
+  __device__ Operand(const u4_t& a, const u4_t& b) : v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w} {}
+  __device__ f4_t operator*(const Operand& other) const {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, other.v, f4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+  }
+};
+
+// Where sums go: to the split's partial sums or, with the bias, to y
+struct Result {
+  void* base;
+  long long stride;
+  int type, rows;
+  bool vectors;  // eight neighbours at a multiple of eight are whole 16-byte units
+  const void* bias;
+  int bias_type;
+  __device__ Result(const onebit_block_product& p, const BlockGrid& grid, int split)
+      : base(grid.splits > 1 ? (void*)(grid.partial + (long long)split * p.tokens * p.rows) : p.y),
+        stride(grid.splits > 1 ? p.rows : p.y_stride),
+        type(grid.splits > 1 ? ONEBIT_DTYPE_F32 : p.y_dtype),
+        rows(p.rows),
+        vectors(stride % 8 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0),
+        bias(grid.splits > 1 ? nullptr : p.bias),
+        bias_type(p.bias_dtype) {}
+  __device__ void load_bias(int row, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bias && row + i < rows ? value_at(bias, bias_type, row + i) : 0.f;
+  }
+  // one sum, without the bias
+  __device__ void put_one(int token, int row, float v) const {
+    if (row >= rows) return;
+    const float one[1] = {bias ? v + value_at(bias, bias_type, row) : v};
+    if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, 1>(base, token * stride + row, one);
+    else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 1>(base, token * stride + row, one);
+    else store_values<ONEBIT_DTYPE_BF16, 1>(base, token * stride + row, one);
+  }
+  // eight sums of a token from weight row `row` on, a multiple of eight, with the bias
+  __device__ void put(int token, int row, const float (&v)[8]) const {
+    const long long at = token * stride + row;
+    if (vectors && row + 8 <= rows) {
+      if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, 8>(base, at, v);
+      else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 8>(base, at, v);
+      else store_values<ONEBIT_DTYPE_BF16, 8>(base, at, v);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (row + i >= rows) break;
+      const float one[1] = {v[i]};
+      if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, 1>(base, at + i, one);
+      else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 1>(base, at + i, one);
+      else store_values<ONEBIT_DTYPE_BF16, 1>(base, at + i, one);
+    }
+  }
+};
+
+}  // namespace onebit

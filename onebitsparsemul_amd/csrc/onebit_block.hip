@@ -1,75 +1,187 @@
-// The matrix product of 8-bit codes with a scale for each 128 (onebit_head.h).
+// The product of 8-bit codes with a scale for each 128 (onebit_head.h): few tokens, and which kernel takes a call.
 //
 // Codes go into the matrix instructions as fp16, exactly, whose products are exact and whose sums are fp32 (v_mfma_f32_16x16x32_f16: 9e-9 off over a group of 128
-// normal values; those of the 8-bit instructions drop what lies 2^-14 below the largest product of a few neighbours, 1.5e-5). The sum of a group, from 0 on, times the
+// normal values; those of the 8-bit instructions cut the products of eight neighbours off at 2^-13 of the largest, 1.5e-5: they serve 16-bit results of many tokens). The sum of a group, from 0 on, times the
 // product of the two scales is added to the sums in fp32. The weight is the matrix operand A, the tokens are B's columns: a lane then holds four neighbouring rows of y of
 // one token, so that its scale is one register, the weight's is the same for all lanes, and y is written in vectors.
-#include "onebit_codes.h"
-#include "onebit_head_launch.h"
+#include "onebit_block.h"
+
+#include <algorithm>
 
 namespace onebit {
 namespace {
 
-// A lane's 32 codes of a group as fp16
-struct Values {
-  h8_t v[4];
-};
-__device__ inline Values load32(const uint8_t* p) {
-  const u4_t low = ((const u4_t*)p)[0], high = ((const u4_t*)p)[1];
-  return {codes_to_f16<ONEBIT_CODE_E4M3>(low.x, low.y), codes_to_f16<ONEBIT_CODE_E4M3>(low.z, low.w), codes_to_f16<ONEBIT_CODE_E4M3>(high.x, high.y),
-          codes_to_f16<ONEBIT_CODE_E4M3>(high.z, high.w)};
-}
-
-__device__ inline f4_t multiply(const Values& a, const Values& b) {
-  f4_t sum = {0.f, 0.f, 0.f, 0.f};
+// Few tokens: the weight goes by once. A workgroup has R * 16 of its rows and 16 tokens, its wavefronts a part of the groups each; operands come straight from memory,
+// a row's 128 codes as two halves that four lanes read side by side, and the wavefronts' sums meet in LDS. UNROLL groups are asked for at once.
+template <int R, int WAVES, int UNROLL>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(onebit_block_product p, BlockGrid grid) {
+  typedef Operand<false> Values;
+  constexpr int kRows = R * 16, kPitch = kRows + 1;
+  __shared__ float sums[WAVES][16][kPitch];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane % 16, q = lane / 16;
+  const int tile = blockIdx.x / grid.tiles_n, first_row = tile * kRows, first_token = (blockIdx.x - tile * grid.tiles_n) * 16, split = blockIdx.y;
+  const int low = split * grid.groups_per_split, high = min(low + grid.groups_per_split, p.columns / ONEBIT_CODE_GROUP);
+  const int each = (high - low + WAVES - 1) / WAVES, begin = min(low + wave * each, high), end = min(begin + each, high);
+  const uint8_t* w[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[i], b.v[i], sum, 0, 0, 0);
-  return sum;
-}
-
-__device__ inline float value_at(const void* base, int type, long long at) {
-  if (type == ONEBIT_DTYPE_F32) return ((const float*)base)[at];
-  return type == ONEBIT_DTYPE_F16 ? (float)((const _Float16*)base)[at] : (float)((const __bf16*)base)[at];
-}
-
-// A wavefront: 16 rows of the weight, 16 tokens, operands straight from memory.
-template <int TYPE>
-__global__ __launch_bounds__(256) void product_kernel(onebit_block_product p) {
-  const int lane = threadIdx.x % 64, n = lane % 16, quarter = lane / 16;
-  const int first_row = (blockIdx.x * 4 + threadIdx.x / 64) * 16, first_token = blockIdx.y * 16;
-  if (first_row >= p.rows) return;
-  const int token = min(first_token + n, p.tokens - 1), row = min(first_row + n, p.rows - 1), groups = p.columns / ONEBIT_CODE_GROUP;
-  const uint8_t* w = (const uint8_t*)p.weight.codes + row * p.weight.row_stride + quarter * 32;
-  const uint8_t* x = (const uint8_t*)p.x.codes + token * p.x.row_stride + quarter * 32;
-  const float* w_scale = p.weight.scales + first_row / ONEBIT_CODE_GROUP * p.weight.scale_stride;
-  const float* x_scale = p.x.scales + token * p.x.scale_stride;
-  f4_t sum = {0.f, 0.f, 0.f, 0.f};
-  for (int g = 0; g < groups; ++g) {
-    const f4_t part = multiply(load32(w + g * ONEBIT_CODE_GROUP), load32(x + g * ONEBIT_CODE_GROUP));
-    const float scale = w_scale[g] * x_scale[g];
+  for (int i = 0; i < R; ++i) w[i] = (const uint8_t*)p.weight.codes + min(first_row + i * 16 + r, p.rows - 1) * p.weight.row_stride + q * 16;
+  const int token = min(first_token + r, p.tokens - 1);
+  const uint8_t* const x = (const uint8_t*)p.x.codes + token * p.x.row_stride + q * 16;
+  const float* const x_scale = p.x.scales + token * p.x.scale_stride;
+  const float* const w_scale = p.weight.scales + first_row / ONEBIT_CODE_GROUP * p.weight.scale_stride;
+  f4_t sum[R] = {};
+  auto groups = [&](int g, auto count) {
+    constexpr int kCount = decltype(count)::value;
+    u4_t a[kCount][R][2], b[kCount][2];
+    float scale[kCount];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += scale * part[i];
+    for (int u = 0; u < kCount; ++u)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[u][i][h] = *(const u4_t*)(w[i] + (long long)(g + u) * ONEBIT_CODE_GROUP + h * 64);
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) b[u][h] = *(const u4_t*)(x + (long long)(g + u) * ONEBIT_CODE_GROUP + h * 64);
+      scale[u] = x_scale[g + u];
+    }
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+      const Values bv(b[u][0], b[u][1]);
+      const float s = scale[u] * w_scale[g + u];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const f4_t part = Values(a[u][i][0], a[u][i][1]) * bv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(part[e], s, sum[i][e]);
+      }
+    }
+  };
+  int g = begin;
+  for (; g + UNROLL <= end; g += UNROLL) groups(g, std::integral_constant<int, UNROLL>());
+  for (; g < end; ++g) groups(g, std::integral_constant<int, 1>());
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[wave][r][i * 16 + q * 4 + e] = sum[i][e];
+  __syncthreads();
+  const Result result(p, grid, split);
+  const int tokens = min(16, p.tokens - first_token);
+  for (int at = threadIdx.x; at < tokens * kRows; at += 64 * WAVES) {
+    const int t = at / kRows, row = at % kRows;
+    float total = 0.f;
+#pragma unroll
+    for (int s = 0; s < WAVES; ++s) total += sums[s][t][row];
+    result.put_one(first_token + t, first_row + row, total);
   }
-  if (first_token + n >= p.tokens) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = first_row + quarter * 4 + i;
-    if (at >= p.rows) return;
-    const float y[1] = {p.bias ? sum[i] + value_at(p.bias, p.bias_dtype, at) : sum[i]};
-    store_values<TYPE, 1>(p.y, token * p.y_stride + at, y);
-  }
 }
 
-template <int TYPE>
-hipError_t launch_as(const onebit_block_product& p, hipStream_t stream) {
-  return launch_kernel(product_kernel<TYPE>, dim3((p.rows + 63) / 64, (p.tokens + 15) / 16), dim3(256), 0, stream, p);
+// Sums of the splits, in their order, with the bias. One thread: eight rows of a token.
+__global__ __launch_bounds__(256) void add_splits_kernel(onebit_block_product p, BlockGrid grid) {
+  const int units = (p.rows + 7) / 8;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (long long)p.tokens * units) return;
+  const int token = (int)(at / units), row = (int)(at % units) * 8;
+  const long long apart = (long long)p.tokens * p.rows;
+  const float* from = grid.partial + (long long)token * p.rows + row;
+  const BlockGrid whole = {0, 0, 1, 0, 0, nullptr};
+  const Result result(p, whole, 0);
+  float sum[8];
+  result.load_bias(row, sum);
+  if (p.rows % 4 == 0 && row + 8 <= p.rows) {
+    f4_t low = {}, high = {};
+#pragma unroll 4
+    for (int s = 0; s < grid.splits; ++s, from += apart) low += ((const f4_t*)from)[0], high += ((const f4_t*)from)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += low[i], sum[i + 4] += high[i];
+  } else {
+    float total[8] = {};
+    for (int s = 0; s < grid.splits; ++s, from += apart)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (row + i < p.rows) total[i] += from[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += total[i];
+  }
+  result.put(token, row, sum);
+}
+
+template <int R, int WAVES, int UNROLL>
+hipError_t launch_few_as(const onebit_block_product& p, BlockGrid grid, hipStream_t stream) {
+  grid.tiles_n = (p.tokens + 15) / 16;
+  const long long tiles = (p.rows + R * 16 - 1) / (R * 16) * (long long)grid.tiles_n;
+  if (tiles * 64 * WAVES >= 1ll << 32) return hipErrorInvalidConfiguration;
+  return launch_kernel(few_kernel<R, WAVES, UNROLL>, dim3((unsigned)tiles, grid.splits), dim3(64 * WAVES), 0, stream, p, grid);
 }
 
 }  // namespace
 
-hipError_t launch_block_linear(const onebit_block_product& p, hipStream_t stream) {
-  if (p.y_dtype == ONEBIT_DTYPE_F32) return launch_as<ONEBIT_DTYPE_F32>(p, stream);
-  return p.y_dtype == ONEBIT_DTYPE_F16 ? launch_as<ONEBIT_DTYPE_F16>(p, stream) : launch_as<ONEBIT_DTYPE_BF16>(p, stream);
+BlockGrid plan_block(const onebit_block_product& p, int compute_units) {
+  const int groups = p.columns / ONEBIT_CODE_GROUP;
+  BlockGrid grid = {0, kBlock16, 1, groups, compute_units / 32 < 1 ? 1 : std::min(compute_units / 32, 8), nullptr};
+  auto split = [&](int splits) {
+    grid.groups_per_split = (groups + splits - 1) / splits;
+    grid.splits = (groups + grid.groups_per_split - 1) / grid.groups_per_split;
+  };
+  // (a tile's copies know a row's distance in 32 bits)
+  auto near = [](const onebit_codes& c) { return c.row_stride >= 0 && c.row_stride < 1 << 23; };
+  if (p.tokens <= 16 || groups < kLeastTileGroups || !near(p.x) || !near(p.weight)) {
+    // 64 rows to a workgroup, where there are enough of them: the tokens' codes are read for four times as many of the weight. 16 tokens on 131072 x 4096: 109 us (4.9 TB/s),
+    // with 32 rows 136, with 16 rows 163; 11008 x 4096 13.0, 14.6, 14.6 (one token 10.7, 11.5, 10.0); 4096 x 4096 12.7, 8.9, 6.7 (eight wavefronts), 4096 x 512 3.6, 3.9, 2.7.
+    const int rows = (p.rows + 15) / 16, tokens = (p.tokens + 15) / 16;
+    if ((long long)(rows + 3) / 4 * tokens >= compute_units / 2) {
+      grid.kernel = kBlock64;
+    } else {
+      grid.kernel = groups >= 16 ? kBlock16Wide : kBlock16;
+      // (300 x 28672 with 16 tokens 29.5 us, in two splits 16.2; 4096 x 4096 6.7, in two 6.9)
+      if ((long long)rows * tokens * 2 <= compute_units && groups >= 32) split((int)std::min<long long>(groups / 16, compute_units / ((long long)rows * tokens)));
+    }
+    return grid;
+  }
+  // A group's time in a tile where workgroups are few and where every compute unit has one, and what a tile costs beside them, as measured: 128 tokens on 11008 x 4096,
+  // 4096 on 8192 x 8192, 64 on 32000 x 4096.
+  struct Kind {
+    int kernel, rows, tokens, on_unit;
+    double alone, crowded, start;
+  };
+  static const Kind kinds[] = {{kBlock128x32, 128, 32, 1, 0.40, 0.80, 3.0}, {kBlock64x64, 64, 64, 2, 0.35, 0.55, 3.0}, {kBlock128x64, 128, 64, 1, 0.42, 0.62, 3.5},
+                               {kBlock256x128, 256, 128, 1, 0.80, 1.08, 6.0}, {kBlock256x256, 256, 256, 1, 1.28, 1.65, 8.0}};
+  double least = 1e30;
+  for (const Kind& kind : kinds) {
+    if (kind.kernel == kBlock128x32 && p.tokens > 32) continue;
+    const long long tiles = (long long)((p.rows + kind.rows - 1) / kind.rows) * ((p.tokens + kind.tokens - 1) / kind.tokens), places = (long long)compute_units * kind.on_unit;
+    for (int splits = 1; splits <= 16 && groups / splits >= kLeastTileGroups; ++splits) {
+      const long long blocks = tiles * splits;
+      if (splits > 1 && blocks > places) break;
+      const double filled = std::min(1.0, (double)blocks / places), step = kind.alone + (kind.crowded - kind.alone) * filled;
+      const double rounds = (double)((blocks + places - 1) / places);
+      double time = rounds * (((groups + splits - 1) / splits) * step + kind.start);
+      if (splits > 1) time += 3.0 + 8e-6 * splits * p.tokens * p.rows / 3.0;  // sums out and in again, at 3 TB/s
+      if (time < least) {
+        least = time;
+        grid.kernel = kind.kernel;
+        split(splits);
+      }
+    }
+  }
+  return grid;
+}
+
+size_t block_workspace(const onebit_block_product& p, const BlockGrid& grid) { return grid.splits > 1 ? (size_t)grid.splits * p.tokens * p.rows * sizeof(float) : 0; }
+
+hipError_t launch_block_linear(const onebit_block_product& p, const BlockGrid& grid, hipStream_t stream) {
+  hipError_t status;
+  switch (grid.kernel) {
+    case kBlock16: status = launch_few_as<1, 4, 2>(p, grid, stream); break;
+    case kBlock16Wide: status = launch_few_as<1, 8, 2>(p, grid, stream); break;
+    case kBlock64: status = launch_few_as<4, 4, 1>(p, grid, stream); break;
+    default: status = launch_block_tiles(p, grid, stream);
+  }
+  if (status != hipSuccess || grid.splits == 1) return status;
+  const long long blocks = ((long long)p.tokens * ((p.rows + 7) / 8) + 255) / 256;
+  if (blocks >= 1ll << 24) return hipErrorInvalidConfiguration;
+  return launch_kernel(add_splits_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, grid);
 }
 
 }  // namespace onebit

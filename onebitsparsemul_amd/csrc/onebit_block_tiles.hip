@@ -1,0 +1,242 @@
+// The product of 8-bit codes for many tokens: tiles of both operands in LDS.
+#include "onebit_block.h"
+#include "onebit_device.h"
+
+#include <atomic>
+
+namespace onebit {
+namespace {
+
+// Wave tiles of FM x FN products of 16 x 16, WM x WN of them to a workgroup; a ring of STAGES groups in LDS. NARROW: the 8-bit matrix instruction.
+template <int WM, int WN, int FM, int FN, int STAGES>
+struct Tile {
+  static constexpr int kWaves = WM * WN, kRows = WM * FM * 16, kTokens = WN * FN * 16;
+  // Scales of a wavefront's own tokens, of four groups at a time, of eight in all
+  static constexpr int kStage = (kRows + kTokens) * ONEBIT_CODE_GROUP, kScales = 2 * 64 * 16, kLds = STAGES * kStage + kWaves * kScales;
+  static constexpr int kCopies = (kRows + kTokens) / 8 / kWaves;  // of 8 rows of 128 codes, to a wavefront
+  // A group in a wavefront's products of FM rows: in front of row kRelease all of it is in registers, and copies may begin to take its place, one to each kApart
+  // products from there on; in front of row kLanding the next group is there.
+  static constexpr int kRelease = FM / 2, kLanding = FM > 4 ? FM - 2 : kRelease, kSlots = FM > 4 ? 5 : 4;
+  static constexpr int kApart = FM * FN >= 2 * kCopies ? 2 : 1, kAtOnce = (kCopies + FM * FN - 1) / (FM * FN);
+  static constexpr int copies_before(int row) {  // of those from row kRelease on
+    const int copies = ((row - kRelease) * FN + kApart - 1) / kApart * kAtOnce;
+    return copies < kCopies ? copies : kCopies;
+  }
+  static constexpr int kEarly = copies_before(FM);  // the others in the next group's rows, in front of row kRelease
+  static_assert((kRows + kTokens) / 8 % kWaves == 0 && kRows / 8 % kWaves == 0 && FM * 16 <= 128 && kLds <= 160 * 1024 && FM >= 2 && FN <= 4, "");
+};
+
+// Rows of 128 codes in LDS, their pieces of 16 at their number exclusive-or half of the row's: the sixteen lanes that LDS serves at a time read a piece of sixteen
+// neighbouring rows from different banks. A lane takes pieces q and q + 4 of both operands' rows: any order of a group's columns will do, if it is one for both.
+template <int WM, int WN, int FM, int FN, int STAGES, bool NARROW>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product p, BlockGrid grid) {
+  typedef Tile<WM, WN, FM, FN, STAGES> T;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave_m = wave / WN, wave_n = wave % WN;
+  // the tiles of an XCD side by side, four rows of tiles at a time
+  int m, n;
+  {
+    const int total = gridDim.x, tiles_m = total / grid.tiles_n, x = blockIdx.x % grid.xcds;
+    const int tile = total / grid.xcds * x + min(x, total % grid.xcds) + blockIdx.x / grid.xcds;
+    constexpr int kStrip = 4;
+    const int strip = tile / (kStrip * grid.tiles_n), rest = tile - strip * kStrip * grid.tiles_n, high = min(kStrip, tiles_m - strip * kStrip);
+    n = rest / high;
+    m = strip * kStrip + rest - n * high;
+  }
+  const int split = blockIdx.y, all = p.columns / ONEBIT_CODE_GROUP, begin = split * grid.groups_per_split, count = min(grid.groups_per_split, all - begin);
+
+  // copies: eight rows each, the weight's first
+  uint32_t offset[T::kCopies];
+#pragma unroll
+  for (int c = 0; c < T::kCopies; ++c) {
+    const int piece = c * T::kWaves + wave, row = piece * 8 + lane / 8, chunk = (lane % 8) ^ (row / 2 % 8);
+    const bool of_weight = c < T::kRows / 8 / T::kWaves;
+    const int from = of_weight ? min(m * T::kRows + row, p.rows - 1) - m * T::kRows : min(n * T::kTokens + row - T::kRows, p.tokens - 1) - n * T::kTokens;
+    offset[c] = (uint32_t)(from * (int)(of_weight ? p.weight.row_stride : p.x.row_stride) + chunk * 16);
+  }
+  const char* weight = (const char*)p.weight.codes + (long long)m * T::kRows * p.weight.row_stride + (long long)begin * ONEBIT_CODE_GROUP;
+  const char* x = (const char*)p.x.codes + (long long)n * T::kTokens * p.x.row_stride + (long long)begin * ONEBIT_CODE_GROUP;
+  const float* x_scale = p.x.scales + (long long)min(n * T::kTokens + wave_n * FN * 16 + lane % (FN * 16), p.tokens - 1) * p.x.scale_stride;
+  const float* w_scale = p.weight.scales + (long long)min((m * T::kRows + wave_m * FM * 16) / ONEBIT_CODE_GROUP, (p.rows - 1) / ONEBIT_CODE_GROUP) * p.weight.scale_stride + begin;
+  const uint32_t lds = lds_offset_of(smem);
+  auto copy = [&](int c, int g, int stage) {  // of a group beyond the last: of the last again, so that as many copies are under way
+    g = min(g, count - 1);
+    const uint32_t to = lds + stage * T::kStage;
+    lds_dma16_base((c < T::kRows / 8 / T::kWaves ? weight : x) + (long long)g * ONEBIT_CODE_GROUP, offset[c], to + (c * T::kWaves + wave) * 1024);
+  };
+  // Scales of groups 4 b ... 4 b + 3; where the row ends among them, its last four. Each in a line of its own, they would cost a copy as much of the load path as eight rows of codes.
+  const uint32_t scales = STAGES * T::kStage + wave * T::kScales;
+  auto first_scale = [&](int b) { return min(begin + 4 * b, all - 4); };
+  auto copy_scales = [&](int b) { lds_dma16(x_scale + first_scale(b), lds + scales + b % 2 * 1024); };
+
+  typedef Operand<NARROW> Values;
+  f4_t sum[FM][FN] = {}, part[2][FN] = {};
+  float scale[FN] = {};
+  // this lane's pieces of row lane % 16 of a 16-row part
+  const int r = lane % 16, q = lane / 16, low = r * ONEBIT_CODE_GROUP + (q ^ (r / 2)) * 16, high = r * ONEBIT_CODE_GROUP + ((q + 4) ^ (r / 2)) * 16;
+  auto read = [&](const char* part) { return Values(*(const u4_t*)(part + low), *(const u4_t*)(part + high)); };
+  auto add = [&](f4_t& to, const f4_t& v, float s) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = __builtin_fmaf(v[e], s, to[e]);
+  };
+  // Registers hold what the products need next: all of the tokens' values of a group, and some rows of the weight's.
+  Values av[T::kSlots], bv[FN];
+  float next[FN];
+  auto read_weight = [&](int stage, int i) { av[i % T::kSlots] = read(smem + stage * T::kStage + (wave_m * FM + i) * 16 * ONEBIT_CODE_GROUP); };
+  auto read_tokens = [&](int stage, int j) { bv[j] = read(smem + stage * T::kStage + (T::kRows + (wave_n * FN + j) * 16) * ONEBIT_CODE_GROUP); };
+  auto read_scales = [&](int g) {
+    const float* const of_group = (const float*)(smem + scales + g / 4 % 2 * 1024) + (begin + g - first_scale(g / 4));
+#pragma unroll
+    for (int j = 0; j < FN; ++j) next[j] = of_group[(j * 16 + r) * 4];
+  };
+  // The weight's scales of 64 groups, one to a lane: a load in the loop would be waited for with the copies in front of it.
+  auto read_weight_scales = [&](int g) {
+    float w = w_scale[min(g + lane, count - 1)];
+    asm volatile("" : "+v"(w));  // (waited for here)
+    return w;
+  };
+  float w = read_weight_scales(0);
+  copy_scales(0);
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+#pragma unroll
+    for (int c = 0; c < (s == STAGES - 1 ? T::kEarly : T::kCopies); ++c) copy(c, s, s);
+  wait_vmcnt_lgkm0<(STAGES - 2) * T::kCopies + T::kEarly>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < FN; ++j) read_tokens(0, j);
+  read_weight(0, 0);
+  read_weight(0, 1);
+  read_scales(0);
+  int stage = 0;
+  for (int g = 0; g < count; ++g) {
+    const int following = stage + 1 == STAGES ? 0 : stage + 1, leading = stage ? stage - 1 : STAGES - 1;
+    // the last group's last row; nothing before the first
+#pragma unroll
+    for (int j = 0; j < FN; ++j) add(sum[FM - 1][j], part[(FM - 1) % 2][j], scale[j]);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) scale[j] = next[j] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), g % 64));
+    if (g % 64 == 63) w = read_weight_scales(g + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      if (i == T::kLanding) {
+        wait_vmcnt_lgkm0<(STAGES - 2) * T::kCopies + T::copies_before(T::kLanding)>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      } else if (i == T::kRelease) {
+        wait_lgkm0();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      // rows 2 ... FM - 1 of the weight by row kRelease, two at a time in front and at the end
+      if (i < T::kRelease) {
+        constexpr int kDouble = FM - 2 - T::kRelease;  // rows of products that read two
+        const int first = 2 + i + min(i, (kDouble + 1) / 2) + max(0, i - (T::kRelease - kDouble / 2));
+        const bool two = i < (kDouble + 1) / 2 || i >= T::kRelease - kDouble / 2;
+        if (first < FM) read_weight(stage, first);
+        if (two) read_weight(stage, first + 1);
+      }
+      if (i == T::kLanding) read_scales(min(g + 1, count - 1));
+      if (i == 0 && g % 4 == 0 && g + 4 < count) copy_scales(g / 4 + 1);
+      if (i == FM - 1) read_weight(following, 0);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        part[i % 2][j] = av[i % T::kSlots] * bv[j];
+        if (i > 0) add(sum[i - 1][j], part[(i - 1) % 2][j], scale[j]);
+        if (i == FM - 1) read_tokens(following, j);
+        // products from row kRelease on, in the next group's rows from there on
+        const int at = (i >= T::kRelease ? i - T::kRelease : FM - T::kRelease + i) * FN + j;
+        if (at % T::kApart == 0) {
+#pragma unroll
+          for (int c = at / T::kApart * T::kAtOnce; c < min((at / T::kApart + 1) * T::kAtOnce, T::kCopies); ++c) {
+            if (i >= T::kRelease) copy(c, g + STAGES, stage);
+            else copy(c, g - 1 + STAGES, leading);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    read_weight(following, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    stage = following;
+  }
+#pragma unroll
+  for (int j = 0; j < FN; ++j) add(sum[FM - 1][j], part[(FM - 1) % 2][j], scale[j]);
+  wait_vmcnt<0>();  // none into what follows, nor into LDS that another workgroup has by then
+  __syncthreads();
+
+  // Sixteen tokens at a time through LDS: a lane then has eight neighbouring rows of a token.
+  const Result result(p, grid, split);
+  constexpr int kLanes = FM * 2, kPitch = FM * 16 + 4;  // lanes to a token, floats between tokens
+  float* const rows = (float*)smem + wave * 16 * kPitch;
+  static_assert(T::kWaves * 16 * kPitch * 4 <= T::kLds, "");
+  const int row = m * T::kRows + wave_m * FM * 16 + lane % kLanes * 8;
+  float bias[8];
+  result.load_bias(row, bias);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) *(f4_t*)(rows + r * kPitch + i * 16 + q * 4) = sum[i][j];
+    __builtin_amdgcn_wave_barrier();
+    const int first = n * T::kTokens + (wave_n * FN + j) * 16;
+    if (result.vectors) {
+#pragma unroll 1
+      for (int t = lane / kLanes; t < 16 && first + t < p.tokens; t += 64 / kLanes) {
+        const f4_t v0 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8), v1 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8 + 4);
+        const float v[8] = {v0.x + bias[0], v0.y + bias[1], v0.z + bias[2], v0.w + bias[3], v1.x + bias[4], v1.y + bias[5], v1.z + bias[6], v1.w + bias[7]};
+        result.put(first + t, row, v);
+      }
+    } else {  // neighbours from neighbouring lanes
+      constexpr int kAcross = FM * 16 < 64 ? FM * 16 : 64;
+#pragma unroll 1
+      for (int t = lane / kAcross; t < 16 && first + t < p.tokens; t += 64 / kAcross)
+#pragma unroll
+        for (int at = 0; at < FM * 16; at += kAcross) result.put_one(first + t, m * T::kRows + wave_m * FM * 16 + at + lane % kAcross, rows[t * kPitch + at + lane % kAcross]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int WM, int WN, int FM, int FN, int STAGES, bool NARROW>
+hipError_t launch_tiles_as(const onebit_block_product& p, BlockGrid grid, hipStream_t stream) {
+  typedef Tile<WM, WN, FM, FN, STAGES> T;
+  auto kernel = tile_kernel<WM, WN, FM, FN, STAGES, NARROW>;
+  // the dynamic-LDS limit is a per-device attribute of the kernel; threads that race here set the same value
+  static std::atomic<bool> set[64] = {};
+  int device = 0;
+  if (hipError_t status = hipGetDevice(&device); status != hipSuccess) return status;
+  if (device < 0 || device >= 64) return hipErrorInvalidDevice;
+  if (!set[device].load(std::memory_order_acquire)) {
+    if (hipError_t status = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds); status != hipSuccess) return status;
+    set[device].store(true, std::memory_order_release);
+  }
+  const int tiles_m = (p.rows + T::kRows - 1) / T::kRows, tiles_n = (p.tokens + T::kTokens - 1) / T::kTokens;
+  grid.tiles_n = tiles_n;
+  if ((long long)tiles_m * tiles_n * 64 * T::kWaves >= 1ll << 32) return hipErrorInvalidConfiguration;
+  return launch_kernel(kernel, dim3((unsigned)((long long)tiles_m * tiles_n), grid.splits), dim3(64 * T::kWaves), T::kLds, stream, p, grid);
+}
+
+template <int WM, int WN, int FM, int FN, int STAGES>
+hipError_t launch_tiles(const onebit_block_product& p, const BlockGrid& grid, hipStream_t stream) {
+  // 16-bit results: the 8-bit instruction, twice as fast. It cuts the products of eight neighbouring columns off at 2^-13 of the largest: 1.5e-5 off over normal values, a
+  // fourteenth of an fp16 result's own rounding. fp32 results take the products in fp16.
+  return p.y_dtype == ONEBIT_DTYPE_F32 ? launch_tiles_as<WM, WN, FM, FN, STAGES, false>(p, grid, stream) : launch_tiles_as<WM, WN, FM, FN, STAGES, true>(p, grid, stream);
+}
+
+}  // namespace
+
+hipError_t launch_block_tiles(const onebit_block_product& p, const BlockGrid& grid, hipStream_t stream) {
+  switch (grid.kernel) {
+    case kBlock128x32: return launch_tiles<4, 1, 2, 2, 3>(p, grid, stream);
+    case kBlock64x64: return launch_tiles<2, 2, 2, 2, 4>(p, grid, stream);
+    case kBlock128x64: return launch_tiles<4, 2, 2, 2, 3>(p, grid, stream);
+    case kBlock256x128: return launch_tiles<4, 2, 4, 4, 3>(p, grid, stream);
+    default:
+      // (in fp16 the wave tile of 128 x 64 spills)
+      return p.y_dtype == ONEBIT_DTYPE_F32 ? launch_tiles_as<4, 2, 4, 4, 2, false>(p, grid, stream) : launch_tiles_as<2, 4, 8, 4, 2, true>(p, grid, stream);
+  }
+}
+
+}  // namespace onebit

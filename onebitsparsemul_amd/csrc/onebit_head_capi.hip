@@ -42,14 +42,18 @@ int onebit_quantize_rows(const void* x, int dtype, long long x_stride, int rows,
 size_t onebit_block_linear_workspace(const onebit_block_product* product) {
   onebit::report(ONEBIT_OK, "");
   if (check_product(product)) return 0;
-  return 0;
+  return onebit::block_workspace(*product, onebit::plan_block(*product, onebit::device_compute_units()));
 }
 
 int onebit_block_linear(const onebit_block_product* product, void* workspace, void* stream) {
   onebit::report(ONEBIT_OK, "");
   CHECKED(check_product(product));
-  (void)workspace;
-  return launched(onebit::launch_block_linear(*product, (hipStream_t)stream), "onebit_block_linear");
+  onebit::BlockGrid grid = onebit::plan_block(*product, onebit::device_compute_units());
+  if (const size_t bytes = onebit::block_workspace(*product, grid)) {
+    if (!workspace || !aligned(workspace, 16)) return refuse("this call needs a workspace of %zu bytes, 16-byte aligned", bytes);
+    grid.partial = (float*)workspace;
+  }
+  return launched(onebit::launch_block_linear(*product, grid, (hipStream_t)stream), "onebit_block_linear");
 }
 
 size_t onebit_sample_workspace(const onebit_sampling* sampling) {

@@ -7,7 +7,21 @@ namespace onebit {
 
 hipError_t launch_quantize_rows(const void* x, int dtype, long long x_stride, int rows, int columns, const onebit_codes& out, hipStream_t stream);
 
-hipError_t launch_block_linear(const onebit_block_product& args, hipStream_t stream);
+// A product's launch. Groups of 128 columns split over workgroups: split s takes groups [s * groups_per_split, ...) of all, and writes fp32 sums to
+// partial + s * tokens * rows; a second kernel adds them in order. splits == 1: straight into y.
+enum BlockKernel { kBlock16, kBlock16Wide, kBlock64, kBlock128x32, kBlock64x64, kBlock128x64, kBlock256x128, kBlock256x256 };  // rows of the weight (a sixteenth; wide: on eight wavefronts); rows x tokens
+constexpr int kLeastTileGroups = 4;  // of a tile's split
+struct BlockGrid {
+  int tiles_n;  // of tokens, filled by the launcher
+  int kernel;
+  int splits, groups_per_split;
+  int xcds;  // workgroup b runs on XCD b % xcds
+  float* partial;
+};
+BlockGrid plan_block(const onebit_block_product& args, int compute_units);
+size_t block_workspace(const onebit_block_product& args, const BlockGrid& grid);
+hipError_t launch_block_linear(const onebit_block_product& args, const BlockGrid& grid, hipStream_t stream);
+hipError_t launch_block_tiles(const onebit_block_product& args, const BlockGrid& grid, hipStream_t stream);  // without the pass that adds splits
 
 hipError_t launch_sample(const onebit_sampling& args, hipStream_t stream);
 
