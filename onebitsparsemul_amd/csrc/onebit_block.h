@@ -52,19 +52,20 @@ struct Result {
         vectors(stride % 8 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0),
         bias(grid.splits > 1 ? nullptr : p.bias),
         bias_type(p.bias_dtype) {}
+  __device__ float bias_of(int row) const { return bias && row < rows ? value_at(bias, bias_type, row) : 0.f; }
   __device__ void load_bias(int row, float (&v)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = bias && row + i < rows ? value_at(bias, bias_type, row + i) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = bias_of(row + i);
   }
-  // one sum, without the bias
+  // sums with the bias: one
   __device__ void put_one(int token, int row, float v) const {
     if (row >= rows) return;
-    const float one[1] = {bias ? v + value_at(bias, bias_type, row) : v};
+    const float one[1] = {v};
     if (type == ONEBIT_DTYPE_F32) store_values<ONEBIT_DTYPE_F32, 1>(base, token * stride + row, one);
     else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 1>(base, token * stride + row, one);
     else store_values<ONEBIT_DTYPE_BF16, 1>(base, token * stride + row, one);
   }
-  // eight sums of a token from weight row `row` on, a multiple of eight, with the bias
+  // and eight of a token from weight row `row` on, a multiple of eight
   __device__ void put(int token, int row, const float (&v)[8]) const {
     const long long at = token * stride + row;
     if (vectors && row + 8 <= rows) {

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(onebit_block_product p,
     float total = 0.f;
 #pragma unroll
     for (int s = 0; s < WAVES; ++s) total += sums[s][t][row];
-    result.put_one(first_token + t, first_row + row, total);
+    result.put_one(first_token + t, first_row + row, total + result.bias_of(first_row + row));
   }
 }
 

@@ -173,8 +173,12 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product
   float* const rows = (float*)smem + wave * 16 * kPitch;
   static_assert(T::kWaves * 16 * kPitch * 4 <= T::kLds, "");
   const int row = m * T::kRows + wave_m * FM * 16 + lane % kLanes * 8;
-  float bias[8];
+  constexpr int kAcross = FM * 16 < 64 ? FM * 16 : 64;  // or one row after the other
+  const int single = m * T::kRows + wave_m * FM * 16 + lane % kAcross;
+  float bias[8], single_bias[FM * 16 / kAcross];
   result.load_bias(row, bias);
+#pragma unroll
+  for (int at = 0; at < FM * 16 / kAcross; ++at) single_bias[at] = result.bias_of(single + at * kAcross);
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
 #pragma unroll
@@ -189,11 +193,11 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product
         result.put(first + t, row, v);
       }
     } else {  // neighbours from neighbouring lanes
-      constexpr int kAcross = FM * 16 < 64 ? FM * 16 : 64;
-#pragma unroll 1
-      for (int t = lane / kAcross; t < 16 && first + t < p.tokens; t += 64 / kAcross)
+#pragma unroll 4
+      for (int t = lane / kAcross; t < 16; t += 64 / kAcross)
 #pragma unroll
-        for (int at = 0; at < FM * 16; at += kAcross) result.put_one(first + t, m * T::kRows + wave_m * FM * 16 + at + lane % kAcross, rows[t * kPitch + at + lane % kAcross]);
+        for (int at = 0; at < FM * 16 / kAcross; ++at)
+          if (first + t < p.tokens) result.put_one(first + t, single + at * kAcross, rows[t * kPitch + at * kAcross + lane % kAcross] + single_bias[at]);
     }
     __builtin_amdgcn_wave_barrier();
   }

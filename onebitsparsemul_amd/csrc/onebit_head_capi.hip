@@ -58,15 +58,15 @@ int onebit_block_linear(const onebit_block_product* product, void* workspace, vo
 
 size_t onebit_sample_workspace(const onebit_sampling* sampling) {
   onebit::report(ONEBIT_OK, "");
-  if (check_sampling(sampling)) return 0;
-  return 0;
+  return check_sampling(sampling) ? 0 : onebit::sample_workspace(*sampling);
 }
 
 int onebit_sample(const onebit_sampling* sampling, void* workspace, void* stream) {
   onebit::report(ONEBIT_OK, "");
   CHECKED(check_sampling(sampling));
-  (void)workspace;
-  return launched(onebit::launch_sample(*sampling, (hipStream_t)stream), "onebit_sample");
+  const size_t bytes = onebit::sample_workspace(*sampling);
+  if (bytes && (!workspace || !aligned(workspace, 16))) return refuse("this call needs a workspace of %zu bytes, 16-byte aligned", bytes);
+  return launched(onebit::launch_sample(*sampling, workspace, (hipStream_t)stream), "onebit_sample");
 }
 
 }  // extern "C"

@@ -23,6 +23,7 @@ size_t block_workspace(const onebit_block_product& args, const BlockGrid& grid);
 hipError_t launch_block_linear(const onebit_block_product& args, const BlockGrid& grid, hipStream_t stream);
 hipError_t launch_block_tiles(const onebit_block_product& args, const BlockGrid& grid, hipStream_t stream);  // without the pass that adds splits
 
-hipError_t launch_sample(const onebit_sampling& args, hipStream_t stream);
+size_t sample_workspace(const onebit_sampling& args);
+hipError_t launch_sample(const onebit_sampling& args, void* workspace, hipStream_t stream);
 
 }  // namespace onebit

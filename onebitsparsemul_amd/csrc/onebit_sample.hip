@@ -1,13 +1,21 @@
-// Tokens from logits (onebit_head.h). Nothing is sorted: the filters keep what lies above a value, and of the logits equal to it those of the lowest indices, so
-// that each of them is a search for that value, digit by digit from the top in a histogram of counts and masses. Masses are integers (2^-42 of the largest
+// Tokens from logits (onebit_head.h). Nothing is sorted: what the filters keep lies above a value, with those of the logits equal to it that have the lowest indices, so
+// that a filter is a search for that value, a digit after the other in a histogram of counts or masses. Masses are integers (2^-42 of the largest
 // weight): their sums do not depend on an order, and 2^-43 is the most a weight is off, so that which token a number falls on is what 64-bit sums give.
+//
+// A row is looked at once in full: the largest of each group of neighbouring logits stays. The k largest logits are not below the k-th largest of the groups' largest, and
+// those that make up a share of the mass not below the value above which the groups' largest make it up alone; so that the filters
+// see a list of few candidates, from the few groups that reach that value, in the order of their indices. Where a list would not hold them they go over the row's groups instead.
 #include "onebit_decoder_device.h"
 #include "onebit_head_launch.h"
+
+#include <algorithm>
 
 namespace onebit {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048, kFraction = 42;
+constexpr int kBins = 2048, kFraction = 42, kListed = 4096, kAll = INT_MAX;
+constexpr int kGroup = 16, kGroups = 8192;        // logits of a group, or that times a power of two; groups of a row
+constexpr int kChunk = 4096, kChunkThreads = 256;  // logits of a workgroup of the first pass
 typedef unsigned long long mass_t;
 
 // Floats as integers of the same order; -0 as 0.
@@ -16,35 +24,54 @@ __device__ inline uint32_t key_of(float x) {
   return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ inline float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
-constexpr uint32_t kKeyOfMinusInfinity = 0x007fffffu;
+constexpr uint32_t kKeyOfNan = 0xffffffffu, kLeast = 0x00800000u, kNothing = 0;  // the key of the lowest finite logit; nothing: below all
+__device__ inline uint32_t key_or_nan(float x) { return x != x ? kKeyOfNan : key_of(x); }
 
-// The weight of a logit as an integer: 2^(distance + 42), distance = log2 e (logit - largest) / temperature <= 0. 2^n r, r by the exponential series of the fraction
-// of n, at most 1/2: its twelve terms leave 2e-14 out.
-__device__ inline mass_t weight_of(double distance) {
-  if (!(distance >= -kFraction - 1)) return 0;
-  const double n = __builtin_rint(distance), x = (distance - n) * 0.693147180559945309417;
+// 2^(x + 42) as an integer, x <= 0: 2^n r, r by the exponential series of the fraction of x, at most 1/2 of either sign: its twelve terms leave 2e-14 out.
+__device__ inline mass_t power_as_integer(double x) {
+  if (!(x >= -kFraction - 1)) return 0;
+  const double n = __builtin_rint(x), f = (x - n) * 0.693147180559945309417;
   double r = 1. / 39916800;
-  r = r * x + 1. / 3628800;
-  r = r * x + 1. / 362880;
-  r = r * x + 1. / 40320;
-  r = r * x + 1. / 5040;
-  r = r * x + 1. / 720;
-  r = r * x + 1. / 120;
-  r = r * x + 1. / 24;
-  r = r * x + 1. / 6;
-  r = r * x + 0.5;
-  r = r * x + 1.;
-  r = r * x + 1.;
+  r = r * f + 1. / 3628800;
+  r = r * f + 1. / 362880;
+  r = r * f + 1. / 40320;
+  r = r * f + 1. / 5040;
+  r = r * f + 1. / 720;
+  r = r * f + 1. / 120;
+  r = r * f + 1. / 24;
+  r = r * f + 1. / 6;
+  r = r * f + 0.5;
+  r = r * f + 1.;
+  r = r * f + 1.;
   // (added to 2^52, the integer stands in the low bits)
   return (mass_t)(__double_as_longlong(__builtin_ldexp(r, (int)n + kFraction) + 4503599627370496.0) & 0xfffffffffffffll);
 }
 
-template <class T>
-__device__ inline T wave_total(T x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
+// Weights beside the row's, or a part's, largest logit
+struct Scale {
+  uint32_t largest;  // its key
+  float top;         // its value
+  double rate;       // log2 e / temperature
+  __device__ Scale(uint32_t key, float temperature) : largest(key), top(value_of(key)), rate(1.44269504088896340736 / (double)temperature) {}
+  __device__ double distance(float logit) const { return logit == top ? 0. : ((double)logit - (double)top) * rate; }
+  __device__ mass_t weight(uint32_t key) const { return key == largest ? (mass_t)1 << kFraction : power_as_integer(distance(value_of(key))); }
+};
+
+struct Parameters {
+  float temperature, top_p, min_p;
+  int top_k;
+  bool greedy, masses;  // the first token alone; all of the row's mass counts
+  __device__ Parameters(const onebit_sampling& a, int row) {
+    temperature = a.temperatures ? a.temperatures[row] : a.temperature;
+    top_p = a.top_ps ? a.top_ps[row] : a.top_p;
+    min_p = a.min_ps ? a.min_ps[row] : a.min_p;
+    top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+    if (top_k <= 0 || top_k >= a.vocabulary) top_k = kAll;
+    greedy = !(temperature > 0.f) || top_k == 1 || min_p > 1.f || top_p <= 0.f;
+    masses = !greedy && top_k == kAll && (top_p < 1.f || !(min_p > 0.f));
+  }
+};
+
 template <class T>
 __device__ inline T wave_running(T x, int lane) {  // with the lane's own
 #pragma unroll
@@ -54,14 +81,20 @@ __device__ inline T wave_running(T x, int lane) {  // with the lane's own
   }
   return x;
 }
-
-struct Row {
-  uint32_t largest;  // key of the largest logit
-  float top;         // its value
-  double rate;       // log2 e / temperature
-  __device__ double distance(float logit) const { return logit == top ? 0. : ((double)logit - (double)top) * rate; }
-  __device__ mass_t weight(uint32_t key) const { return key == largest ? (mass_t)1 << kFraction : weight_of(distance(value_of(key))); }
-};
+__device__ inline mass_t wave_sum_of(mass_t x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+template <class T>
+__device__ inline T wave_most(T x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const T other = __shfl_xor(x, d);
+    x = other > x ? other : x;
+  }
+  return x;
+}
 
 // What stays of a row: keys above `key` and the first `ties` of those equal to it
 struct Kept {
@@ -69,172 +102,531 @@ struct Kept {
   int ties;
 };
 
+template <int THREADS>
 struct Shared {
-  uint32_t count[kBins];
-  mass_t mass[kBins];
-  mass_t parts[kWaves];
+  mass_t bins[kBins];
+  uint32_t keys[kListed], indices[kListed];  // candidates in the order of their indices
+  uint32_t reaching[kGroups / 2];            // groups that reach the candidates' value, 16 bits each
+  mass_t parts[2][THREADS / 64];
   mass_t above;
-  mass_t other;
-  uint32_t digit;
+  uint32_t bin;
 };
 
-// The key in the falling order of those in `kept` behind which the running count or mass is `share` of the total or more (for counts: share is the count). In each
-// pass the digit of 11 or 10 bits in whose bin that happens.
-template <int TYPE, bool MASS>
-__device__ Kept search(const void* logits, long long base, int vocabulary, const Row& row, const Kept& kept, double share, Shared& s) {
+// A workgroup of THREADS on a row
+template <int THREADS>
+struct Block {
+  Shared<THREADS>& s;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  uint32_t prefix = 0;
-  mass_t above = 0, target = 0;
-  int shift = 21, bits = 11;
-  const mass_t tied = kept.ties == INT_MAX ? 0 : (MASS ? row.weight(kept.key) : 1) * kept.ties;
-  for (int level = 0; level < 3; ++level) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
+  int turn = 0;  // which of the parts is next, so that one barrier does
+  __device__ Block(Shared<THREADS>& shared) : s(shared) {}
+
+  __device__ mass_t most(mass_t x) {
+    x = wave_most(x);
+    mass_t* const parts = s.parts[turn ^= 1];
+    if (lane == 0) parts[wave] = x;
     __syncthreads();
-    for (int i = threadIdx.x; i < vocabulary; i += kThreads) {
-      float x[1];
-      load_values<TYPE, 1>(logits, base + i, x);
-      const uint32_t key = key_of(x[0]);
-      if (key <= kept.key && kept.ties != INT_MAX) continue;
-      if (level && key >> (shift + bits) != prefix) continue;
-      atomicAdd(&s.mass[key >> shift & ((1 << bits) - 1)], MASS ? row.weight(key) : 1);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0 && tied && (!level || kept.key >> (shift + bits) == prefix)) s.mass[kept.key >> shift & ((1 << bits) - 1)] += tied;
-    __syncthreads();
-    const mass_t first = s.mass[kBins - 1 - 2 * threadIdx.x], second = s.mass[kBins - 2 - 2 * threadIdx.x];
-    const mass_t running = wave_running(first + second, lane);
-    if (lane == 63) s.parts[wave] = running;
-    __syncthreads();
-    mass_t before = above, total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) before += s.parts[w];
-      total += s.parts[w];
-    }
-    if (level == 0) {
-      target = MASS ? (mass_t)ceil(share * (double)total) : (mass_t)share;
-      target = min(max(target, (mass_t)1), total);
-    }
-    before += running - first - second;
-    if (before < target && before + first >= target) s.digit = kBins - 1 - 2 * threadIdx.x, s.above = before;
-    before += first;
-    if (before < target && before + second >= target) s.digit = kBins - 2 - 2 * threadIdx.x, s.above = before;
-    __syncthreads();
-    above = s.above;
-    prefix = prefix << bits | s.digit;
-    bits = level == 1 ? 10 : 11;
-    shift = level == 0 ? 10 : 0;
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) x = parts[w] > x ? parts[w] : x;
+    return x;
   }
-  const mass_t each = MASS ? row.weight(prefix) : 1;
-  return {prefix, (int)((target - above + each - 1) / each)};
+  // sum of the threads in front, and of all
+  __device__ mass_t before(mass_t x, mass_t& total) {
+    const mass_t running = wave_running(x, lane);
+    mass_t* const parts = s.parts[turn ^= 1];
+    if (lane == 63) parts[wave] = running;
+    __syncthreads();
+    mass_t front = running - x;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      const mass_t part = parts[w];
+      if (w < wave) front += part;
+      total += part;
+    }
+    return front;
+  }
+
+  // The key, from `high` down to `low`, with which the running sum of the items' amounts comes to `target` or more, the sum in front of it, and whether it comes to it. each(f) calls
+  // f(key, amount) for the thread's items. In each round the bin of 2^shift keys in which that happens.
+  template <class Each>
+  __device__ bool search(uint32_t high, uint32_t low, mass_t target, Each each, uint32_t& key, mass_t& in_front) {
+    mass_t above = 0;
+    for (;;) {
+      const int shift = max(0, 32 - __clz((int)(high - low)) - 11);
+      for (int i = threadIdx.x; i < kBins; i += THREADS) s.bins[i] = 0;
+      __syncthreads();
+      each([&](uint32_t own, mass_t amount) {
+        if (own <= high && own >= low) atomicAdd(&s.bins[(high - own) >> shift], amount);
+      });
+      __syncthreads();
+      constexpr int kEach = kBins / THREADS;
+      mass_t own[kEach], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += own[i] = s.bins[threadIdx.x * kEach + i];
+      mass_t front = above + before(sum, total);
+      if (above + total < target) return false;  // (in the first round, and for all threads)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (front < target && front + own[i] >= target) s.bin = threadIdx.x * kEach + i, s.above = front;
+        front += own[i];
+      }
+      __syncthreads();
+      above = s.above;
+      high -= s.bin << shift;
+      low = max(low, high - ((1u << shift) - 1));
+      if (shift == 0) break;
+    }
+    key = high;
+    in_front = above;
+    return true;
+  }
+};
+
+// The filters by rank and by share. each(f) calls f(key) for the thread's items, all of them from key `low` on, in any order; mass: the row's, where it counts.
+template <int THREADS, class Each>
+__device__ Kept filtered(Block<THREADS>& block, const Scale& scale, const Parameters& p, uint32_t low, double mass, Each each) {
+  Kept kept = {kNothing, kAll};
+  uint32_t key;
+  mass_t in_front;
+  if (p.top_k != kAll && block.search(scale.largest, low, p.top_k, [&](auto add) { each([&](uint32_t own) { add(own, (mass_t)1); }); }, key, in_front))
+    kept = {key, p.top_k - (int)in_front};
+  if (p.top_p < 1.f) {
+    const mass_t tied = kept.ties == kAll ? 0 : scale.weight(kept.key) * kept.ties;
+    auto masses = [&](auto add) {
+      each([&](uint32_t own) {
+        if (own > kept.key || kept.ties == kAll) add(own, scale.weight(own));
+      });
+      if (threadIdx.x == 0 && tied) add(kept.key, tied);
+    };
+    if (p.top_k != kAll) {  // of those that top_k left
+      mass_t own_mass = 0, total;
+      masses([&](uint32_t, mass_t amount) { own_mass += amount; });
+      block.before(own_mass, total);
+      mass = (double)total;
+    }
+    // (where rounding leaves the running sum below: all stay)
+    const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
+    if (block.search(scale.largest, max(low, kept.key), target, masses, key, in_front)) {
+      const mass_t one = scale.weight(key);
+      kept = {key, (int)((target - in_front + one - 1) / one)};
+    }
+  }
+  return kept;
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void sample_kernel(onebit_sampling a) {
-  __shared__ Shared s;
-  const int row_at = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const long long base = row_at * a.logits_stride;
-  const float temperature = a.temperatures ? a.temperatures[row_at] : a.temperature;
-  const float top_p = a.top_ps ? a.top_ps[row_at] : a.top_p, min_p = a.min_ps ? a.min_ps[row_at] : a.min_p;
-  const int top_k = a.top_ks ? a.top_ks[row_at] : a.top_k;
+// The weight of an item in the last sum: 0 where min_p leaves it out
+struct Last {
+  const Scale& scale;
+  double least;
+  __device__ Last(const Scale& s, const Parameters& p) : scale(s), least(p.min_p > 0.f ? log2((double)p.min_p) : -__builtin_inf()) {}
+  __device__ mass_t weight(uint32_t key) const { return scale.distance(value_of(key)) >= least ? scale.weight(key) : 0; }
+};
+__device__ inline mass_t target_of(float uniform, double total, mass_t whole) {
+  const double at = uniform > 0.f ? (double)uniform * total : 0.;
+  return at < total ? min((mass_t)at, whole - 1) : whole - 1;
+}
 
-  // the largest, of equals the lowest index; NaN
-  mass_t best = 0;
-  for (int i = threadIdx.x; i < a.vocabulary; i += kThreads) {
-    float x[1];
-    load_values<TYPE, 1>(a.logits, base + i, x);
-    const mass_t own = x[0] != x[0] ? ~(mass_t)0 : (mass_t)key_of(x[0]) << 32 | (0xffffffffu - i);
-    best = own > best ? own : best;
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const mass_t other = __shfl_xor(best, d);
-    best = other > best ? other : best;
-  }
-  if (lane == 0) s.parts[wave] = best;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) best = s.parts[w] > best ? s.parts[w] : best;
-  __syncthreads();
-  Row row;
-  row.largest = (uint32_t)(best >> 32);
-  if (best == ~(mass_t)0 || row.largest == kKeyOfMinusInfinity) {
-    if (threadIdx.x == 0) a.tokens[row_at] = -1;
-    return;
-  }
-  if (!(temperature > 0.f) || top_k == 1 || min_p > 1.f) {  // the first token alone
-    if (threadIdx.x == 0) a.tokens[row_at] = 0xffffffffu - (uint32_t)best;
-    return;
-  }
-  row.top = value_of(row.largest);
-  row.rate = 1.44269504088896340736 / (double)temperature;
-  const double least = min_p > 0.f ? log2((double)min_p) : -__builtin_inf();
-
-  Kept kept = {0, INT_MAX};
-  if (top_k > 0 && top_k < a.vocabulary) kept = search<TYPE, false>(a.logits, base, a.vocabulary, row, kept, top_k, s);
-  if (top_p < 1.f) kept = search<TYPE, true>(a.logits, base, a.vocabulary, row, kept, fmaxf(top_p, 0.f), s);
-
-  // masses of the wavefronts' own parts of the row, in the order of the indices
-  const int part = (a.vocabulary + 64 * kWaves - 1) / (64 * kWaves) * 64, begin = min(wave * part, a.vocabulary), end = min(begin + part, a.vocabulary);
-  auto stays = [&](float x) { return row.distance(x) >= least; };
-  mass_t mass = 0;
-  uint32_t ties = 0;
+// Items 0 ... count - 1, which get(i) gives as key and index, in the order of their indices. Of those that `kept` leaves, the first at which the running mass exceeds `at`,
+// or uniform times the total where `at` is negative. A wavefront has a stretch of the items, 64 of them at a time.
+template <int THREADS, class Get>
+__device__ void choose(Block<THREADS>& block, const Last& last, const Kept& kept, float uniform, double at, int count, Get get, long long* token) {
+  const int stretch = (count + THREADS - 1) / THREADS * 64, begin = min(block.wave * stretch, count), end = min(begin + stretch, count), lane = block.lane;
+  const bool bounded = kept.ties != kAll;
+  const mass_t each = bounded ? last.weight(kept.key) : 0;
+  mass_t ties = 0, mass = 0, ignored, total;
   for (int i = begin + lane; i < end; i += 64) {
-    float x[1];
-    load_values<TYPE, 1>(a.logits, base + i, x);
-    const uint32_t key = key_of(x[0]);
-    if (kept.ties != INT_MAX && key == kept.key) ++ties;
-    else if (key >= kept.key && stays(x[0])) mass += row.weight(key);
+    const uint32_t key = get(i).x;
+    if (bounded && key == kept.key) ++ties;
+    else if (key >= kept.key) mass += last.weight(key);
   }
-  ties = wave_total(ties);
-  mass = wave_total(mass);
-  if (lane == 0) s.parts[wave] = mass, s.count[wave] = ties;
-  __syncthreads();
-  const mass_t each = stays(value_of(kept.key)) ? row.weight(kept.key) : 0;
-  mass_t before = 0, total = 0, own = 0;
-  uint32_t ties_before = 0, own_ties_before = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    const uint32_t left = (uint32_t)kept.ties > ties_before ? (uint32_t)kept.ties - ties_before : 0;
-    const mass_t of_wave = s.parts[w] + each * min(left, s.count[w]);
-    if (w == wave) before = total, own = of_wave, own_ties_before = ties_before;
-    total += of_wave;
-    ties_before += s.count[w];
+  mass_t left = 0;  // ties that the wavefront's stretch may keep
+  if (each) {
+    const mass_t in_front = block.before(ties, ignored), of_wave = wave_sum_of(ties);
+    const mass_t wave_front = __shfl(in_front, 0);
+    left = (mass_t)kept.ties > wave_front ? (mass_t)kept.ties - wave_front : 0;
+    if (lane == 0) mass += min(left, of_wave) * each;
   }
-  const float u = a.uniform[row_at];
-  const double at = u > 0.f ? (double)u * (double)total : 0.;
-  const mass_t target = at < (double)total ? min((mass_t)at, total - 1) : total - 1;
-  if (target < before || target >= before + own) return;
-  mass_t running = before;
+  const mass_t running = block.before(mass, total), of_wave = wave_sum_of(mass);
+  const mass_t target = at < 0. ? target_of(uniform, (double)total, total) : min((mass_t)at, total - 1);
+  mass_t front = __shfl(running, 0);
+  if (front > target || front + of_wave <= target) return;
   for (int i = begin; i < end; i += 64) {
-    float x[1] = {0.f};
-    if (i + lane < end) load_values<TYPE, 1>(a.logits, base + i + lane, x);
-    const uint32_t key = key_of(x[0]);
-    const bool tie = i + lane < end && kept.ties != INT_MAX && key == kept.key;
+    const bool there = i + lane < end;
+    const u2_t item = there ? get(i + lane) : u2_t{kNothing, 0};
+    const bool tie = there && bounded && item.x == kept.key;
     const mass_t tied = __ballot(tie);
-    const uint32_t rank = own_ties_before + __popcll(tied & (((mass_t)1 << lane) - 1));
     mass_t w = 0;
-    if (tie) w = rank < (uint32_t)kept.ties ? each : 0;
-    else if (i + lane < end && key >= kept.key && stays(x[0])) w = row.weight(key);
-    const mass_t sum = running + wave_running(w, lane);
-    const mass_t over = __ballot(sum > target);
+    if (tie) w = (mass_t)__popcll(tied & (((mass_t)1 << lane) - 1)) < left ? each : 0;
+    else if (there && item.x >= kept.key) w = last.weight(item.x);
+    const mass_t sum = front + wave_running(w, lane), over = __ballot(sum > target);
     if (over) {
-      if (lane == 0) a.tokens[row_at] = i + __builtin_ctzll(over);
+      const int found = __builtin_ctzll(over);
+      if (lane == found) *token = item.y;
       return;
     }
-    running = __shfl(sum, 63);
-    own_ties_before += __popcll(tied);
+    front = __shfl(sum, 63);
+    left -= min(left, (mass_t)__popcll(tied));
   }
 }
 
+// Few candidates: each is compared with each other, wavefronts taking every so manieth of them: how many are in front of it, and their mass
+constexpr int kPaired = 256;
+template <int THREADS>
+__device__ void choose_of_few(Block<THREADS>& block, const Scale& scale, const Last& last, const Parameters& p, double mass, float uniform, int count, long long* token) {
+  Shared<THREADS>& s = block.s;
+  mass_t *const weights = s.bins, *const fronts = s.bins + kPaired, *const ranks = s.bins + 2 * kPaired;
+  const int own = threadIdx.x;
+  if (own < count) weights[own] = scale.weight(s.keys[own]), fronts[own] = ranks[own] = 0;
+  __syncthreads();
+  for (int i = block.lane; i < count; i += 64) {
+    const uint32_t key = s.keys[i];
+    mass_t front = 0;
+    int rank = 0;
+    for (int j = block.wave; j < count; j += THREADS / 64) {
+      const uint32_t other = s.keys[j];
+      const bool better = other > key || (other == key && j < i);
+      rank += better;
+      front += better ? weights[j] : 0;
+    }
+    if (rank) atomicAdd(&ranks[i], (mass_t)rank), atomicAdd(&fronts[i], front);
+  }
+  __syncthreads();
+  const bool there = own < count;
+  bool stays = there && ranks[own] < (mass_t)p.top_k;
+  if (p.top_p < 1.f) {
+    if (p.top_k != kAll) {
+      mass_t total;
+      block.before(stays ? weights[own] : 0, total);
+      mass = (double)total;
+    }
+    stays = stays && fronts[own] < max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
+  }
+  const mass_t w = stays ? last.weight(s.keys[own]) : 0;
+  mass_t total;
+  const mass_t front = block.before(w, total), target = target_of(uniform, (double)total, total);
+  if (front <= target && front + w > target) *token = s.indices[own];
+}
+
+// The row's groups of `group` logits: the thread's are kCount from number `first` on, their largest keys as given; key(i): of logit i.
+template <int THREADS, int kCount, class Key>
+__device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount], int first, int group, Key key_at, const onebit_sampling& a, int row, const Scale& scale,
+                           const Parameters& p, double mass) {
+  Shared<THREADS>& s = block.s;
+  // a value that all candidates reach, above -inf
+  uint32_t low = kLeast, key;
+  mass_t in_front;
+  auto largest = [&](auto add, auto amount) {
+#pragma unroll 1
+    for (int i = 0; i < kCount; ++i) {
+      uint32_t own = most[0];
+#pragma unroll
+      for (int j = 1; j < kCount; ++j) own = i == j ? most[j] : own;
+      if (own >= kLeast) add(own, amount(own));
+    }
+  };
+  if (p.top_k != kAll) {
+    if (block.search(scale.largest, kLeast, p.top_k, [&](auto add) { largest(add, [](uint32_t) { return (mass_t)1; }); }, key, in_front)) low = key;
+  } else if (p.top_p < 1.f) {
+    const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
+    if (block.search(scale.largest, kLeast, target, [&](auto add) { largest(add, [&](uint32_t own) { return scale.weight(own); }); }, key, in_front)) low = key;
+  }
+  const Last last(scale, p);
+  const float uniform = a.uniform[row];
+  long long* const token = a.tokens + row;
+  // min_p comes behind the others: top_p's mass counts what it leaves out. (It asks for a weight's distance, not a key's: this key may stand a step below the border, which
+  // `last` then decides.)
+  if (p.min_p > 0.f && p.top_p >= 1.f) {
+    const double least = (double)scale.top + last.least / scale.rate;  // (+inf among the logits: only such)
+    const float edge = (float)(least - fabs(least) * 0x1p-22);
+    if (edge == edge) low = max(low, key_of(edge));
+  }
+  // the groups that reach it, in order
+  mass_t own_groups = 0, total;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) own_groups += most[i] >= low;
+  int at = (int)block.before(own_groups, total);
+  uint16_t* const reaching = (uint16_t*)s.reaching;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i)
+    if (most[i] >= low) reaching[at++] = (uint16_t)(first + i);
+  const int items = (int)total * group, shift = __builtin_ctz(group);  // (at most the vocabulary, rounded up)
+  __syncthreads();
+  auto item = [&](int i) {
+    const int index = (int)reaching[i >> shift] * group + (i & (group - 1));
+    return u2_t{index < a.vocabulary ? key_at(index) : kNothing, (uint32_t)index};
+  };
+  // their logits that reach it, listed in order where they are few
+  int listed = 0;
+  for (int i = 0; i < items && listed <= kListed; i += THREADS) {
+    u2_t one = {kNothing, 0};
+    if (i + (int)threadIdx.x < items) one = item(i + threadIdx.x);
+    const bool candidate = one.x >= low;
+    const mass_t to = listed + block.before(candidate ? 1 : 0, total);
+    if (candidate && to < kListed) s.keys[to] = one.x, s.indices[to] = one.y;
+    listed += (int)total;
+  }
+  __syncthreads();
+  if (listed <= kPaired) {
+    choose_of_few(block, scale, last, p, mass, uniform, listed, token);
+  } else if (listed <= kListed) {
+    const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
+      for (int i = threadIdx.x; i < listed; i += THREADS) f(s.keys[i]);
+    });
+    choose(block, last, kept, uniform, -1., listed, [&](int i) { return u2_t{s.keys[i], s.indices[i]}; }, token);
+  } else {
+    auto reached = [&](int i) {
+      u2_t one = item(i);
+      if (one.x < low) one.x = kNothing;
+      return one;
+    };
+    const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
+      for (int i = threadIdx.x; i < items; i += THREADS) f(reached(i).x);
+    });
+    choose(block, last, kept, uniform, -1., items, reached, token);
+  }
+}
+
+// N consecutive logits from `at` on as keys, nothing beyond the row's end
+template <int TYPE, int N>
+__device__ inline void load_keys(const void* logits, long long base, int at, int vocabulary, uint32_t (&keys)[N]) {
+  typedef typename Stored<TYPE>::type T;
+  constexpr int kOf16 = 16 / sizeof(T);
+  typedef T vector __attribute__((ext_vector_type(kOf16), aligned(sizeof(T))));  // (16 bytes from any address)
+  const T* const from = (const T*)logits + base + at;
+  if (at + N <= vocabulary) {
+    vector v[N / kOf16];
+#pragma unroll
+    for (int i = 0; i < N / kOf16; ++i) v[i] = ((const vector*)from)[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) keys[i] = key_or_nan((float)v[i / kOf16][i % kOf16]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) keys[i] = at + i < vocabulary ? key_or_nan((float)from[i]) : kNothing;
+  }
+}
+template <int N>
+__device__ inline uint32_t most_of(const uint32_t (&keys)[N]) {
+  uint32_t most = keys[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) most = max(most, keys[i]);
+  return most;
+}
+// The largest with the lowest index of equals
+template <int N>
+__device__ inline mass_t first_most(const uint32_t (&keys)[N], uint32_t most, int at) {
+  int first = N - 1;
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i)
+    if (keys[i] == most) first = i;
+  return (mass_t)most << 32 | (0xffffffffu - (uint32_t)(at + first));
+}
+// The token where it follows from the largest alone
+__device__ inline bool settled(mass_t best, const Parameters& p, long long* token) {
+  const uint32_t key = (uint32_t)(best >> 32);
+  const bool none = key == kKeyOfNan || key < kLeast;
+  if (!none && !p.greedy) return false;
+  if (threadIdx.x == 0) *token = none ? -1 : (long long)(0xffffffffu - (uint32_t)best);
+  return true;
+}
+
+// A row in one workgroup's LDS
+template <int TYPE, int THREADS, int MOST>
+__global__ __launch_bounds__(THREADS) void sample_short_kernel(onebit_sampling a) {
+  __shared__ Shared<THREADS> s;
+  __shared__ __attribute__((aligned(16))) uint32_t row_keys[MOST];
+  Block<THREADS> block(s);
+  const int row = blockIdx.x;
+  const Parameters p(a, row);
+  constexpr int kCount = MOST / kGroup / THREADS;
+  uint32_t most[kCount];
+  mass_t best = 0;
+#pragma unroll
+  for (int g = 0; g < kCount; ++g) {
+    const int at = (threadIdx.x * kCount + g) * kGroup;
+    uint32_t keys[kGroup];
+    load_keys<TYPE, kGroup>(a.logits, row * a.logits_stride, at, a.vocabulary, keys);
+#pragma unroll
+    for (int i = 0; i < kGroup; i += 4) *(u4_t*)(row_keys + at + i) = u4_t{keys[i], keys[i + 1], keys[i + 2], keys[i + 3]};
+    most[g] = most_of(keys);
+    const mass_t own = first_most(keys, most[g], at);
+    best = own > best ? own : best;
+  }
+  best = block.most(best);  // (with a barrier: the keys are there)
+  if (settled(best, p, a.tokens + row)) return;
+  const Scale scale((uint32_t)(best >> 32), p.temperature);
+  double mass = 0.;
+  if (p.masses) {
+    if (p.top_p >= 1.f) {  // no filter
+      choose(block, Last(scale, p), {kNothing, kAll}, a.uniform[row], -1., a.vocabulary, [&](int i) { return u2_t{row_keys[i], (uint32_t)i}; }, a.tokens + row);
+      return;
+    }
+    mass_t own = 0, total;
+    for (int i = threadIdx.x; i < a.vocabulary; i += THREADS) own += row_keys[i] >= kLeast ? scale.weight(row_keys[i]) : 0;
+    block.before(own, total);
+    mass = (double)total;
+  }
+  sample_row(block, most, threadIdx.x * kCount, kGroup, [&](int i) { return row_keys[i]; }, a, row, scale, p, mass);
+}
+
+// Long rows, first pass: a chunk's largest, its mass beside that where masses count, and its groups' largest
+struct Chunks {
+  mass_t *best, *mass;   // rows x chunks
+  uint32_t* largest;     // rows x groups
+  int chunks, groups;    // of a row
+  int group;             // logits of a group
+};
 template <int TYPE>
-hipError_t launch_as(const onebit_sampling& a, hipStream_t stream) {
-  return launch_kernel(sample_kernel<TYPE>, dim3(a.rows), dim3(kThreads), 0, stream, a);
+__global__ __launch_bounds__(kChunkThreads) void chunk_kernel(onebit_sampling a, Chunks c) {
+  __shared__ mass_t parts[2][kChunkThreads / 64];
+  const int chunk = blockIdx.x, row = blockIdx.y, at = chunk * kChunk + threadIdx.x * kGroup, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const Parameters p(a, row);
+  uint32_t keys[kGroup];
+  load_keys<TYPE, kGroup>(a.logits, row * a.logits_stride, at, a.vocabulary, keys);
+  const uint32_t most = most_of(keys);
+  uint32_t of_group = most;
+  for (int d = 1; d < c.group / kGroup; d <<= 1) of_group = max(of_group, (uint32_t)__shfl_xor((int)of_group, d));
+  const int group = at / c.group;
+  if (at % c.group == 0 && group < c.groups) c.largest[(long long)row * c.groups + group] = of_group;
+  mass_t best = wave_most(first_most(keys, most, at));
+  if (lane == 0) parts[0][wave] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kChunkThreads / 64; ++w) best = parts[0][w] > best ? parts[0][w] : best;
+  const uint32_t key = (uint32_t)(best >> 32);
+  mass_t mass = 0;
+  if (p.masses && key >= kLeast && key != kKeyOfNan) {
+    const Scale scale(key, p.temperature);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) mass += keys[i] >= kLeast ? scale.weight(keys[i]) : 0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) mass += __shfl_xor(mass, d);
+    if (lane == 0) parts[1][wave] = mass;
+    __syncthreads();
+    mass = 0;
+#pragma unroll
+    for (int w = 0; w < kChunkThreads / 64; ++w) mass += parts[1][w];
+  }
+  if (threadIdx.x == 0) {
+    c.best[(long long)row * c.chunks + chunk] = best;
+    c.mass[(long long)row * c.chunks + chunk] = mass;
+  }
+}
+
+constexpr int kLongThreads = 1024;
+template <int TYPE>
+__global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampling a, Chunks c) {
+  __shared__ Shared<kLongThreads> s;
+  Block<kLongThreads> block(s);
+  const int row = blockIdx.x;
+  const Parameters p(a, row);
+  const mass_t own_best = (int)threadIdx.x < c.chunks ? c.best[(long long)row * c.chunks + threadIdx.x] : 0;
+  const mass_t best = block.most(own_best);
+  if (settled(best, p, a.tokens + row)) return;
+  const Scale scale((uint32_t)(best >> 32), p.temperature);
+  auto key_at = [&](int i) {
+    float x[1];
+    load_values<TYPE, 1>(a.logits, row * a.logits_stride + i, x);
+    return key_of(x[0]);
+  };
+  double mass = 0.;
+  if (p.masses) {
+    // The chunks' masses in the row's unit, in their order: 64 bits of a float, rounded alike each time
+    double own = 0.;
+    if ((int)threadIdx.x < c.chunks && (uint32_t)(own_best >> 32) >= kLeast)
+      own = (double)c.mass[(long long)row * c.chunks + threadIdx.x] * exp2(scale.distance(value_of((uint32_t)(own_best >> 32))));
+    // (at most 256 chunks: four wavefronts)
+    double* const sums = (double*)s.bins;
+    const double running = wave_running(own, block.lane);
+    if (block.lane == 63) sums[block.wave] = running;
+    __syncthreads();
+    double front = running - own;
+    for (int w = 0; w < 4; ++w) {
+      if (w < block.wave) front += sums[w];
+      mass += sums[w];
+    }
+    if (p.top_p >= 1.f) {  // no filter: the chunk, then the token in it
+      const float uniform = a.uniform[row];
+      const double at = uniform < 1.f ? (uniform > 0.f ? (double)uniform * mass : 0.) : mass;
+      const mass_t beyond = front + own > at && own > 0. ? 1 : 0, any = own > 0. ? 1 : 0;
+      // the first chunk beyond, or the last one with a mass
+      const mass_t found = block.most(beyond ? (mass_t)1 << 40 | (mass_t)(kLongThreads - threadIdx.x) : any ? (mass_t)threadIdx.x + 1 : 0);
+      const bool over = found >> 40;
+      const int chunk = over ? kLongThreads - (int)(found & 0xffffffff) : (int)found - 1;
+      if ((int)threadIdx.x == chunk) ((double*)s.bins)[16] = over ? at - front : -1.;
+      __syncthreads();
+      double rest = ((double*)s.bins)[16];
+      const int begin = chunk * kChunk, count = min(kChunk, a.vocabulary - begin);
+      // (a chunk whose weights all round to nothing beside the row's largest: its largest)
+      if (scale.weight((uint32_t)(c.best[(long long)row * c.chunks + chunk] >> 32)) == 0) {
+        if (threadIdx.x == 0) a.tokens[row] = 0xffffffffu - (uint32_t)c.best[(long long)row * c.chunks + chunk];
+        return;
+      }
+      if (rest < 0.) rest = 0x1p62;
+      choose(block, Last(scale, p), {kNothing, kAll}, uniform, rest, count, [&](int i) { return u2_t{key_at(begin + i), (uint32_t)(begin + i)}; }, a.tokens + row);
+      return;
+    }
+    __syncthreads();  // the sums' readers are through
+  }
+  constexpr int kCount = kGroups / kLongThreads;
+  const int share = (c.groups + kLongThreads - 1) / kLongThreads, first = threadIdx.x * share;  // at most kCount
+  uint32_t most[kCount];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) most[i] = i < share && first + i < c.groups ? c.largest[(long long)row * c.groups + first + i] : kNothing;
+  sample_row(block, most, first, c.group, key_at, a, row, scale, p, mass);
+}
+
+constexpr int kShort = 8192;
+
+Chunks chunks_of(const onebit_sampling& a, void* workspace) {
+  Chunks c = {};
+  c.chunks = (a.vocabulary + kChunk - 1) / kChunk;
+  c.group = kGroup;
+  while ((a.vocabulary + c.group - 1) / c.group > kGroups) c.group *= 2;
+  c.groups = (a.vocabulary + c.group - 1) / c.group;
+  c.best = (mass_t*)workspace;
+  c.mass = c.best + (size_t)a.rows * c.chunks;
+  c.largest = (uint32_t*)(c.mass + (size_t)a.rows * c.chunks);
+  return c;
+}
+
+template <int TYPE>
+hipError_t launch_as(const onebit_sampling& a, void* workspace, hipStream_t stream) {
+  if ((long long)a.rows * 1024 >= 1ll << 32) return hipErrorInvalidConfiguration;
+  if (a.vocabulary <= kShort) {
+    if (a.vocabulary <= 4096) return launch_kernel(sample_short_kernel<TYPE, 256, 4096>, dim3(a.rows), dim3(256), 0, stream, a);
+    return launch_kernel(sample_short_kernel<TYPE, 512, kShort>, dim3(a.rows), dim3(512), 0, stream, a);
+  }
+  const Chunks c = chunks_of(a, workspace);
+  // (a grid's second dimension ends at 65535: rows in parts)
+  for (int first = 0; first < a.rows; first += 32768) {
+    onebit_sampling part = a;
+    Chunks of_part = c;
+    part.rows = std::min(a.rows - first, 32768);
+    const size_t size = a.logits_dtype == ONEBIT_DTYPE_F32 ? 4 : 2;
+    part.logits = (const char*)a.logits + (long long)first * a.logits_stride * (long long)size;
+    part.uniform += first, part.tokens += first;
+    if (a.temperatures) part.temperatures += first;
+    if (a.top_ps) part.top_ps += first;
+    if (a.min_ps) part.min_ps += first;
+    if (a.top_ks) part.top_ks += first;
+    of_part.best += (size_t)first * c.chunks, of_part.mass += (size_t)first * c.chunks, of_part.largest += (size_t)first * c.groups;
+    if (hipError_t status = launch_kernel(chunk_kernel<TYPE>, dim3(c.chunks, part.rows), dim3(kChunkThreads), 0, stream, part, of_part); status != hipSuccess) return status;
+    if (hipError_t status = launch_kernel(sample_long_kernel<TYPE>, dim3(part.rows), dim3(kLongThreads), 0, stream, part, of_part); status != hipSuccess) return status;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
 
-hipError_t launch_sample(const onebit_sampling& a, hipStream_t stream) {
-  if (a.logits_dtype == ONEBIT_DTYPE_F32) return launch_as<ONEBIT_DTYPE_F32>(a, stream);
-  return a.logits_dtype == ONEBIT_DTYPE_F16 ? launch_as<ONEBIT_DTYPE_F16>(a, stream) : launch_as<ONEBIT_DTYPE_BF16>(a, stream);
+size_t sample_workspace(const onebit_sampling& a) {
+  if (a.vocabulary <= kShort) return 0;
+  const Chunks c = chunks_of(a, nullptr);
+  return (size_t)a.rows * (2 * sizeof(mass_t) * c.chunks + sizeof(uint32_t) * c.groups);
+}
+
+hipError_t launch_sample(const onebit_sampling& a, void* workspace, hipStream_t stream) {
+  if (a.logits_dtype == ONEBIT_DTYPE_F32) return launch_as<ONEBIT_DTYPE_F32>(a, workspace, stream);
+  return a.logits_dtype == ONEBIT_DTYPE_F16 ? launch_as<ONEBIT_DTYPE_F16>(a, workspace, stream) : launch_as<ONEBIT_DTYPE_BF16>(a, workspace, stream);
 }
 
 }  // namespace onebit
