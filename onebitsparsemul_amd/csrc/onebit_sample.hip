@@ -14,6 +14,7 @@ namespace onebit {
 namespace {
 
 constexpr int kBins = 2048, kFraction = 42, kListed = 4096, kAll = INT_MAX;
+constexpr float kFarthest = 50.f;
 constexpr int kGroup = 16, kGroups = 8192;        // logits of a group, or that times a power of two; groups of a row
 constexpr int kChunk = 4096, kChunkThreads = 256;  // logits of a workgroup of the first pass
 typedef unsigned long long mass_t;
@@ -72,28 +73,46 @@ struct Parameters {
   }
 };
 
-template <class T>
-__device__ inline T wave_running(T x, int lane) {  // with the lane's own
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T other = __shfl_up(x, d);
-    if (lane >= d) x += other;
+// Running sums over the lanes, with the lane's own: within rows of 16 by moves of 1, 2, 4 and 8 lanes, then the rows' last lanes to the rows behind.
+template <int CTRL, int ROWS, class T>
+__device__ inline T moved(T x) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+  } else {
+    const u2_t v = __builtin_bit_cast(u2_t, x);
+    return __builtin_bit_cast(T, u2_t{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)v.x, CTRL, ROWS, 0xf, false), (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v.y, CTRL, ROWS, 0xf, false)});
   }
-  return x;
-}
-__device__ inline mass_t wave_sum_of(mass_t x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
 }
 template <class T>
-__device__ inline T wave_most(T x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const T other = __shfl_xor(x, d);
-    x = other > x ? other : x;
+__device__ inline T row_running(T x) {
+  x += moved<0x111, 0xf>(x);
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  return x + moved<0x118, 0xf>(x);
+}
+template <class T>
+__device__ inline T wave_running(T x) {
+  x = row_running(x);
+  x += moved<0x142, 0xa>(x);
+  return x + moved<0x143, 0xc>(x);
+}
+template <class T>
+__device__ inline T of_lane(T x, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+  } else {
+    const u2_t v = __builtin_bit_cast(u2_t, x);
+    return __builtin_bit_cast(T, u2_t{(uint32_t)__builtin_amdgcn_readlane((int)v.x, lane), (uint32_t)__builtin_amdgcn_readlane((int)v.y, lane)});
   }
-  return x;
+}
+__device__ inline mass_t wave_most(mass_t x) {
+  auto larger = [](mass_t a, mass_t b) { return a > b ? a : b; };
+  x = larger(x, moved<0x111, 0xf>(x));
+  x = larger(x, moved<0x112, 0xf>(x));
+  x = larger(x, moved<0x114, 0xf>(x));
+  x = larger(x, moved<0x118, 0xf>(x));
+  x = larger(x, moved<0x142, 0xa>(x));
+  return of_lane(larger(x, moved<0x143, 0xc>(x)), 63);
 }
 
 // What stays of a row: keys above `key` and the first `ties` of those equal to it
@@ -115,35 +134,27 @@ struct Shared {
 // A workgroup of THREADS on a row
 template <int THREADS>
 struct Block {
+  static constexpr int kWaves = THREADS / 64;  // at most 16: the lanes of a row
   Shared<THREADS>& s;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   int turn = 0;  // which of the parts is next, so that one barrier does
   __device__ Block(Shared<THREADS>& shared) : s(shared) {}
 
-  __device__ mass_t most(mass_t x) {
-    x = wave_most(x);
-    mass_t* const parts = s.parts[turn ^= 1];
-    if (lane == 0) parts[wave] = x;
+  // Each wavefront's part, over a barrier: lane w has that of wavefront w
+  template <class T>
+  __device__ T part_of_lane(T own) {
+    T* const parts = (T*)s.parts[turn ^= 1];
+    if (lane == 0) parts[wave] = own;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) x = parts[w] > x ? parts[w] : x;
-    return x;
+    return parts[lane % kWaves];
   }
+  __device__ mass_t most(mass_t x) { return wave_most(part_of_lane(wave_most(x))); }
   // sum of the threads in front, and of all
-  __device__ mass_t before(mass_t x, mass_t& total) {
-    const mass_t running = wave_running(x, lane);
-    mass_t* const parts = s.parts[turn ^= 1];
-    if (lane == 63) parts[wave] = running;
-    __syncthreads();
-    mass_t front = running - x;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-      const mass_t part = parts[w];
-      if (w < wave) front += part;
-      total += part;
-    }
-    return front;
+  template <class T>
+  __device__ T before(T x, T& total) {
+    const T running = wave_running(x), parts = row_running(part_of_lane(of_lane(running, 63)));
+    total = of_lane(parts, kWaves - 1);
+    return running - x + (wave ? of_lane(parts, wave - 1) : 0);
   }
 
   // The key, from `high` down to `low`, with which the running sum of the items' amounts comes to `target` or more, the sum in front of it, and whether it comes to it. each(f) calls
@@ -241,14 +252,14 @@ __device__ void choose(Block<THREADS>& block, const Last& last, const Kept& kept
   }
   mass_t left = 0;  // ties that the wavefront's stretch may keep
   if (each) {
-    const mass_t in_front = block.before(ties, ignored), of_wave = wave_sum_of(ties);
-    const mass_t wave_front = __shfl(in_front, 0);
+    const mass_t in_front = block.before(ties, ignored), of_wave = of_lane(wave_running(ties), 63);
+    const mass_t wave_front = of_lane(in_front, 0);
     left = (mass_t)kept.ties > wave_front ? (mass_t)kept.ties - wave_front : 0;
     if (lane == 0) mass += min(left, of_wave) * each;
   }
-  const mass_t running = block.before(mass, total), of_wave = wave_sum_of(mass);
+  const mass_t running = block.before(mass, total), of_wave = of_lane(wave_running(mass), 63);
   const mass_t target = at < 0. ? target_of(uniform, (double)total, total) : min((mass_t)at, total - 1);
-  mass_t front = __shfl(running, 0);
+  mass_t front = of_lane(running, 0);
   if (front > target || front + of_wave <= target) return;
   for (int i = begin; i < end; i += 64) {
     const bool there = i + lane < end;
@@ -258,13 +269,13 @@ __device__ void choose(Block<THREADS>& block, const Last& last, const Kept& kept
     mass_t w = 0;
     if (tie) w = (mass_t)__popcll(tied & (((mass_t)1 << lane) - 1)) < left ? each : 0;
     else if (there && item.x >= kept.key) w = last.weight(item.x);
-    const mass_t sum = front + wave_running(w, lane), over = __ballot(sum > target);
+    const mass_t sum = front + wave_running(w), over = __ballot(sum > target);
     if (over) {
       const int found = __builtin_ctzll(over);
       if (lane == found) *token = item.y;
       return;
     }
-    front = __shfl(sum, 63);
+    front = of_lane(sum, 63);
     left -= min(left, (mass_t)__popcll(tied));
   }
 }
@@ -312,44 +323,62 @@ template <int THREADS, int kCount, class Key>
 __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount], int first, int group, Key key_at, const onebit_sampling& a, int row, const Scale& scale,
                            const Parameters& p, double mass) {
   Shared<THREADS>& s = block.s;
-  // a value that all candidates reach, above -inf
-  uint32_t low = kLeast, key;
-  mass_t in_front;
-  auto largest = [&](auto add, auto amount) {
-#pragma unroll 1
-    for (int i = 0; i < kCount; ++i) {
-      uint32_t own = most[0];
+  // A value that all candidates reach. Weights 2^-50 of the largest are 0: no such logit matters, whatever its rank.
+  const float steep = (float)scale.rate;
+  float distance[kCount], reach = kFarthest;
 #pragma unroll
-      for (int j = 1; j < kCount; ++j) own = i == j ? most[j] : own;
-      if (own >= kLeast) add(own, amount(own));
+  for (int i = 0; i < kCount; ++i) distance[i] = most[i] >= kLeast ? most[i] == scale.largest ? 0.f : (scale.top - value_of(most[i])) * steep : INFINITY;
+  if (p.top_k != kAll || p.top_p < 1.f) {
+    // The groups' largest within `reach` are top_k, or have top_p of the mass: found by quarters, five times. In fp32, and therefore with some room.
+    const bool by_rank = p.top_k != kAll;
+    const float target = by_rank ? (float)p.top_k : (float)((double)p.top_p * mass * 0x1p-42) * (1.f + 0x1p-10f);
+    float amount[kCount], low = 0.f;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) amount[i] = by_rank ? 1.f : __builtin_amdgcn_exp2f(-distance[i]);
+    for (int round = 0; round < 5; ++round) {
+      const float step = (reach - low) * 0.25f;
+      float sum[3] = {};
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) sum[q] += distance[i] <= low + (q + 1) * step ? amount[i] : 0.f;
+        sum[q] = wave_sum(sum[q]);
+      }
+      float* const parts = (float*)s.bins + (round & 1) * 4 * Block<THREADS>::kWaves;
+      if (block.lane == 0) *(f4_t*)(parts + 4 * block.wave) = f4_t{sum[0], sum[1], sum[2], 0.f};
+      __syncthreads();
+      f4_t all = *(const f4_t*)(parts + 4 * (block.lane % Block<THREADS>::kWaves));
+      int within = 0;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) within += of_lane(row_running(all[q]), Block<THREADS>::kWaves - 1) < target;
+      if (within < 3) reach = low + (within + 1) * step;
+      low += within * step;
     }
-  };
-  if (p.top_k != kAll) {
-    if (block.search(scale.largest, kLeast, p.top_k, [&](auto add) { largest(add, [](uint32_t) { return (mass_t)1; }); }, key, in_front)) low = key;
-  } else if (p.top_p < 1.f) {
-    const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
-    if (block.search(scale.largest, kLeast, target, [&](auto add) { largest(add, [&](uint32_t own) { return scale.weight(own); }); }, key, in_front)) low = key;
   }
+  // (a step further than fp32 rounds)
+  const double farthest = (double)scale.top - ((double)reach * (1. + 0x1p-20) + 0x1p-20) / scale.rate;
+  const float edge = (float)(farthest - fabs(farthest) * 0x1p-22);
+  uint32_t low = edge == edge ? max(kLeast, key_of(edge)) : scale.largest;  // (NaN: +inf among the logits, and only such)
+  mass_t total;
   const Last last(scale, p);
   const float uniform = a.uniform[row];
   long long* const token = a.tokens + row;
-  // min_p comes behind the others: top_p's mass counts what it leaves out. (It asks for a weight's distance, not a key's: this key may stand a step below the border, which
-  // `last` then decides.)
+  // min_p comes behind the others: top_p's mass counts what it leaves out.
   if (p.min_p > 0.f && p.top_p >= 1.f) {
-    const double least = (double)scale.top + last.least / scale.rate;  // (+inf among the logits: only such)
-    const float edge = (float)(least - fabs(least) * 0x1p-22);
-    if (edge == edge) low = max(low, key_of(edge));
+    const double least = (double)scale.top + last.least / scale.rate;
+    const float least_edge = (float)(least - fabs(least) * 0x1p-22);
+    if (least_edge == least_edge) low = max(low, key_of(least_edge));
   }
   // the groups that reach it, in order
-  mass_t own_groups = 0, total;
+  int own_groups = 0, reaching_groups;
 #pragma unroll
   for (int i = 0; i < kCount; ++i) own_groups += most[i] >= low;
-  int at = (int)block.before(own_groups, total);
+  int at = block.before(own_groups, reaching_groups);
   uint16_t* const reaching = (uint16_t*)s.reaching;
 #pragma unroll
   for (int i = 0; i < kCount; ++i)
     if (most[i] >= low) reaching[at++] = (uint16_t)(first + i);
-  const int items = (int)total * group, shift = __builtin_ctz(group);  // (at most the vocabulary, rounded up)
+  const int items = reaching_groups * group, shift = __builtin_ctz(group);  // (at most the vocabulary, rounded up)
   __syncthreads();
   auto item = [&](int i) {
     const int index = (int)reaching[i >> shift] * group + (i & (group - 1));
@@ -357,13 +386,36 @@ __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount]
   };
   // their logits that reach it, listed in order where they are few
   int listed = 0;
-  for (int i = 0; i < items && listed <= kListed; i += THREADS) {
-    u2_t one = {kNothing, 0};
-    if (i + (int)threadIdx.x < items) one = item(i + threadIdx.x);
-    const bool candidate = one.x >= low;
-    const mass_t to = listed + block.before(candidate ? 1 : 0, total);
-    if (candidate && to < kListed) s.keys[to] = one.x, s.indices[to] = one.y;
-    listed += (int)total;
+  constexpr int kBatch = 8;
+  int* const counts = (int*)s.bins;  // of a batch: of each part of it, wavefront by wavefront
+  for (int i = 0; i < items && listed <= kListed; i += kBatch * THREADS) {
+    u2_t one[kBatch];
+    mass_t candidates[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      one[j] = {kNothing, 0};
+      if (i + j * THREADS + (int)threadIdx.x < items) one[j] = item(i + j * THREADS + threadIdx.x);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      candidates[j] = __ballot(one[j].x >= low);
+      if (block.lane == 0) counts[j * Block<THREADS>::kWaves + block.wave] = __popcll(candidates[j]);
+    }
+    __syncthreads();
+    int running[2];  // lane l: of entries 2 l and 2 l + 1
+    constexpr int kEntries = kBatch * Block<THREADS>::kWaves;
+    static_assert(kEntries <= 128, "");
+#pragma unroll
+    for (int e = 0; e < 2; ++e) running[e] = 2 * block.lane + e < kEntries ? counts[2 * block.lane + e] : 0;
+    const int pairs = wave_running(running[0] + running[1]), front = pairs - running[0] - running[1];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int entry = j * Block<THREADS>::kWaves + block.wave;
+      const int to = listed + of_lane(front, entry / 2) + (entry & 1 ? of_lane(running[0], entry / 2) : 0) + __popcll(candidates[j] & (((mass_t)1 << block.lane) - 1));
+      if (one[j].x >= low && to < kListed) s.keys[to] = one[j].x, s.indices[to] = one[j].y;
+    }
+    listed += of_lane(pairs, 63);
   }
   __syncthreads();
   if (listed <= kPaired) {
@@ -498,8 +550,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(onebit_sampling a,
     const Scale scale(key, p.temperature);
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) mass += keys[i] >= kLeast ? scale.weight(keys[i]) : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) mass += __shfl_xor(mass, d);
+    mass = of_lane(wave_running(mass), 63);
     if (lane == 0) parts[1][wave] = mass;
     __syncthreads();
     mass = 0;
@@ -536,7 +587,7 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
       own = (double)c.mass[(long long)row * c.chunks + threadIdx.x] * exp2(scale.distance(value_of((uint32_t)(own_best >> 32))));
     // (at most 256 chunks: four wavefronts)
     double* const sums = (double*)s.bins;
-    const double running = wave_running(own, block.lane);
+    const double running = wave_running(own);
     if (block.lane == 63) sums[block.wave] = running;
     __syncthreads();
     double front = running - own;
@@ -571,7 +622,21 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
   const int share = (c.groups + kLongThreads - 1) / kLongThreads, first = threadIdx.x * share;  // at most kCount
   uint32_t most[kCount];
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) most[i] = i < share && first + i < c.groups ? c.largest[(long long)row * c.groups + first + i] : kNothing;
+  for (int i = 0; i < kCount; ++i) most[i] = kNothing;
+  const uint32_t* const largest = c.largest + (long long)row * c.groups;
+  if (share == kCount && first + kCount <= c.groups) {
+    typedef uint32_t vector __attribute__((ext_vector_type(4), aligned(4)));  // (16 bytes from any address)
+    static_assert(kCount % 4 == 0, "");
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) {
+      const vector v = *(const vector*)(largest + first + i);
+      most[i] = v.x, most[i + 1] = v.y, most[i + 2] = v.z, most[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+      if (i < share && first + i < c.groups) most[i] = largest[first + i];
+  }
   sample_row(block, most, first, c.group, key_at, a, row, scale, p, mass);
 }
 
