@@ -29,7 +29,7 @@ constexpr uint32_t kKeyOfNan = 0xffffffffu, kLeast = 0x00800000u, kNothing = 0; 
 __device__ inline uint32_t key_or_nan(float x) { return x != x ? kKeyOfNan : key_of(x); }
 
 // 2^(x + 42) as an integer, x <= 0: 2^n r, r by the exponential series of the fraction of x, at most 1/2 of either sign: its twelve terms leave 2e-14 out.
-__device__ inline mass_t power_as_integer(double x) {
+__device__ __forceinline__ mass_t power_as_integer(double x) {
   if (!(x >= -kFraction - 1)) return 0;
   const double n = __builtin_rint(x), f = (x - n) * 0.693147180559945309417;
   double r = 1. / 39916800;
@@ -53,9 +53,9 @@ struct Scale {
   uint32_t largest;  // its key
   float top;         // its value
   double rate;       // log2 e / temperature
-  __device__ Scale(uint32_t key, float temperature) : largest(key), top(value_of(key)), rate(1.44269504088896340736 / (double)temperature) {}
-  __device__ double distance(float logit) const { return logit == top ? 0. : ((double)logit - (double)top) * rate; }
-  __device__ mass_t weight(uint32_t key) const { return key == largest ? (mass_t)1 << kFraction : power_as_integer(distance(value_of(key))); }
+  __device__ __forceinline__ Scale(uint32_t key, float temperature) : largest(key), top(value_of(key)), rate(1.44269504088896340736 / (double)temperature) {}
+  __device__ __forceinline__ double distance(float logit) const { return logit == top ? 0. : ((double)logit - (double)top) * rate; }
+  __device__ __forceinline__ mass_t weight(uint32_t key) const { return key == largest ? (mass_t)1 << kFraction : power_as_integer(distance(value_of(key))); }
 };
 
 struct Parameters {
@@ -115,6 +115,26 @@ __device__ inline mass_t wave_most(mass_t x) {
   return of_lane(larger(x, moved<0x143, 0xc>(x)), 63);
 }
 
+// f of each of four, or eight, keys: once in the code, which is fetched anew by every launch's workgroups and costs them more than the moves
+template <class F>
+__device__ __forceinline__ void each_of(u4_t four, F f) {
+#pragma unroll 1
+  for (int e = 0; e < 4; ++e) {
+    f(four.x);
+    four = u4_t{four.y, four.z, four.w, four.x};
+  }
+}
+template <class F>
+__device__ __forceinline__ void each_of(u4_t one, u4_t other, F f) {
+#pragma unroll 1
+  for (int e = 0; e < 8; ++e) {
+    f(one.x);
+    const uint32_t first = one.x;
+    one = u4_t{one.y, one.z, one.w, other.x};
+    other = u4_t{other.y, other.z, other.w, first};
+  }
+}
+
 // What stays of a row: keys above `key` and the first `ties` of those equal to it
 struct Kept {
   uint32_t key;
@@ -124,7 +144,8 @@ struct Kept {
 template <int THREADS>
 struct Shared {
   mass_t bins[kBins];
-  uint32_t keys[kListed], indices[kListed];  // candidates in the order of their indices
+  __attribute__((aligned(16))) uint32_t keys[kListed + 4];
+  uint32_t indices[kListed + 4];  // candidates in the order of their indices
   uint32_t reaching[kGroups / 2];            // groups that reach the candidates' value, 16 bits each
   mass_t parts[2][THREADS / 64];
   mass_t above;
@@ -158,17 +179,18 @@ struct Block {
   }
 
   // The key, from `high` down to `low`, with which the running sum of the items' amounts comes to `target` or more, the sum in front of it, and whether it comes to it. each(f) calls
-  // f(key, amount) for the thread's items. In each round the bin of 2^shift keys in which that happens.
-  template <class Each>
-  __device__ bool search(uint32_t high, uint32_t low, mass_t target, Each each, uint32_t& key, mass_t& in_front) {
+  // f(key) for the thread's items; of key `extra` there is extra_amount once. In each round the bin of 2^shift keys in which that happens.
+  template <class Each, class Amount>
+  __device__ __forceinline__ bool search(uint32_t high, uint32_t low, mass_t target, Each each, Amount amount, uint32_t extra, mass_t extra_amount, uint32_t& key, mass_t& in_front) {
     mass_t above = 0;
     for (;;) {
       const int shift = max(0, 32 - __clz((int)(high - low)) - 11);
       for (int i = threadIdx.x; i < kBins; i += THREADS) s.bins[i] = 0;
       __syncthreads();
-      each([&](uint32_t own, mass_t amount) {
-        if (own <= high && own >= low) atomicAdd(&s.bins[(high - own) >> shift], amount);
+      each([&](uint32_t own) {
+        if (own <= high && own >= low) atomicAdd(&s.bins[(high - own) >> shift], amount(own));
       });
+      if (threadIdx.x == 0 && extra_amount && extra <= high && extra >= low) atomicAdd(&s.bins[(high - extra) >> shift], extra_amount);
       __syncthreads();
       constexpr int kEach = kBins / THREADS;
       mass_t own[kEach], sum = 0, total;
@@ -195,29 +217,27 @@ struct Block {
 
 // The filters by rank and by share. each(f) calls f(key) for the thread's items, all of them from key `low` on, in any order; mass: the row's, where it counts.
 template <int THREADS, class Each>
-__device__ Kept filtered(Block<THREADS>& block, const Scale& scale, const Parameters& p, uint32_t low, double mass, Each each) {
+__device__ __forceinline__ Kept filtered(Block<THREADS>& block, const Scale& scale, const Parameters& p, uint32_t low, double mass, Each each) {
   Kept kept = {kNothing, kAll};
   uint32_t key;
   mass_t in_front;
-  if (p.top_k != kAll && block.search(scale.largest, low, p.top_k, [&](auto add) { each([&](uint32_t own) { add(own, (mass_t)1); }); }, key, in_front))
-    kept = {key, p.top_k - (int)in_front};
+  if (p.top_k != kAll && block.search(scale.largest, low, p.top_k, each, [](uint32_t) { return (mass_t)1; }, 0, 0, key, in_front)) kept = {key, p.top_k - (int)in_front};
   if (p.top_p < 1.f) {
     const mass_t tied = kept.ties == kAll ? 0 : scale.weight(kept.key) * kept.ties;
-    auto masses = [&](auto add) {
+    auto above = [&](auto f) {
       each([&](uint32_t own) {
-        if (own > kept.key || kept.ties == kAll) add(own, scale.weight(own));
+        if (own > kept.key || kept.ties == kAll) f(own);
       });
-      if (threadIdx.x == 0 && tied) add(kept.key, tied);
     };
     if (p.top_k != kAll) {  // of those that top_k left
-      mass_t own_mass = 0, total;
-      masses([&](uint32_t, mass_t amount) { own_mass += amount; });
+      mass_t own_mass = threadIdx.x == 0 ? tied : 0, total;
+      above([&](uint32_t own) { own_mass += own >= low ? scale.weight(own) : 0; });
       block.before(own_mass, total);
       mass = (double)total;
     }
     // (where rounding leaves the running sum below: all stay)
     const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
-    if (block.search(scale.largest, max(low, kept.key), target, masses, key, in_front)) {
+    if (block.search(scale.largest, max(low, kept.key), target, above, [&](uint32_t own) { return scale.weight(own); }, kept.key, tied, key, in_front)) {
       const mass_t one = scale.weight(key);
       kept = {key, (int)((target - in_front + one - 1) / one)};
     }
@@ -229,61 +249,98 @@ __device__ Kept filtered(Block<THREADS>& block, const Scale& scale, const Parame
 struct Last {
   const Scale& scale;
   double least;
-  __device__ Last(const Scale& s, const Parameters& p) : scale(s), least(p.min_p > 0.f ? log2((double)p.min_p) : -__builtin_inf()) {}
-  __device__ mass_t weight(uint32_t key) const { return scale.distance(value_of(key)) >= least ? scale.weight(key) : 0; }
+  __device__ __forceinline__ Last(const Scale& s, const Parameters& p) : scale(s), least(p.min_p > 0.f ? log2((double)p.min_p) : -__builtin_inf()) {}
+  __device__ __forceinline__ mass_t weight(uint32_t key) const { return scale.distance(value_of(key)) >= least ? scale.weight(key) : 0; }
 };
 __device__ inline mass_t target_of(float uniform, double total, mass_t whole) {
   const double at = uniform > 0.f ? (double)uniform * total : 0.;
   return at < total ? min((mass_t)at, whole - 1) : whole - 1;
 }
 
-// Items 0 ... count - 1, which get(i) gives as key and index, in the order of their indices. Of those that `kept` leaves, the first at which the running mass exceeds `at`,
-// or uniform times the total where `at` is negative. A wavefront has a stretch of the items, 64 of them at a time.
-template <int THREADS, class Get>
-__device__ void choose(Block<THREADS>& block, const Last& last, const Kept& kept, float uniform, double at, int count, Get get, long long* token) {
-  const int stretch = (count + THREADS - 1) / THREADS * 64, begin = min(block.wave * stretch, count), end = min(begin + stretch, count), lane = block.lane;
+// Items in fours: keys(i) gives those of items 4 i ... 4 i + 3, i < count, in the order of their indices, index(item) an item's. Of those that `kept` leaves, the first at which
+// the running mass exceeds `at`, or uniform times the total where `at` is negative. Each wavefront sums a stretch, 64 fours at a time; the stretch in which it happens is
+// shared out again until one wavefront walks through it.
+template <int THREADS, class Keys, class Index>
+__device__ __forceinline__ void choose(Block<THREADS>& block, const Last& last, const Kept& kept, float uniform, double at, int count, Keys keys, Index index, long long* token) {
   const bool bounded = kept.ties != kAll;
   const mass_t each = bounded ? last.weight(kept.key) : 0;
-  mass_t ties = 0, mass = 0, ignored, total;
-  for (int i = begin + lane; i < end; i += 64) {
-    const uint32_t key = get(i).x;
-    if (bounded && key == kept.key) ++ties;
-    else if (key >= kept.key) mass += last.weight(key);
+  const int lane = block.lane;
+  int first = 0;
+  mass_t front = 0, left = bounded ? (mass_t)kept.ties : 0, target = 0;  // in front of the items, ties that they may keep
+  for (bool whole = true;; whole = false) {
+    const int stretch = (count + THREADS - 1) / THREADS * 64, begin = first + min(block.wave * stretch, count), end = min(begin + stretch, first + count);
+    mass_t ties = 0, mass = 0, total;
+    constexpr u4_t kNone = {kNothing, kNothing, kNothing, kNothing};
+    for (int i = begin + lane; i < end; i += 128) {
+      const u4_t one = keys(i), other = i + 64 < end ? keys(i + 64) : kNone;
+      each_of(one, other, [&](uint32_t key) {
+        const bool tie = bounded && key == kept.key;
+        ties += tie;
+        mass += key >= kept.key && key >= kLeast && !tie ? last.weight(key) : 0;
+      });
+    }
+    mass_t in_front = 0;  // ties in front of the wavefront's
+    if (each) {
+      mass_t ignored;
+      in_front = of_lane(block.before(ties, ignored), 0);
+      const mass_t of_wave = of_lane(wave_running(ties), 63), may = left > in_front ? left - in_front : 0;
+      if (lane == 0) mass += min(may, of_wave) * each;
+    }
+    const mass_t running = front + of_lane(block.before(mass, total), 0), of_wave = of_lane(wave_running(mass), 63);
+    if (whole) target = at < 0. ? target_of(uniform, (double)total, total) : min((mass_t)at, total - 1);
+    const bool here = running <= target && running + of_wave > target;
+    left = left > in_front ? left - in_front : 0;
+    if (stretch <= 64 * 4) {
+      if (!here) return;
+      first = begin, count = end - begin, front = running;
+      break;
+    }
+    if (here && lane == 0) block.s.bins[0] = (mass_t)begin, block.s.bins[1] = (mass_t)end, block.s.bins[2] = running, block.s.bins[3] = left;
+    __syncthreads();
+    first = (int)block.s.bins[0], count = (int)block.s.bins[1] - first, front = block.s.bins[2], left = block.s.bins[3];
+    __syncthreads();
   }
-  mass_t left = 0;  // ties that the wavefront's stretch may keep
-  if (each) {
-    const mass_t in_front = block.before(ties, ignored), of_wave = of_lane(wave_running(ties), 63);
-    const mass_t wave_front = of_lane(in_front, 0);
-    left = (mass_t)kept.ties > wave_front ? (mass_t)kept.ties - wave_front : 0;
-    if (lane == 0) mass += min(left, of_wave) * each;
-  }
-  const mass_t running = block.before(mass, total), of_wave = of_lane(wave_running(mass), 63);
-  const mass_t target = at < 0. ? target_of(uniform, (double)total, total) : min((mass_t)at, total - 1);
-  mass_t front = of_lane(running, 0);
-  if (front > target || front + of_wave <= target) return;
-  for (int i = begin; i < end; i += 64) {
-    const bool there = i + lane < end;
-    const u2_t item = there ? get(i + lane) : u2_t{kNothing, 0};
-    const bool tie = there && bounded && item.x == kept.key;
-    const mass_t tied = __ballot(tie);
-    mass_t w = 0;
-    if (tie) w = (mass_t)__popcll(tied & (((mass_t)1 << lane) - 1)) < left ? each : 0;
-    else if (there && item.x >= kept.key) w = last.weight(item.x);
-    const mass_t sum = front + wave_running(w), over = __ballot(sum > target);
+  for (int i = first; i < first + count; i += 64) {
+    u4_t four = {kNothing, kNothing, kNothing, kNothing};
+    if (i + lane < first + count) four = keys(i + lane);
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ties += bounded && four[e] == kept.key;
+    const int ties_running = wave_running(ties);
+    mass_t may = (mass_t)(ties_running - ties);
+    may = left > may ? left - may : 0;
+    mass_t own = 0;
+    auto weigh = [&](uint32_t key, mass_t& may) -> mass_t {
+      if (bounded && key == kept.key) {
+        const mass_t w = may ? each : 0;
+        may -= may ? 1 : 0;
+        return w;
+      }
+      return key >= kept.key && key >= kLeast ? last.weight(key) : 0;
+    };
+    const mass_t may_at_first = may;
+    each_of(four, [&](uint32_t key) { own += weigh(key, may); });
+    const mass_t running = wave_running(own), over = __ballot(front + running > target);
     if (over) {
-      const int found = __builtin_ctzll(over);
-      if (lane == found) *token = item.y;
+      if (lane == __builtin_ctzll(over)) {
+        mass_t sum = front + running - own;
+        int found = 0;
+        may = may_at_first;
+        each_of(four, [&](uint32_t key) { found += (sum += weigh(key, may)) <= target; });
+        *token = index(4 * (i + lane) + found);
+      }
       return;
     }
-    front = of_lane(sum, 63);
-    left -= min(left, (mass_t)__popcll(tied));
+    front += of_lane(running, 63);
+    const mass_t all = (mass_t)of_lane(ties_running, 63);
+    left = left > all ? left - all : 0;
   }
 }
 
 // Few candidates: each is compared with each other, wavefronts taking every so manieth of them: how many are in front of it, and their mass
 constexpr int kPaired = 256;
 template <int THREADS>
-__device__ void choose_of_few(Block<THREADS>& block, const Scale& scale, const Last& last, const Parameters& p, double mass, float uniform, int count, long long* token) {
+__device__ __forceinline__ void choose_of_few(Block<THREADS>& block, const Scale& scale, const Last& last, const Parameters& p, double mass, float uniform, int count, long long* token) {
   Shared<THREADS>& s = block.s;
   mass_t *const weights = s.bins, *const fronts = s.bins + kPaired, *const ranks = s.bins + 2 * kPaired;
   const int own = threadIdx.x;
@@ -318,9 +375,9 @@ __device__ void choose_of_few(Block<THREADS>& block, const Scale& scale, const L
   if (front <= target && front + w > target) *token = s.indices[own];
 }
 
-// The row's groups of `group` logits: the thread's are kCount from number `first` on, their largest keys as given; key(i): of logit i.
+// The row's groups of `group` logits: the thread's are kCount from number `first` on, their largest keys as given; four_at(i): the keys of logits i ... i + 3, i a multiple of four.
 template <int THREADS, int kCount, class Key>
-__device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount], int first, int group, Key key_at, const onebit_sampling& a, int row, const Scale& scale,
+__device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount], int first, int group, Key four_at, const onebit_sampling& a, int row, const Scale& scale,
                            const Parameters& p, double mass) {
   Shared<THREADS>& s = block.s;
   // A value that all candidates reach. Weights 2^-50 of the largest are 0: no such logit matters, whatever its rank.
@@ -329,30 +386,49 @@ __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount]
 #pragma unroll
   for (int i = 0; i < kCount; ++i) distance[i] = most[i] >= kLeast ? most[i] == scale.largest ? 0.f : (scale.top - value_of(most[i])) * steep : INFINITY;
   if (p.top_k != kAll || p.top_p < 1.f) {
-    // The groups' largest within `reach` are top_k, or have top_p of the mass: found by quarters, five times. In fp32, and therefore with some room.
+    // The groups' largest within `reach` are top_k, or have top_p of the mass: found by quarters, five times. In fp32, and therefore with some room. First with the
+    // threads' largest alone; where they do not come to it, with all.
     const bool by_rank = p.top_k != kAll;
     const float target = by_rank ? (float)p.top_k : (float)((double)p.top_p * mass * 0x1p-42) * (1.f + 0x1p-10f);
-    float amount[kCount], low = 0.f;
+    constexpr int kWaves = Block<THREADS>::kWaves;
+    auto quarters = [&](auto number, const auto& distance) __attribute__((always_inline)) {
+      constexpr int kNumber = decltype(number)::value;
+      float amount[kNumber], low = 0.f;
+      bool enough = false;
+      reach = kFarthest;
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) amount[i] = by_rank ? 1.f : __builtin_amdgcn_exp2f(-distance[i]);
-    for (int round = 0; round < 5; ++round) {
-      const float step = (reach - low) * 0.25f;
-      float sum[3] = {};
+      for (int i = 0; i < kNumber; ++i) amount[i] = by_rank ? 1.f : __builtin_amdgcn_exp2f(-distance[i]);
+#pragma unroll 1
+      for (int round = 0; round < 5; ++round) {
+        const float step = (reach - low) * 0.25f;
+        f4_t sum = {};
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
+        for (int q = 0; q < 4; ++q)
+          if (q < 3 || round == 0) {
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) sum[q] += distance[i] <= low + (q + 1) * step ? amount[i] : 0.f;
-        sum[q] = wave_sum(sum[q]);
+            for (int i = 0; i < kNumber; ++i) sum[q] += distance[i] <= low + (q + 1) * step ? amount[i] : 0.f;
+            sum[q] = of_lane(wave_running(sum[q]), 63);
+          }
+        float* const parts = (float*)s.bins + (round & 1) * 4 * kWaves;
+        if (block.lane == 0) *(f4_t*)(parts + 4 * block.wave) = sum;
+        __syncthreads();
+        const f4_t all = *(const f4_t*)(parts + 4 * (block.lane % kWaves));
+        int within = 0;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) within += of_lane(row_running(all[q]), kWaves - 1) < target;
+        if (round == 0) enough = of_lane(row_running(all[3]), kWaves - 1) >= target;
+        if (!enough) return false;
+        if (within < 3) reach = low + (within + 1) * step;
+        low += within * step;
       }
-      float* const parts = (float*)s.bins + (round & 1) * 4 * Block<THREADS>::kWaves;
-      if (block.lane == 0) *(f4_t*)(parts + 4 * block.wave) = f4_t{sum[0], sum[1], sum[2], 0.f};
-      __syncthreads();
-      f4_t all = *(const f4_t*)(parts + 4 * (block.lane % Block<THREADS>::kWaves));
-      int within = 0;
+      return true;
+    };
+    float nearest[1] = {distance[0]};
 #pragma unroll
-      for (int q = 0; q < 3; ++q) within += of_lane(row_running(all[q]), Block<THREADS>::kWaves - 1) < target;
-      if (within < 3) reach = low + (within + 1) * step;
-      low += within * step;
+    for (int i = 1; i < kCount; ++i) nearest[0] = fminf(nearest[0], distance[i]);
+    if (!quarters(std::integral_constant<int, 1>(), nearest)) {
+      __syncthreads();  // the sums' readers are through
+      if (kCount > 1 && !quarters(std::integral_constant<int, kCount>(), distance)) reach = kFarthest;
     }
   }
   // (a step further than fp32 rounds)
@@ -378,45 +454,46 @@ __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount]
 #pragma unroll
   for (int i = 0; i < kCount; ++i)
     if (most[i] >= low) reaching[at++] = (uint16_t)(first + i);
-  const int items = reaching_groups * group, shift = __builtin_ctz(group);  // (at most the vocabulary, rounded up)
+  const int fours = reaching_groups * group / 4, shift = __builtin_ctz(group) - 2;  // (at most the vocabulary, rounded up)
   __syncthreads();
-  auto item = [&](int i) {
-    const int index = (int)reaching[i >> shift] * group + (i & (group - 1));
-    return u2_t{index < a.vocabulary ? key_at(index) : kNothing, (uint32_t)index};
-  };
+  auto index_of_four = [&](int i) { return (int)reaching[i >> shift] * group + (i & (group / 4 - 1)) * 4; };
+  auto four = [&](int i) { return four_at(index_of_four(i)); };
   // their logits that reach it, listed in order where they are few
   int listed = 0;
-  constexpr int kBatch = 8;
-  int* const counts = (int*)s.bins;  // of a batch: of each part of it, wavefront by wavefront
-  for (int i = 0; i < items && listed <= kListed; i += kBatch * THREADS) {
-    u2_t one[kBatch];
-    mass_t candidates[kBatch];
+  constexpr int kBatch = 2;
+  for (int i = 0; i < fours && listed <= kListed; i += kBatch * THREADS) {
+    u4_t one[kBatch];
+    int own[kBatch], in_front[kBatch], all[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      one[j] = {kNothing, 0};
-      if (i + j * THREADS + (int)threadIdx.x < items) one[j] = item(i + j * THREADS + threadIdx.x);
+      const int at = i + j * THREADS + threadIdx.x;
+      one[j] = at < fours ? four(at) : u4_t{kNothing, kNothing, kNothing, kNothing};
     }
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      candidates[j] = __ballot(one[j].x >= low);
-      if (block.lane == 0) counts[j * Block<THREADS>::kWaves + block.wave] = __popcll(candidates[j]);
-    }
-    __syncthreads();
-    int running[2];  // lane l: of entries 2 l and 2 l + 1
-    constexpr int kEntries = kBatch * Block<THREADS>::kWaves;
-    static_assert(kEntries <= 128, "");
+      own[j] = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) running[e] = 2 * block.lane + e < kEntries ? counts[2 * block.lane + e] : 0;
-    const int pairs = wave_running(running[0] + running[1]), front = pairs - running[0] - running[1];
+      for (int e = 0; e < 4; ++e) own[j] += one[j][e] >= low;
+    }
+    // (both at once, 16 bits each)
+    const int both = block.before(own[0] | own[1] << 16, all[0]);
+    in_front[0] = both & 0xffff, in_front[1] = both >> 16, all[1] = all[0] >> 16, all[0] &= 0xffff;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int entry = j * Block<THREADS>::kWaves + block.wave;
-      const int to = listed + of_lane(front, entry / 2) + (entry & 1 ? of_lane(running[0], entry / 2) : 0) + __popcll(candidates[j] & (((mass_t)1 << block.lane) - 1));
-      if (one[j].x >= low && to < kListed) s.keys[to] = one[j].x, s.indices[to] = one[j].y;
+      int to = listed + in_front[j];
+      if (own[j]) {
+        const int index = index_of_four(i + j * THREADS + threadIdx.x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (one[j][e] >= low) {
+            if (to < kListed) s.keys[to] = one[j][e], s.indices[to] = index + e;
+            ++to;
+          }
+      }
+      listed += all[j];
     }
-    listed += of_lane(pairs, 63);
   }
+  if (threadIdx.x < 4 && listed <= kListed) s.keys[listed + threadIdx.x] = kNothing;
   __syncthreads();
   if (listed <= kPaired) {
     choose_of_few(block, scale, last, p, mass, uniform, listed, token);
@@ -424,17 +501,21 @@ __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount]
     const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
       for (int i = threadIdx.x; i < listed; i += THREADS) f(s.keys[i]);
     });
-    choose(block, last, kept, uniform, -1., listed, [&](int i) { return u2_t{s.keys[i], s.indices[i]}; }, token);
+    choose(block, last, kept, uniform, -1., (listed + 3) / 4, [&](int i) { return *(const u4_t*)(s.keys + 4 * i); }, [&](int i) { return (long long)s.indices[i]; }, token);
   } else {
     auto reached = [&](int i) {
-      u2_t one = item(i);
-      if (one.x < low) one.x = kNothing;
+      u4_t one = four(i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) one[e] = one[e] >= low ? one[e] : kNothing;
       return one;
     };
     const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
-      for (int i = threadIdx.x; i < items; i += THREADS) f(reached(i).x);
+      for (int i = threadIdx.x; i < fours; i += 2 * THREADS) {
+        const u4_t one = reached(i), other = i + THREADS < fours ? reached(i + THREADS) : u4_t{kNothing, kNothing, kNothing, kNothing};
+        each_of(one, other, f);
+      }
     });
-    choose(block, last, kept, uniform, -1., items, reached, token);
+    choose(block, last, kept, uniform, -1., fours, reached, [&](int i) { return (long long)index_of_four(i / 4) + i % 4; }, token);
   }
 }
 
@@ -442,7 +523,7 @@ __device__ void sample_row(Block<THREADS>& block, const uint32_t (&most)[kCount]
 template <int TYPE, int N>
 __device__ inline void load_keys(const void* logits, long long base, int at, int vocabulary, uint32_t (&keys)[N]) {
   typedef typename Stored<TYPE>::type T;
-  constexpr int kOf16 = 16 / sizeof(T);
+  constexpr int kOf16 = N < 16 / (int)sizeof(T) ? N : 16 / (int)sizeof(T);
   typedef T vector __attribute__((ext_vector_type(kOf16), aligned(sizeof(T))));  // (16 bytes from any address)
   const T* const from = (const T*)logits + base + at;
   if (at + N <= vocabulary) {
@@ -506,10 +587,12 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(onebit_sampling a
   best = block.most(best);  // (with a barrier: the keys are there)
   if (settled(best, p, a.tokens + row)) return;
   const Scale scale((uint32_t)(best >> 32), p.temperature);
+  auto four_at = [&](int i) { return *(const u4_t*)(row_keys + i); };
   double mass = 0.;
   if (p.masses) {
+    auto four_at_place = [&](int i) { return four_at(4 * i); };
     if (p.top_p >= 1.f) {  // no filter
-      choose(block, Last(scale, p), {kNothing, kAll}, a.uniform[row], -1., a.vocabulary, [&](int i) { return u2_t{row_keys[i], (uint32_t)i}; }, a.tokens + row);
+      choose(block, Last(scale, p), {kNothing, kAll}, a.uniform[row], -1., (a.vocabulary + 3) / 4, four_at_place, [](int i) { return (long long)i; }, a.tokens + row);
       return;
     }
     mass_t own = 0, total;
@@ -517,7 +600,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(onebit_sampling a
     block.before(own, total);
     mass = (double)total;
   }
-  sample_row(block, most, threadIdx.x * kCount, kGroup, [&](int i) { return row_keys[i]; }, a, row, scale, p, mass);
+  sample_row(block, most, threadIdx.x * kCount, kGroup, four_at, a, row, scale, p, mass);
 }
 
 // Long rows, first pass: a chunk's largest, its mass beside that where masses count, and its groups' largest
@@ -549,7 +632,9 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(onebit_sampling a,
   if (p.masses && key >= kLeast && key != kKeyOfNan) {
     const Scale scale(key, p.temperature);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) mass += keys[i] >= kLeast ? scale.weight(keys[i]) : 0;
+    for (int i = 0; i < kGroup; i += 8)
+      each_of(u4_t{keys[i], keys[i + 1], keys[i + 2], keys[i + 3]}, u4_t{keys[i + 4], keys[i + 5], keys[i + 6], keys[i + 7]},
+              [&](uint32_t key) { mass += key >= kLeast ? scale.weight(key) : 0; });
     mass = of_lane(wave_running(mass), 63);
     if (lane == 0) parts[1][wave] = mass;
     __syncthreads();
@@ -574,10 +659,10 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
   const mass_t best = block.most(own_best);
   if (settled(best, p, a.tokens + row)) return;
   const Scale scale((uint32_t)(best >> 32), p.temperature);
-  auto key_at = [&](int i) {
-    float x[1];
-    load_values<TYPE, 1>(a.logits, row * a.logits_stride + i, x);
-    return key_of(x[0]);
+  auto four_at = [&](int i) {
+    uint32_t keys[4];
+    load_keys<TYPE, 4>(a.logits, row * a.logits_stride, i, a.vocabulary, keys);
+    return u4_t{keys[0], keys[1], keys[2], keys[3]};
   };
   double mass = 0.;
   if (p.masses) {
@@ -613,7 +698,7 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
         return;
       }
       if (rest < 0.) rest = 0x1p62;
-      choose(block, Last(scale, p), {kNothing, kAll}, uniform, rest, count, [&](int i) { return u2_t{key_at(begin + i), (uint32_t)(begin + i)}; }, a.tokens + row);
+      choose(block, Last(scale, p), {kNothing, kAll}, uniform, rest, (count + 3) / 4, [&](int i) { return four_at(begin + 4 * i); }, [&](int i) { return (long long)(begin + i); }, a.tokens + row);
       return;
     }
     __syncthreads();  // the sums' readers are through
@@ -637,7 +722,7 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
     for (int i = 0; i < kCount; ++i)
       if (i < share && first + i < c.groups) most[i] = largest[first + i];
   }
-  sample_row(block, most, first, c.group, key_at, a, row, scale, p, mass);
+  sample_row(block, most, first, c.group, four_at, a, row, scale, p, mass);
 }
 
 constexpr int kShort = 8192;
