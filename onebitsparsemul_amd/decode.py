@@ -1,17 +1,18 @@
-"""A small decoder of one-bit projections with random weights: norms, rotation, 8-bit cache and attention as a serving program
-calls them.
+"""A small decoder of one-bit projections with random weights: norms, rotation, 8-bit cache and attention, and the way to the next
+tokens, as a serving program calls them.
 
     python -m onebitsparsemul_amd.decode [--layers 2] [--hidden 512] [--sequences 16] [--prompt 512] [--tokens 64]
+    python -m onebitsparsemul_amd.decode --head e4m3 [--temperature 0.8] [--top-k 50] [--top-p 0.95] [--min-p 0.0]
 
 A prompt goes into the caches in one pass, tokens are decoded one by one behind it, and the logits are compared with those of one
-pass over everything.
+pass over everything. With --head e4m3 the projection onto the vocabulary is in 8 bits, and each token is drawn from the logits in front of it.
 """
 import argparse
 import time
 
 import torch
 
-from . import BinaryLinear_2_4, QuantizedCache, block_norm, forward_grouped, rotary_table
+from . import BinaryLinear_2_4, BlockLinear, QuantizedCache, block_norm, block_norm_codes, forward_grouped, rotary_table, sample
 
 
 class DecoderLayer(torch.nn.Module):
@@ -51,12 +52,16 @@ class Decoder:
     """A few layers with their caches, for the sequences of one batch: pages are handed out as the sequences grow."""
 
     def __init__(self, layers, sequences, length, hidden=512, intermediate=1408, heads=8, kv_heads=4, head_dim=64, vocabulary=4096, block=64,
-                 dtype=torch.float8_e4m3fn, seed=0, device="cuda"):
+                 dtype=torch.float8_e4m3fn, seed=0, device="cuda", head=None):
+        """head: None, the logits from the embedding in 32 bits; "e4m3": from its 8-bit codes, with the last norm's output in such codes."""
+        if head not in (None, "e4m3"):
+            raise ValueError(f"head must be None or 'e4m3', got {head!r}")
         generator = torch.Generator(device=device)
         generator.manual_seed(seed)
         self.layers = [DecoderLayer(hidden, intermediate, heads, kv_heads, head_dim, generator, device) for _ in range(layers)]
         self.embedding = torch.randn((vocabulary, hidden), generator=generator, device=device).half()
         self.norm = torch.ones(hidden, dtype=torch.float16, device=device)
+        self.head = BlockLinear(self.embedding, out_dtype=torch.float32) if head else None
         width = -(-length // block)
         self.caches = [QuantizedCache(sequences * width, kv_heads, head_dim, block=block, dtype=dtype, device=device) for _ in range(layers)]
         # sequence s owns pages s, s + sequences, ...: nothing is to be gained from neighbouring pages
@@ -73,8 +78,23 @@ class Decoder:
         x, residual = None, self.embedding[tokens]
         for layer, cache in zip(self.layers, self.caches):
             x, residual = layer(x, residual, cache, self.pages, self.lengths, None, self.table, new, longest)
+        if self.head is not None:  # the last tokens' rows alone
+            x, residual = (t if t is None else t.view(sequences, new, -1)[:, -1] for t in (x, residual))
+            return self.head(block_norm_codes(x, residual, self.norm)[1:])
         _, h = block_norm(x, residual, self.norm)
         return h.view(sequences, new, -1)[:, -1].float() @ self.embedding.float().T
+
+    @torch.no_grad()
+    def generate(self, prompt, uniform, **options):
+        """prompt (sequences, length): ids; uniform (tokens, sequences): a random number in [0, 1) for each token and sequence; options: sample's. Returns the ids of
+        the tokens behind the prompt, (sequences, tokens); the caches hold the prompt and all but the last of them."""
+        count, new = uniform.shape[0], prompt.shape[1]
+        ids, tokens = prompt.reshape(-1), []
+        longest = int(self.lengths.max()) + new if count else 0
+        for step in range(count):
+            tokens.append(sample(self.step(ids, new, longest), uniform[step], **options))
+            ids, new, longest = tokens[-1], 1, longest + 1
+        return torch.stack(tokens, dim=1) if tokens else prompt.new_empty((prompt.shape[0], 0))
 
 
 def main(argv=None):
@@ -85,11 +105,16 @@ def main(argv=None):
     ap.add_argument("--sequences", type=int, default=16)
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--tokens", type=int, default=64, help="decoded behind the prompt")
+    ap.add_argument("--head", choices=["e4m3"], default=None, help="logits from 8-bit codes, and tokens drawn from them")
+    ap.add_argument("--temperature", type=float, default=0.8)
+    ap.add_argument("--top-k", type=int, default=50)
+    ap.add_argument("--top-p", type=float, default=0.95)
+    ap.add_argument("--min-p", type=float, default=0.0)
     args = ap.parse_args(argv)
     heads = max(1, args.hidden // 64)
     sizes = dict(hidden=args.hidden, intermediate=args.intermediate, heads=heads, kv_heads=max(1, heads // 2))
     total = args.prompt + args.tokens
-    stepwise, whole = (Decoder(args.layers, args.sequences, total, **sizes) for _ in range(2))
+    stepwise, whole = (Decoder(args.layers, args.sequences, total, head=args.head, **sizes) for _ in range(2))
     ids = torch.randint(0, 4096, (args.sequences, total), device="cuda")
     for warm in (True, False):
         stepwise.lengths.zero_()
@@ -108,6 +133,17 @@ def main(argv=None):
     print(f"{args.layers} layers, {args.sequences} sequences: {args.tokens} tokens behind a prompt of {args.prompt}: {seconds / args.tokens * 1e6:.0f} us a step; "
           f"all {total} in one pass: {prompt_seconds * 1e3:.2f} ms")
     print(f"logits behind the last token, step by step against the one pass: {off:.4f} apart (the caches' pages are rounded again as they grow)")
+    if args.head:
+        uniform = torch.rand((args.tokens, args.sequences), device="cuda")
+        options = dict(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
+        for _ in range(2):
+            stepwise.lengths.zero_()
+            torch.cuda.synchronize()
+            begin = time.perf_counter()
+            drawn = stepwise.generate(ids[:, :args.prompt], uniform, **options)
+            torch.cuda.synchronize()
+            seconds = time.perf_counter() - begin
+        print(f"{args.tokens} tokens drawn behind the prompt: {seconds * 1e3:.2f} ms with the prompt's pass; the first sequence's: {drawn[0, :12].tolist()}")
     return off
 
 

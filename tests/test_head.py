@@ -487,3 +487,65 @@ def test_two_streams_at_once():
     for i, results in enumerate(got):
         for result in results:
             assert all(same(a, b) for a, b in zip(result, want[i]))
+
+
+def test_a_decoder_answers_with_tokens():
+    """Norm, codes, product and sampling behind two layers of one-bit projections, as decode.py runs them: the logits are those of the plain forms from the same rows, tokens those that
+    their logits give, and a decoder that is given the drawn tokens in one pass comes to the same caches' lengths"""
+    from onebitsparsemul_amd.decode import Decoder
+    g = generator(3)
+    prompt = torch.randint(0, 4096, (5, 48), generator=g).cuda()
+    uniform = torch.rand((9, 5), generator=g).cuda()
+    options = dict(temperature=0.9, top_k=40, top_p=0.9, min_p=0.01)
+    decoder, again, plain = Decoder(2, 5, 64, block=16, head="e4m3"), Decoder(2, 5, 64, block=16, head="e4m3"), Decoder(2, 5, 64, block=16)
+    tokens = decoder.generate(prompt, uniform, **options)
+    assert tokens.shape == (5, 9) and bool((decoder.lengths == 48 + 8).all()) and bool(((tokens >= 0) & (tokens < 4096)).all())
+    ids, new = prompt.reshape(-1), 48
+    for step in range(9):
+        logits = again.step(ids, new, 48 + step)
+        assert logits.dtype == torch.float32 and tokens[:, step].tolist() == plain_tokens(logits, uniform[step], **options)
+        ids, new = tokens[:, step], 1
+    # codes of both sides are off by 2^-4 at most, their products' errors of mixed signs: far within 2^-4 of the logits' norm
+    first, want = Decoder(2, 5, 64, block=16, head="e4m3").step(prompt.reshape(-1), 48, 48), plain.step(prompt.reshape(-1), 48, 48)
+    assert float((first - want).norm() / want.norm()) < 2.0**-4
+    assert Decoder(1, 2, 64, head="e4m3").generate(prompt[:2], uniform[:0]).shape == (2, 0)
+    with pytest.raises(ValueError, match="head must be"):
+        Decoder(1, 2, 64, head="int8")
+
+
+def test_the_command_draws_tokens(capsys):
+    from onebitsparsemul_amd import decode
+    decode.main(["--layers", "1", "--sequences", "3", "--prompt", "33", "--tokens", "4", "--head", "e4m3"])
+    assert "4 tokens drawn behind the prompt" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("count", [1, 17])
+def test_two_graphs_of_one_call_keep_apart(count):
+    """Two captured calls with a workspace each, replayed in turn and together with an eager one"""
+    g = generator(count)
+    (x, xs), (w, ws) = random_codes(64, 8192, g), random_codes(100, 8192, g, 128)  # groups split over workgroups
+    x, xs, w, ws = x.cuda(), xs.cuda(), w.cuda(), ws.cuda()
+    logits, u = random_logits(count, 40000, g, torch.float16).cuda(), torch.rand(count, generator=g).cuda()
+    inputs = [(x, logits), (x.flip(0).contiguous(), logits.flip(1).contiguous())]
+
+    def call(codes, row):
+        return onebit.block_linear(codes, xs, w, ws), onebit.sample(row, u, top_p=0.9)
+
+    want = [call(*i) for i in inputs]
+    stream = torch.cuda.Stream()
+    graphs, results = [torch.cuda.CUDAGraph() for _ in inputs], []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for graph, i in zip(graphs, inputs):
+            with torch.cuda.graph(graph, stream=stream):
+                results.append(call(*i))
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for _ in range(6):
+        graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        eager = call(*inputs[0])
+        torch.cuda.synchronize()
+        for got, expected in zip([*results, eager], [*want, want[0]]):
+            assert all(torch.equal(a, b) for a, b in zip(got, expected))
