@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void add_splits_kernel(onebit_block_product p,
   const int token = (int)(at / units), row = (int)(at % units) * 8;
   const long long apart = (long long)p.tokens * p.rows;
   const float* from = grid.partial + (long long)token * p.rows + row;
-  const BlockGrid whole = {0, 0, 1, 0, 0, nullptr};
+  const BlockGrid whole = {0, 0, 0, 1, 0, 0, nullptr};
   const Result result(p, whole, 0);
   float sum[8];
   result.load_bias(row, sum);
@@ -119,7 +119,7 @@ hipError_t launch_few_as(const onebit_block_product& p, BlockGrid grid, hipStrea
 
 BlockGrid plan_block(const onebit_block_product& p, int compute_units) {
   const int groups = p.columns / ONEBIT_CODE_GROUP;
-  BlockGrid grid = {0, kBlock16, 1, groups, compute_units / 32 < 1 ? 1 : std::min(compute_units / 32, 8), nullptr};
+  BlockGrid grid = {0, kBlock16, 0, 1, groups, compute_units / 32 < 1 ? 1 : std::min(compute_units / 32, 8), nullptr};
   auto split = [&](int splits) {
     grid.groups_per_split = (groups + splits - 1) / splits;
     grid.splits = (groups + grid.groups_per_split - 1) / grid.groups_per_split;
@@ -164,6 +164,16 @@ BlockGrid plan_block(const onebit_block_product& p, int compute_units) {
         split(splits);
       }
     }
+  }
+  // Whole rounds of the largest tiles, and what is left in halves of them
+  const Kind &half = kinds[3], &large = kinds[4];
+  const long long tiles_n = (p.tokens + large.tokens - 1) / large.tokens, tiles_m = (p.rows + large.rows - 1) / large.rows, rounds = tiles_m * tiles_n / compute_units;
+  const long long rows_of_tiles = rounds * compute_units / tiles_n;
+  if (p.y_dtype != ONEBIT_DTYPE_F32 && rounds > 0 && rows_of_tiles < tiles_m) {
+    const long long halves = (tiles_m - rows_of_tiles) * ((p.tokens + half.tokens - 1) / half.tokens);
+    const double filled = std::min(1.0, (double)halves / compute_units), step = half.alone + (half.crowded - half.alone) * filled;
+    const double time = rounds * (groups * large.crowded + large.start) + (double)((halves + compute_units - 1) / compute_units) * (groups * step + half.start);
+    if (time < least) grid.kernel = kBlockMixed, grid.large = (int)(rows_of_tiles * tiles_n), split(1);
   }
   return grid;
 }

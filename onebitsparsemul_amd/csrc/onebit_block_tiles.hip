@@ -29,20 +29,9 @@ struct Tile {
 // Rows of 128 codes in LDS, their pieces of 16 at their number exclusive-or half of the row's: the sixteen lanes that LDS serves at a time read a piece of sixteen
 // neighbouring rows from different banks. A lane takes pieces q and q + 4 of both operands' rows: any order of a group's columns will do, if it is one for both.
 template <int WM, int WN, int FM, int FN, int STAGES, bool NARROW>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product p, BlockGrid grid) {
+__device__ __forceinline__ void tile(const onebit_block_product& p, const BlockGrid& grid, int first_row, int m, int n, char* smem) {
   typedef Tile<WM, WN, FM, FN, STAGES> T;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave_m = wave / WN, wave_n = wave % WN;
-  // the tiles of an XCD side by side, four rows of tiles at a time
-  int m, n;
-  {
-    const int total = gridDim.x, tiles_m = total / grid.tiles_n, x = blockIdx.x % grid.xcds;
-    const int tile = total / grid.xcds * x + min(x, total % grid.xcds) + blockIdx.x / grid.xcds;
-    constexpr int kStrip = 4;
-    const int strip = tile / (kStrip * grid.tiles_n), rest = tile - strip * kStrip * grid.tiles_n, high = min(kStrip, tiles_m - strip * kStrip);
-    n = rest / high;
-    m = strip * kStrip + rest - n * high;
-  }
   const int split = blockIdx.y, all = p.columns / ONEBIT_CODE_GROUP, begin = split * grid.groups_per_split, count = min(grid.groups_per_split, all - begin);
 
   // copies: eight rows each, the weight's first
@@ -51,13 +40,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product
   for (int c = 0; c < T::kCopies; ++c) {
     const int piece = c * T::kWaves + wave, row = piece * 8 + lane / 8, chunk = (lane % 8) ^ (row / 2 % 8);
     const bool of_weight = c < T::kRows / 8 / T::kWaves;
-    const int from = of_weight ? min(m * T::kRows + row, p.rows - 1) - m * T::kRows : min(n * T::kTokens + row - T::kRows, p.tokens - 1) - n * T::kTokens;
+    const int from = of_weight ? min(first_row + m * T::kRows + row, p.rows - 1) - (first_row + m * T::kRows) : min(n * T::kTokens + row - T::kRows, p.tokens - 1) - n * T::kTokens;
     offset[c] = (uint32_t)(from * (int)(of_weight ? p.weight.row_stride : p.x.row_stride) + chunk * 16);
   }
-  const char* weight = (const char*)p.weight.codes + (long long)m * T::kRows * p.weight.row_stride + (long long)begin * ONEBIT_CODE_GROUP;
+  const char* weight = (const char*)p.weight.codes + (long long)(first_row + m * T::kRows) * p.weight.row_stride + (long long)begin * ONEBIT_CODE_GROUP;
   const char* x = (const char*)p.x.codes + (long long)n * T::kTokens * p.x.row_stride + (long long)begin * ONEBIT_CODE_GROUP;
   const float* x_scale = p.x.scales + (long long)min(n * T::kTokens + wave_n * FN * 16 + lane % (FN * 16), p.tokens - 1) * p.x.scale_stride;
-  const float* w_scale = p.weight.scales + (long long)min((m * T::kRows + wave_m * FM * 16) / ONEBIT_CODE_GROUP, (p.rows - 1) / ONEBIT_CODE_GROUP) * p.weight.scale_stride + begin;
+  const float* w_scale = p.weight.scales + (long long)min((first_row + m * T::kRows + wave_m * FM * 16) / ONEBIT_CODE_GROUP, (p.rows - 1) / ONEBIT_CODE_GROUP) * p.weight.scale_stride + begin;
   const uint32_t lds = lds_offset_of(smem);
   auto copy = [&](int c, int g, int stage) {  // of a group beyond the last: of the last again, so that as many copies are under way
     g = min(g, count - 1);
@@ -172,50 +161,77 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product
   constexpr int kLanes = FM * 2, kPitch = FM * 16 + 4;  // lanes to a token, floats between tokens
   float* const rows = (float*)smem + wave * 16 * kPitch;
   static_assert(T::kWaves * 16 * kPitch * 4 <= T::kLds, "");
-  const int row = m * T::kRows + wave_m * FM * 16 + lane % kLanes * 8;
-  constexpr int kAcross = FM * 16 < 64 ? FM * 16 : 64;  // or one row after the other
-  const int single = m * T::kRows + wave_m * FM * 16 + lane % kAcross;
-  float bias[8], single_bias[FM * 16 / kAcross];
+  const int row = first_row + m * T::kRows + wave_m * FM * 16 + lane % kLanes * 8;
+  float bias[8];
   result.load_bias(row, bias);
-#pragma unroll
-  for (int at = 0; at < FM * 16 / kAcross; ++at) single_bias[at] = result.bias_of(single + at * kAcross);
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) *(f4_t*)(rows + r * kPitch + i * 16 + q * 4) = sum[i][j];
     __builtin_amdgcn_wave_barrier();
     const int first = n * T::kTokens + (wave_n * FN + j) * 16;
-    if (result.vectors) {
 #pragma unroll 1
-      for (int t = lane / kLanes; t < 16 && first + t < p.tokens; t += 64 / kLanes) {
-        const f4_t v0 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8), v1 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8 + 4);
-        const float v[8] = {v0.x + bias[0], v0.y + bias[1], v0.z + bias[2], v0.w + bias[3], v1.x + bias[4], v1.y + bias[5], v1.z + bias[6], v1.w + bias[7]};
-        result.put(first + t, row, v);
-      }
-    } else {  // neighbours from neighbouring lanes
-#pragma unroll 4
-      for (int t = lane / kAcross; t < 16; t += 64 / kAcross)
-#pragma unroll
-        for (int at = 0; at < FM * 16 / kAcross; ++at)
-          if (first + t < p.tokens) result.put_one(first + t, single + at * kAcross, rows[t * kPitch + at * kAcross + lane % kAcross] + single_bias[at]);
+    for (int t = lane / kLanes; t < 16 && first + t < p.tokens; t += 64 / kLanes) {
+      const f4_t v0 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8), v1 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8 + 4);
+      const float v[8] = {v0.x + bias[0], v0.y + bias[1], v0.z + bias[2], v0.w + bias[3], v1.x + bias[4], v1.y + bias[5], v1.z + bias[6], v1.w + bias[7]};
+      result.put(first + t, row, v);
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// Number `block` of `total` tiles in rows of tiles_n, as a row and a column: the tiles of an XCD side by side, four rows of tiles at a time
+struct Place {
+  int m, n;
+};
+__device__ inline Place place_of(int block, int total, int tiles_n, int xcds) {
+  const int tiles_m = total / tiles_n, x = block % xcds, tile = total / xcds * x + min(x, total % xcds) + block / xcds;
+  constexpr int kStrip = 4;
+  const int strip = tile / (kStrip * tiles_n), rest = tile - strip * kStrip * tiles_n, high = min(kStrip, tiles_m - strip * kStrip), n = rest / high;
+  return {strip * kStrip + rest - n * high, n};
+}
+
+template <int WM, int WN, int FM, int FN, int STAGES, bool NARROW>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(onebit_block_product p, BlockGrid grid) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Place at = place_of(blockIdx.x, gridDim.x, grid.tiles_n, grid.xcds);
+  tile<WM, WN, FM, FN, STAGES, NARROW>(p, grid, 0, at.m, at.n, smem);
+}
+
+// Tiles of 256 x 256 for as many of the weight's rows as whole rounds of the compute units take, the others in tiles of 256 x 128 behind them
+typedef Tile<2, 4, 8, 4, 2> Large;
+typedef Tile<4, 2, 4, 4, 3> Half;
+__global__ __launch_bounds__(512) void mixed_kernel(onebit_block_product p, BlockGrid grid) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int block = blockIdx.x;
+  if (block < grid.large) {
+    const Place at = place_of(block, grid.large, grid.tiles_n, grid.xcds);
+    tile<2, 4, 8, 4, 2, true>(p, grid, 0, at.m, at.n, smem);
+  } else {
+    const int tiles_n = (p.tokens + Half::kTokens - 1) / Half::kTokens;
+    const Place at = place_of(block - grid.large, gridDim.x - grid.large, tiles_n, grid.xcds);
+    tile<4, 2, 4, 4, 3, true>(p, grid, grid.large / grid.tiles_n * Large::kRows, at.m, at.n, smem);
+  }
+}
+
+// The dynamic-LDS limit is a per-device attribute of the kernel; threads that race here set the same value
+template <class Kernel>
+hipError_t allow_lds(Kernel kernel, int bytes, std::atomic<bool> (&set)[64]) {
+  int device = 0;
+  if (hipError_t status = hipGetDevice(&device); status != hipSuccess) return status;
+  if (device < 0 || device >= 64) return hipErrorInvalidDevice;
+  if (set[device].load(std::memory_order_acquire)) return hipSuccess;
+  if (hipError_t status = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); status != hipSuccess) return status;
+  set[device].store(true, std::memory_order_release);
+  return hipSuccess;
 }
 
 template <int WM, int WN, int FM, int FN, int STAGES, bool NARROW>
 hipError_t launch_tiles_as(const onebit_block_product& p, BlockGrid grid, hipStream_t stream) {
   typedef Tile<WM, WN, FM, FN, STAGES> T;
   auto kernel = tile_kernel<WM, WN, FM, FN, STAGES, NARROW>;
-  // the dynamic-LDS limit is a per-device attribute of the kernel; threads that race here set the same value
   static std::atomic<bool> set[64] = {};
-  int device = 0;
-  if (hipError_t status = hipGetDevice(&device); status != hipSuccess) return status;
-  if (device < 0 || device >= 64) return hipErrorInvalidDevice;
-  if (!set[device].load(std::memory_order_acquire)) {
-    if (hipError_t status = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds); status != hipSuccess) return status;
-    set[device].store(true, std::memory_order_release);
-  }
+  if (hipError_t status = allow_lds(kernel, T::kLds, set); status != hipSuccess) return status;
   const int tiles_m = (p.rows + T::kRows - 1) / T::kRows, tiles_n = (p.tokens + T::kTokens - 1) / T::kTokens;
   grid.tiles_n = tiles_n;
   if ((long long)tiles_m * tiles_n * 64 * T::kWaves >= 1ll << 32) return hipErrorInvalidConfiguration;
@@ -233,6 +249,17 @@ hipError_t launch_tiles(const onebit_block_product& p, const BlockGrid& grid, hi
 
 hipError_t launch_block_tiles(const onebit_block_product& p, const BlockGrid& grid, hipStream_t stream) {
   switch (grid.kernel) {
+    case kBlockMixed: {
+      static std::atomic<bool> set[64] = {};
+      constexpr int kLds = Large::kLds > Half::kLds ? Large::kLds : Half::kLds;
+      if (hipError_t status = allow_lds(mixed_kernel, kLds, set); status != hipSuccess) return status;
+      BlockGrid mixed = grid;
+      mixed.tiles_n = (p.tokens + Large::kTokens - 1) / Large::kTokens;
+      const int rows_left = p.rows - grid.large / mixed.tiles_n * Large::kRows;
+      const long long half = (long long)((rows_left + Half::kRows - 1) / Half::kRows) * ((p.tokens + Half::kTokens - 1) / Half::kTokens);
+      if ((grid.large + half) * 512 >= 1ll << 32) return hipErrorInvalidConfiguration;
+      return launch_kernel(mixed_kernel, dim3((unsigned)(grid.large + half)), dim3(512), kLds, stream, p, mixed);
+    }
     case kBlock128x32: return launch_tiles<4, 1, 2, 2, 3>(p, grid, stream);
     case kBlock64x64: return launch_tiles<2, 2, 2, 2, 4>(p, grid, stream);
     case kBlock128x64: return launch_tiles<4, 2, 2, 2, 3>(p, grid, stream);

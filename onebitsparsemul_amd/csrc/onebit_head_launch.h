@@ -9,11 +9,13 @@ hipError_t launch_quantize_rows(const void* x, int dtype, long long x_stride, in
 
 // A product's launch. Groups of 128 columns split over workgroups: split s takes groups [s * groups_per_split, ...) of all, and writes fp32 sums to
 // partial + s * tokens * rows; a second kernel adds them in order. splits == 1: straight into y.
-enum BlockKernel { kBlock16, kBlock16Wide, kBlock64, kBlock128x32, kBlock64x64, kBlock128x64, kBlock256x128, kBlock256x256 };  // rows of the weight (a sixteenth; wide: on eight wavefronts); rows x tokens
+enum BlockKernel { kBlock16, kBlock16Wide, kBlock64, kBlock128x32, kBlock64x64, kBlock128x64, kBlock256x128, kBlock256x256, kBlockMixed };
+// (rows of the weight, wide: on eight wavefronts; rows x tokens; mixed: the last two)
 constexpr int kLeastTileGroups = 4;  // of a tile's split
 struct BlockGrid {
   int tiles_n;  // of tokens, filled by the launcher
   int kernel;
+  int large;    // kBlockMixed: how many tiles of 256 x 256, whole rows of them
   int splits, groups_per_split;
   int xcds;  // workgroup b runs on XCD b % xcds
   float* partial;
