@@ -89,21 +89,25 @@ __global__ __launch_bounds__(256) void add_splits_kernel(onebit_block_product p,
   const Result result(p, whole, 0);
   float sum[8];
   result.load_bias(row, sum);
-  if (p.rows % 4 == 0 && row + 8 <= p.rows) {
-    f4_t low = {}, high = {};
+  // (four splits' loads under way, whole vectors from any place; a row's last few one by one)
+  typedef float vector __attribute__((ext_vector_type(4), aligned(4)));
+  const bool whole_unit = row + 8 <= p.rows;
+  f4_t low = {}, high = {};
 #pragma unroll 4
-    for (int s = 0; s < grid.splits; ++s, from += apart) low += ((const f4_t*)from)[0], high += ((const f4_t*)from)[1];
+  for (int s = 0; s < grid.splits; ++s) {
+    const float* const of_split = from + s * apart;
+    if (whole_unit) {
+      low += ((const vector*)of_split)[0], high += ((const vector*)of_split)[1];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += low[i], sum[i + 4] += high[i];
-  } else {
-    float total[8] = {};
-    for (int s = 0; s < grid.splits; ++s, from += apart)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (row + i < p.rows) total[i] += from[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += total[i];
+      for (int i = 0; i < 4; ++i) {
+        low[i] += row + i < p.rows ? of_split[i] : 0.f;
+        high[i] += row + 4 + i < p.rows ? of_split[4 + i] : 0.f;
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] += low[i], sum[i + 4] += high[i];
   result.put(token, row, sum);
 }
 
@@ -126,54 +130,70 @@ BlockGrid plan_block(const onebit_block_product& p, int compute_units) {
   };
   // (a tile's copies know a row's distance in 32 bits)
   auto near = [](const onebit_codes& c) { return c.row_stride >= 0 && c.row_stride < 1 << 23; };
-  if (p.tokens <= 16 || groups < kLeastTileGroups || !near(p.x) || !near(p.weight)) {
-    // 64 rows to a workgroup, where there are enough of them: the tokens' codes are read for four times as many of the weight. 16 tokens on 131072 x 4096: 109 us (4.9 TB/s),
-    // with 32 rows 136, with 16 rows 163; 11008 x 4096 13.0, 14.6, 14.6 (one token 10.7, 11.5, 10.0); 4096 x 4096 12.7, 8.9, 6.7 (eight wavefronts), 4096 x 512 3.6, 3.9, 2.7.
-    const int rows = (p.rows + 15) / 16, tokens = (p.tokens + 15) / 16;
-    if ((long long)(rows + 3) / 4 * tokens >= compute_units / 2) {
-      grid.kernel = kBlock64;
-    } else {
-      grid.kernel = groups >= 16 ? kBlock16Wide : kBlock16;
-      // (300 x 28672 with 16 tokens 29.5 us, in two splits 16.2; 4096 x 4096 6.7, in two 6.9)
-      if ((long long)rows * tokens * 2 <= compute_units && groups >= 32) split((int)std::min<long long>(groups / 16, compute_units / ((long long)rows * tokens)));
+  const bool tiles_may = groups >= kLeastTileGroups && near(p.x) && near(p.weight);
+  double least = 1e30;
+  auto consider = [&](int kernel, int splits, double time) {
+    // another launch, which waits for the sums of other compute units' caches; sums out and in again, at 3 TB/s
+    if (splits > 1) time += 4.0 + 0.4 * splits + 8e-6 * splits * p.tokens * p.rows / 3.0;
+    if (time < least) {
+      least = time;
+      grid.kernel = kernel;
+      split(splits);
     }
-    return grid;
+  };
+  // 16 tokens to a workgroup: a wavefront's groups one behind the other, or the bytes that the caches and the memory deliver (the tokens' codes for each workgroup again). Measured: 16
+  // tokens on 131072 x 4096 with 64 rows 109 us (4.9 TB/s), with 32 rows 136, with 16 rows 163; 11008 x 4096 13.0, 14.6, 14.6 (one token 10.7, 11.5, 10.0); 4096 x 4096
+  // 12.7, 8.9, 7.3 (eight wavefronts 6.7); 4096 x 512 3.6, 3.9, 2.7; 300 x 28672 67, 44, 36 (29.5, in two splits 16.2).
+  struct Few {
+    int kernel, rows, wavefronts;
+    double start, step;
+  };
+  static const Few few[] = {{kBlock16, 16, 4, 2.2, 0.40}, {kBlock16Wide, 16, 8, 2.0, 0.80}, {kBlock64, 64, 4, 2.9, 1.05}};
+  const long long token_tiles = (p.tokens + 15) / 16;
+  const double weight_bytes = (double)p.rows * p.columns;
+  for (const Few& kind : few) {
+    // (eight wavefronts where each has more than four steps: one token on 11008 x 16384 38 us, with four 46; 8192 columns 18.2 and 19.1, 4096 10.6 and 10.2)
+    if (kind.kernel == (groups > 64 ? kBlock16 : kBlock16Wide) || (kind.kernel == kBlock64 && token_tiles > 1 && tiles_may)) continue;
+    const double blocks = (double)((p.rows + kind.rows - 1) / kind.rows) * token_tiles;
+    const double through = 2.2 + std::max(weight_bytes / 4.9e6, (weight_bytes * token_tiles + blocks * std::min(p.tokens, 16) * p.columns) / 7e6);
+    for (int splits = 1; splits <= 16 && (splits == 1 || groups / splits >= kind.wavefronts); ++splits) {
+      if (splits > 1 && blocks * splits > 2 * compute_units) break;
+      const int steps = ((groups + splits - 1) / splits + kind.wavefronts - 1) / kind.wavefronts;
+      consider(kind.kernel, splits, std::max(kind.start + steps * kind.step, through));
+    }
   }
-  // A group's time in a tile where workgroups are few and where every compute unit has one, and what a tile costs beside them, as measured: 128 tokens on 11008 x 4096,
-  // 4096 on 8192 x 8192, 64 on 32000 x 4096.
+  if (!tiles_may) return grid;
+  // A group's time in a tile where workgroups are few and where every compute unit has its number, and what a tile costs beside them, fitted to 150 random shapes of 1 ... 3000 tokens,
+  // 64 ... 60000 rows and 512 ... 14336 columns, which it meets to 3 to 6 %; not less than the weight takes from memory. The kernel that the plan takes is 2 % slower than the best of all in the mean. Products in fp16 are no good for the largest tile, which spills.
   struct Kind {
     int kernel, rows, tokens, on_unit;
-    double alone, crowded, start;
+    double start, alone, crowded, alone_in_fp16, crowded_in_fp16;
   };
-  static const Kind kinds[] = {{kBlock128x32, 128, 32, 1, 0.40, 0.80, 3.0}, {kBlock64x64, 64, 64, 2, 0.35, 0.55, 3.0}, {kBlock128x64, 128, 64, 1, 0.42, 0.62, 3.5},
-                               {kBlock256x128, 256, 128, 1, 0.80, 1.08, 6.0}, {kBlock256x256, 256, 256, 1, 1.28, 1.65, 8.0}};
-  double least = 1e30;
+  static const Kind kinds[] = {{kBlock128x32, 128, 32, 1, 3.5, 0.34, 0.55, 0.54, 0.57}, {kBlock64x64, 64, 64, 2, 3.5, 0.33, 0.49, 0.56, 0.80}, {kBlock128x64, 128, 64, 1, 3.8, 0.38, 0.48, 0.63, 0.78},
+                               {kBlock256x128, 256, 128, 1, 7.0, 0.68, 0.87, 1.50, 2.10}, {kBlock256x256, 256, 256, 1, 10.0, 1.13, 1.63, 0., 0.}};
+  const bool in_fp16 = !narrow_products(p);
+  auto rounds_of = [&](const Kind& kind, long long blocks, int steps) {
+    const double alone = in_fp16 ? kind.alone_in_fp16 : kind.alone, crowded = in_fp16 ? kind.crowded_in_fp16 : kind.crowded;
+    const long long places = (long long)compute_units * kind.on_unit, rest = blocks % places;
+    const double filled = kind.on_unit == 1 ? (double)rest / places : rest > compute_units;  // (of two workgroups, one has its compute unit to itself or has not)
+    return (double)(blocks / places) * (steps * crowded + kind.start) + (rest ? steps * (alone + (crowded - alone) * filled) + kind.start : 0.);
+  };
   for (const Kind& kind : kinds) {
-    if (kind.kernel == kBlock128x32 && p.tokens > 32) continue;
-    const long long tiles = (long long)((p.rows + kind.rows - 1) / kind.rows) * ((p.tokens + kind.tokens - 1) / kind.tokens), places = (long long)compute_units * kind.on_unit;
+    if ((kind.kernel == kBlock128x32 && p.tokens > 32) || (kind.kernel == kBlock256x256 && in_fp16)) continue;
+    const long long tiles = (long long)((p.rows + kind.rows - 1) / kind.rows) * ((p.tokens + kind.tokens - 1) / kind.tokens);
     for (int splits = 1; splits <= 16 && groups / splits >= kLeastTileGroups; ++splits) {
-      const long long blocks = tiles * splits;
-      if (splits > 1 && blocks > places) break;
-      const double filled = std::min(1.0, (double)blocks / places), step = kind.alone + (kind.crowded - kind.alone) * filled;
-      const double rounds = (double)((blocks + places - 1) / places);
-      double time = rounds * (((groups + splits - 1) / splits) * step + kind.start);
-      if (splits > 1) time += 3.0 + 8e-6 * splits * p.tokens * p.rows / 3.0;  // sums out and in again, at 3 TB/s
-      if (time < least) {
-        least = time;
-        grid.kernel = kind.kernel;
-        split(splits);
-      }
+      if (splits > 1 && tiles * splits > (long long)compute_units * kind.on_unit) break;
+      consider(kind.kernel, splits, std::max(rounds_of(kind, tiles * splits, (groups + splits - 1) / splits), 3.0 + weight_bytes / 4.9e6));
     }
   }
   // Whole rounds of the largest tiles, and what is left in halves of them
   const Kind &half = kinds[3], &large = kinds[4];
   const long long tiles_n = (p.tokens + large.tokens - 1) / large.tokens, tiles_m = (p.rows + large.rows - 1) / large.rows, rounds = tiles_m * tiles_n / compute_units;
   const long long rows_of_tiles = rounds * compute_units / tiles_n;
-  if (p.y_dtype != ONEBIT_DTYPE_F32 && rounds > 0 && rows_of_tiles < tiles_m) {
+  if (!in_fp16 && rounds > 0 && rows_of_tiles < tiles_m) {
     const long long halves = (tiles_m - rows_of_tiles) * ((p.tokens + half.tokens - 1) / half.tokens);
-    const double filled = std::min(1.0, (double)halves / compute_units), step = half.alone + (half.crowded - half.alone) * filled;
-    const double time = rounds * (groups * large.crowded + large.start) + (double)((halves + compute_units - 1) / compute_units) * (groups * step + half.start);
-    if (time < least) grid.kernel = kBlockMixed, grid.large = (int)(rows_of_tiles * tiles_n), split(1);
+    consider(kBlockMixed, 1, rounds_of(large, rows_of_tiles * tiles_n, groups) + rounds_of(half, halves, groups));
+    if (grid.kernel == kBlockMixed) grid.large = (int)(rows_of_tiles * tiles_n);
   }
   return grid;
 }

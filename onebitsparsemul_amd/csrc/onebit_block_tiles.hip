@@ -240,9 +240,7 @@ hipError_t launch_tiles_as(const onebit_block_product& p, BlockGrid grid, hipStr
 
 template <int WM, int WN, int FM, int FN, int STAGES>
 hipError_t launch_tiles(const onebit_block_product& p, const BlockGrid& grid, hipStream_t stream) {
-  // 16-bit results: the 8-bit instruction, twice as fast. It cuts the products of eight neighbouring columns off at 2^-13 of the largest: 1.5e-5 off over normal values, a
-  // fourteenth of an fp16 result's own rounding. fp32 results take the products in fp16.
-  return p.y_dtype == ONEBIT_DTYPE_F32 ? launch_tiles_as<WM, WN, FM, FN, STAGES, false>(p, grid, stream) : launch_tiles_as<WM, WN, FM, FN, STAGES, true>(p, grid, stream);
+  return narrow_products(p) ? launch_tiles_as<WM, WN, FM, FN, STAGES, true>(p, grid, stream) : launch_tiles_as<WM, WN, FM, FN, STAGES, false>(p, grid, stream);
 }
 
 }  // namespace
@@ -264,9 +262,7 @@ hipError_t launch_block_tiles(const onebit_block_product& p, const BlockGrid& gr
     case kBlock64x64: return launch_tiles<2, 2, 2, 2, 4>(p, grid, stream);
     case kBlock128x64: return launch_tiles<4, 2, 2, 2, 3>(p, grid, stream);
     case kBlock256x128: return launch_tiles<4, 2, 4, 4, 3>(p, grid, stream);
-    default:
-      // (in fp16 the wave tile of 128 x 64 spills)
-      return p.y_dtype == ONEBIT_DTYPE_F32 ? launch_tiles_as<4, 2, 4, 4, 2, false>(p, grid, stream) : launch_tiles_as<2, 4, 8, 4, 2, true>(p, grid, stream);
+    default: return !narrow_products(p) ? hipErrorInvalidValue : launch_tiles_as<2, 4, 8, 4, 2, true>(p, grid, stream);  // (the plan takes no other)
   }
 }
 

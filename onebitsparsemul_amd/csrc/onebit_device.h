@@ -251,11 +251,6 @@ __device__ __forceinline__ void lds_dma16_base(const void* base, uint32_t lane_o
                : "memory");
 }
 
-// global_load_lds_dword: four bytes a lane, 256 of a wavefront.
-__device__ __forceinline__ void lds_dma4(const void* gptr, uint32_t lds_wave_base) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_wave_base), "v"(gptr) : "memory");
-}
-
 // Raw buffer loads: address = descriptor base (wave-uniform) + vector offset + scalar offset, so a loop that walks
 // memory needs scalar additions only and one vector register of lane offsets. The descriptor covers `bytes` bytes
 // (untyped 32-bit data format); the scalar offset takes no part in its range check, so callers keep every access

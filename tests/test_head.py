@@ -149,10 +149,15 @@ def check_product(tokens, rows, columns, dtype=torch.float32, bias=False, seed=0
         want, size = want + b.double().cuda(), size + b.double().abs().cuda()
     error = (y.double() - want).abs()
     bound = U[dtype] * (1 + 2.0**-10) * want.abs() + (130 + 3 * (columns // 128)) * 2.0**-23 * size
+    cut = 7 * 2.0**-13 * size if dtype != torch.float32 and tokens > 16 else 0 * size
     if dtype == torch.float16:
         bound = bound + 2.0**-25
+        # a value rounds to infinity from 65520 on, half a step above the largest: the sum before its rounding is off by the bound without that rounding, and all beyond 65504 + 32 + that are infinite
+        before, infinite = (130 + 3 * (columns // 128)) * 2.0**-23 * size + cut, y.isinf()
+        assert bool((want.abs() >= 65520 - before)[infinite].all()) and bool(infinite[want.abs() > 65520 + before].all()) and torch.equal(y[infinite].sign().double(), want[infinite].sign())
+        y, want, error = torch.where(infinite, 0, y), torch.where(infinite, 0, want), torch.where(infinite, 0, error)
     if dtype != torch.float32 and tokens > 16:
-        bound = bound + 7 * 2.0**-13 * size
+        bound = bound + cut
         # (a rounding is off by u / sqrt(3) at most on average)
         assert float(error.norm()) <= (U[dtype] / math.sqrt(3) + 2.0**-13) * float(want.norm())
     assert y.dtype == dtype and y.shape == (tokens, rows) and bool(torch.isfinite(y).all())
@@ -194,6 +199,41 @@ def test_products_of_whole_numbers_are_exact(tokens, rows, columns):
     xd = x.double() * xs.double().repeat_interleave(128, 1)
     wd = w.double() * ws.double().repeat_interleave(128, 0)[:rows].repeat_interleave(128, 1)
     assert torch.equal(y.double().cpu(), xd @ wd.T)
+
+
+# (each of the kernels and splits that the plan takes, among them whole rounds of tiles of 256 x 256 with what is left in halves)
+KERNELS = [(1, 4099, 11008), (16, 900, 14336), (9, 11008, 2048), (20, 37000, 512), (17, 33000, 4096), (20, 37001, 1408), (33, 4099, 8192), (100, 2304, 4096), (128, 11008, 1408),
+           (333, 4099, 1408), (1000, 8192, 640), (200, 37000, 512), (2048, 8192, 512), (512, 37000, 640), (2048, 11008, 512), (2049, 9001, 512), (4096, 4099, 1024), (3000, 7000, 640)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,rows,columns", KERNELS)
+def test_products_of_every_kernel(tokens, rows, columns, dtype):
+    check_product(tokens, rows, columns, dtype, bias=rows % 2 == 1)
+
+
+@pytest.mark.parametrize("tokens,rows,columns", [shape for shape in KERNELS if shape[2] <= 1024] + [(1, 131072, 512), (70, 50257, 512)])
+def test_small_whole_numbers_are_exact_in_any_type(tokens, rows, columns):
+    """Codes -1 ... 1 and scales 1: sums of at most 1024, whole in fp16 and, below 256, in bf16, and no product below another's 2^-13"""
+    g = generator(tokens)
+    x, w = (torch.randint(-1, 2, (n, columns), generator=g).float().cuda() for n in (tokens, rows))
+    xs, ws = torch.ones((tokens, columns // 128), device="cuda"), torch.ones((-(-rows // 128), columns // 128), device="cuda")
+    want = x.double() @ w.double().T.contiguous()
+    x, w = x.to(E4M3), w.to(E4M3)
+    for dtype in DTYPES:
+        assert torch.equal(onebit.block_linear(x, xs, w, ws, out_dtype=dtype), want.to(dtype))
+
+
+def test_products_of_rows_far_apart():
+    """Weights 2^24 codes apart, with an offset beyond 32 bits"""
+    g = generator(5)
+    (x, xs), (w, ws) = random_codes(40, 640, g), random_codes(300, 640, g, 128)
+    x, xs, w, ws = x.cuda(), xs.cuda(), w.cuda(), ws.cuda()
+    apart = torch.empty((300, 1 << 24), dtype=torch.uint8, device="cuda")
+    apart[:, 64:704] = w.view(torch.uint8)
+    want = onebit.block_linear(x, xs, w, ws, out_dtype=torch.float32)
+    got = onebit.block_linear(x, xs, apart[:, 64:704].view(E4M3), ws, out_dtype=torch.float32)
+    assert float((got - want).norm() / want.norm()) < 1e-5  # (fp32 sums in another order)
 
 
 def test_products_of_views_into_given_results():
