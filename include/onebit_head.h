@@ -7,7 +7,7 @@
  * enqueued on `stream` (hipStream_t as void*, NULL = default stream) and the calls return without synchronising. They allocate
  * nothing, keep nothing between calls, and can be captured in a HIP graph. Status codes, dtype codes and
  * onebit_sparse_last_error() are those of onebit_sparse_tensor.h; a call of more than 2^32 threads is refused as HIP refuses it.
- * Results lie apart from the operands, and the workspace from both.
+ * Results lie apart from the operands, their rows from each other, and the workspace from all.
  */
 #ifndef ONEBIT_HEAD_H_
 #define ONEBIT_HEAD_H_
@@ -45,7 +45,7 @@ int onebit_block_norm_codes(const onebit_norm *norm, const onebit_codes *out, vo
  * + bias[m]: tokens x rows values, fp32, fp16 or bf16 (y_dtype), y_stride between tokens. Products of codes are exact, their sums and everything behind
  * them fp32, y is rounded once; but for fp16 and bf16 results of more than 16 tokens the products of eight neighbouring columns are cut off
  * at 2^-13 of the largest of them, as the 8-bit matrix instruction does (1.5e-5 of y over normal values). weight: `rows` rows of codes, scales for each 128 rows and
- * columns (ceil(rows / 128) rows of them). columns: a multiple of 128. bias: `rows` values (bias_dtype), or NULL. workspace:
+ * columns (ceil(rows / 128) rows of them). columns: a multiple of 128. tokens, rows, columns: at most 2^30. bias: `rows` values (bias_dtype), or NULL. workspace:
  * onebit_block_linear_workspace() bytes, 16-byte aligned (NULL where that is 0). A NaN among a token's codes or scales reaches that token's results alone.
  */
 typedef struct onebit_block_product {

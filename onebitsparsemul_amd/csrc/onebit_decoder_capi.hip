@@ -150,6 +150,7 @@ int onebit_block_norm_codes(const onebit_norm* n, const onebit_codes* out, void*
   if (!n || !n->residual || !n->weight) return refuse("residual and weight must not be null");
   CHECKED(check_norm(*n));
   CHECKED(onebit::check_codes(out, "the result"));
+  CHECKED(onebit::check_apart(*out, n->rows, n->hidden));
   return launched(onebit::launch_norm(*n, out, (hipStream_t)stream), "onebit_block_norm_codes");
 }
 

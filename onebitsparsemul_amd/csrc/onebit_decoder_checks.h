@@ -31,6 +31,13 @@ inline int check_codes(const onebit_codes* c, const char* name) {
     return refuse("the codes of %s must be 16-byte aligned, with rows a multiple of 16 apart", name);
   return ONEBIT_OK;
 }
+// Rows that are written must not overlap
+inline int check_apart(const onebit_codes& c, int rows, int columns) {
+  const long long groups = ((long long)columns + ONEBIT_CODE_GROUP - 1) / ONEBIT_CODE_GROUP;
+  if (rows > 1 && (c.row_stride < groups * ONEBIT_CODE_GROUP || c.scale_stride < groups))
+    return refuse("rows of the result's codes and scales must not overlap (strides %lld, %lld)", c.row_stride, c.scale_stride);
+  return ONEBIT_OK;
+}
 
 }  // namespace onebit
 

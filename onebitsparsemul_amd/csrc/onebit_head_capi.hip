@@ -13,8 +13,10 @@ int check_product(const onebit_block_product* p) {
   if (!p || !p->y) return refuse("y must not be null");
   CHECKED(onebit::check_codes(&p->x, "x"));
   CHECKED(onebit::check_codes(&p->weight, "the weight"));
-  if (p->tokens < 1 || p->rows < 1) return refuse("tokens and rows must be positive (got %d, %d)", p->tokens, p->rows);
-  if (p->columns < ONEBIT_CODE_GROUP || p->columns % ONEBIT_CODE_GROUP) return refuse("columns = %d: rows of codes have a positive multiple of 128", p->columns);
+  constexpr int kMost = 1 << 30;
+  if (p->tokens < 1 || p->rows < 1 || p->tokens > kMost || p->rows > kMost) return refuse("tokens and rows must be positive and at most 2^30 (got %d, %d)", p->tokens, p->rows);
+  if (p->columns < ONEBIT_CODE_GROUP || p->columns % ONEBIT_CODE_GROUP || p->columns > kMost) return refuse("columns = %d: rows of codes have a positive multiple of 128, at most 2^30", p->columns);
+  if (p->tokens > 1 && p->y_stride < p->rows) return refuse("rows of y must not overlap (stride %lld)", p->y_stride);
   if (!is_type(p->y_dtype) || (p->bias && !is_type(p->bias_dtype))) return refuse("dtype codes must be 0 (fp32), 1 (fp16) or 2 (bf16)");
   return ONEBIT_OK;
 }
@@ -36,6 +38,7 @@ int onebit_quantize_rows(const void* x, int dtype, long long x_stride, int rows,
   if (!is_type(dtype)) return refuse("dtype code must be 0 (fp32), 1 (fp16) or 2 (bf16), got %d", dtype);
   if (rows < 1 || columns < 1 || columns > 1 << 30) return refuse("rows must be positive and columns 1 to 2^30 (got %d, %d)", rows, columns);
   CHECKED(onebit::check_codes(out, "the result"));
+  CHECKED(onebit::check_apart(*out, rows, columns));
   return launched(onebit::launch_quantize_rows(x, dtype, x_stride, rows, columns, *out, (hipStream_t)stream), "onebit_quantize_rows");
 }
 

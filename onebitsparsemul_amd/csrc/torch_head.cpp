@@ -28,6 +28,7 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
 void check_codes(const torch::Tensor& t, const char* name, const c10::Device& device) {
   check_gpu(t, name, device);
   TORCH_CHECK_TYPE(t.scalar_type() == torch::kFloat8_e4m3fn, name, " must be float8_e4m3fn, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(!t.is_neg(), name, " must not be a negated view");
 }
 void check_scales(const torch::Tensor& t, const char* name, const c10::Device& device) {
   check_gpu(t, name, device);
@@ -72,6 +73,7 @@ torch::Tensor block_linear(const torch::Tensor& codes, const torch::Tensor& scal
     for (const torch::Tensor* t : {&codes, &scales, &weight_codes, &weight_scales})
       TORCH_CHECK_VALUE(!may_meet(*t, *out), "out must lie apart from the operands");
     TORCH_CHECK_VALUE(!bias.has_value() || !may_meet(*bias, *out), "out must lie apart from the operands");
+    TORCH_CHECK_VALUE(out->is_contiguous() || out->size(0) < 2 || out->stride(0) >= rows, "out's rows must not overlap");
   }
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
   torch::Tensor y = out.has_value() ? *out : empty_result(shape, type, device);

@@ -69,6 +69,16 @@ class BlockLinear(torch.nn.Module):
         self.register_buffer("scales", scales)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse=True):
+        # of a change of the module's type (half() and the like) codes and scales take the move alone
+        before = {name: getattr(self, name) for name in ("codes", "scales")}
+        super()._apply(fn, recurse)
+        for name, t in before.items():
+            now = getattr(self, name)
+            if now.dtype != t.dtype:
+                setattr(self, name, t.to(now.device))
+        return self
+
     def forward(self, x):
         """x (..., columns), or its (codes, scales) of quantize_rows or block_norm_codes"""
         if isinstance(x, torch.Tensor):

@@ -280,6 +280,15 @@ def test_what_is_not_finite_stays_in_its_token(tokens):
     got = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
     others = [t for t in range(tokens) if t != tokens // 2]
     assert bool(torch.isnan(got[tokens // 2]).all()) and torch.equal(got[others], clean[others])
+    # a code that is NaN, of a token and of a weight's row
+    xs[tokens // 2, 1] = 1.0
+    x.view(torch.uint8)[tokens // 2, 200] = 0x7f
+    got = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
+    assert bool(torch.isnan(got[tokens // 2]).all()) and torch.equal(got[others], clean[others])
+    x.view(torch.uint8)[tokens // 2, 200] = 0
+    w.view(torch.uint8)[77, 500] = 0xff
+    got = onebit.block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
+    assert bool(torch.isnan(got[:, 77]).all()) and torch.equal(got[others][:, :77], clean[others][:, :77]) and torch.equal(got[others][:, 78:], clean[others][:, 78:])
 
 
 @pytest.mark.parametrize("tokens", [1, 3, 16, 17, 64, 200])

@@ -132,6 +132,28 @@ def test_a_layer_keeps_its_codes_in_its_state(tmp_path):
         assert torch.equal(getattr(layer, name).float(), getattr(other, name).float())
 
 
+def test_rows_that_would_overlap_and_sizes_beyond_int_are_refused(lib):
+    for out in (Codes(A, A, 128, 2), Codes(A, A, 256, 1)):
+        assert lib.onebit_quantize_rows(ctypes.c_void_p(A), 0, ctypes.c_longlong(200), 2, 200, ctypes.byref(out), None) == 1 and "must not overlap" in _native.last_error()
+        from test_decoder_host import Norm
+        assert lib.onebit_block_norm_codes(ctypes.byref(Norm(residual=A, weight=A, rows=2, hidden=200, residual_scale=1, block_scale=1, residual_stride=200)), ctypes.byref(out), None) == 1
+        assert "must not overlap" in _native.last_error()
+    good = dict(x=Codes(A, A, 256, 2), weight=Codes(A, A, 256, 2), y=A, y_stride=64, tokens=3, rows=64, columns=256, y_dtype=1)
+    for change, message in ((dict(y_stride=63), "must not overlap"), (dict(tokens=(1 << 30) + 1), "at most 2^30"), (dict(rows=(1 << 30) + 1), "at most 2^30"),
+                            (dict(columns=(1 << 30) + 128), "at most 2^30")):
+        p = Product(**{**good, **change})
+        assert lib.onebit_block_linear(ctypes.byref(p), None, None) == 1 and message in _native.last_error()
+
+
+def test_a_layer_of_another_type_keeps_its_codes():
+    layer = torch.nn.Sequential(onebit.BlockLinear(torch.randn(70, 130), bias=torch.randn(70)))
+    codes, scales = layer[0].codes.clone(), layer[0].scales.clone()
+    for change in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu")):
+        change(layer)
+        assert layer[0].codes.dtype == torch.float8_e4m3fn and torch.equal(layer[0].codes.float(), codes.float()) and torch.equal(layer[0].scales, scales)
+    assert layer[0].bias.dtype == torch.float64 and layer.to("meta")[0].codes.device.type == "meta"
+
+
 def test_tensors_on_the_host_are_refused():
     x = torch.zeros((2, 256))
     codes, scales = onebit.quantize_weight(x)
@@ -159,6 +181,8 @@ def test_the_binding_refuses():
         (ValueError, "bias must be", lambda: onebit.block_linear(codes, scales, w, ws, bias=u)), (ValueError, "out must have", lambda: onebit.block_linear(codes, scales, w, ws, out=out[:2])),
         (ValueError, "out must have", lambda: onebit.block_linear(codes, scales, w[:100], ws[:1], out=out[:, ::2])),
         (RuntimeError, "single memory location", lambda: onebit.block_linear(codes, scales, w, ws, out=out[:1].expand(3, 200))),
+        (ValueError, "must not overlap", lambda: onebit.block_linear(codes, scales, w, ws, out=out.as_strided((3, 200), (100, 1)))),
+        (ValueError, "negated", lambda: onebit.block_linear(torch._neg_view(codes), scales, w, ws)),
         (ValueError, "apart from", lambda: onebit.block_linear(inside, scales, w, ws, out=whole.view(torch.float16)[100:700].view(3, 200))),
         (ValueError, "whole rows a multiple of 16", lambda: onebit.block_linear(codes, scales, w.as_strided((199, 256), (257, 1)), ws)),
         (TypeError, "uniform must be", lambda: onebit.sample(logits, u.half())), (ValueError, "one number for each row", lambda: onebit.sample(logits, u[:2])),
