@@ -5,6 +5,9 @@
 // A row is looked at once in full: the largest of each group of neighbouring logits stays. The k largest logits are not below the k-th largest of the groups' largest, and
 // those that make up a share of the mass not below the value above which the groups' largest make it up alone; so that the filters
 // see a list of few candidates, from the few groups that reach that value, in the order of their indices. Where a list would not hold them they go over the row's groups instead.
+//
+// Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 10 to 12 us whatever the number of rows;
+// 64 rows of 4096, in one kernel, 5.6. A row of 131072 that keeps more candidates than a list holds takes one workgroup 85 to 250 us, for the arithmetic of its weights.
 #include "onebit_decoder_device.h"
 #include "onebit_head_launch.h"
 
