@@ -74,6 +74,42 @@ struct Result {
     else if (type == ONEBIT_DTYPE_F16) store_values<ONEBIT_DTYPE_F16, 1>(base, token * stride + row, one);
     else store_values<ONEBIT_DTYPE_BF16, 1>(base, token * stride + row, one);
   }
+  // The sums of a matrix instruction's rows 4 q ... 4 q + 3, of lanes 16 q ... 16 q + 15, of two neighbouring parts of 16 rows, in 16 bits: the second and fourth 16 lanes' values of
+  // the first part change places with the first and third 16 lanes' of the second, after which a lane has eight neighbouring rows, from q / 2 * 8 of part q % 2 on.
+  __device__ u4_t eight_of(const f4_t& first, const f4_t& second) const {
+    u2_t a, b;
+    if (type == ONEBIT_DTYPE_F16) a = packed<_Float16>(first), b = packed<_Float16>(second);
+    else a = packed<__bf16>(first), b = packed<__bf16>(second);
+    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+    return u4_t{x[0], y[0], x[1], y[1]};
+  }
+  __device__ void put_eight(int token, int row, const u4_t& eight) const {
+    typedef uint32_t vector __attribute__((ext_vector_type(4), aligned(2)));
+    uint16_t* const to = (uint16_t*)base + token * stride + row;
+    if (row + 8 <= rows) {
+      *(vector*)to = eight;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (row + i < rows) to[i] = (uint16_t)(eight[i / 2] >> i % 2 * 16);
+    }
+  }
+  template <class T>
+  static __device__ u2_t packed(const f4_t& v) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u2_t, four{(T)v.x, (T)v.y, (T)v.z, (T)v.w});
+  }
+  __device__ void put_four(int token, int row, const f4_t& v) const {
+    typedef float vector __attribute__((ext_vector_type(4), aligned(4)));
+    float* const to = (float*)base + token * stride + row;
+    if (row + 4 <= rows) {
+      *(vector*)to = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (row + i < rows) to[i] = v[i];
+    }
+  }
   // and eight of a token from weight row `row` on, a multiple of eight
   __device__ void put(int token, int row, const float (&v)[8]) const {
     const long long at = token * stride + row;

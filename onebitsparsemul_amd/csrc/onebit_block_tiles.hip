@@ -83,13 +83,13 @@ __device__ __forceinline__ void tile(const onebit_block_product& p, const BlockG
 #pragma unroll
     for (int j = 0; j < FN; ++j) next[j] = of_group[(j * 16 + r) * 4];
   };
-  // The weight's scales of 64 groups, one to a lane: a load in the loop would be waited for with the copies in front of it.
+  // The weight's scales of 64 groups, one to a lane: a load in the loop would be waited for with the copies in front of it. The first 64 come with the first copies, where the tokens' second ones will be.
   auto read_weight_scales = [&](int g) {
     float w = w_scale[min(g + lane, count - 1)];
     asm volatile("" : "+v"(w));  // (waited for here)
     return w;
   };
-  float w = read_weight_scales(0);
+  lds_dma16(w_scale - begin + first_scale(lane), lds + scales + 1024);
   copy_scales(0);
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
@@ -103,6 +103,8 @@ __device__ __forceinline__ void tile(const onebit_block_product& p, const BlockG
   read_weight(0, 0);
   read_weight(0, 1);
   read_scales(0);
+  const int own = min(lane, count - 1);
+  float w = ((const float*)(smem + scales + 1024))[own / 4 * 4 + begin + own - first_scale(own / 4)];
   int stage = 0;
   for (int g = 0; g < count; ++g) {
     const int following = stage + 1 == STAGES ? 0 : stage + 1, leading = stage ? stage - 1 : STAGES - 1;
@@ -161,27 +163,52 @@ __device__ __forceinline__ void tile(const onebit_block_product& p, const BlockG
   wait_vmcnt<0>();  // none into what follows, nor into LDS that another workgroup has by then
   __syncthreads();
 
-  // Sixteen tokens at a time through LDS: a lane then has eight neighbouring rows of a token.
   const Result result(p, grid, split);
-  constexpr int kLanes = FM * 2, kPitch = FM * 16 + 4;  // lanes to a token, floats between tokens
-  float* const rows = (float*)smem + wave * 16 * kPitch;
-  static_assert(T::kWaves * 16 * kPitch * 4 <= T::kLds, "");
-  const int row = first_row + m * T::kRows + wave_m * FM * 16 + lane % kLanes * 8;
-  float bias[8];
-  result.load_bias(row, bias);
+  const int row = first_row + m * T::kRows + wave_m * FM * 16;
+  auto add_bias = [&](auto zero) {  // (all loads first)
+    typedef decltype(zero) T;
+    T bias[FM][4];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[i][e] = ((const T*)result.bias)[min(row + i * 16 + q * 4 + e, p.rows - 1)];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i][j][e] += (float)bias[i][e];
+  };
+  if (result.bias) {
+    if (p.bias_dtype == ONEBIT_DTYPE_F32) add_bias(0.f);
+    else if (p.bias_dtype == ONEBIT_DTYPE_F16) add_bias((_Float16)0.f);
+    else add_bias((__bf16)0.f);
+  }
+  // fp32 straight from the matrix instructions' registers; 16 bits through LDS, sixteen tokens at a time: neighbouring lanes then have neighbouring rows
+  if (result.type == ONEBIT_DTYPE_F32) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int token = n * T::kTokens + (wave_n * FN + j) * 16 + r;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        if (token < p.tokens) result.put_four(token, row + i * 16 + q * 4, sum[i][j]);
+    }
+    return;
+  }
+  constexpr int kLanes = FM * 2, kAtOnceTokens = 64 / kLanes, kPitch = FM * 32 + 16;  // lanes to a token, tokens of a store, bytes between tokens
+  static_assert(T::kWaves * 2 * 16 * kPitch <= T::kLds, "");
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
+    char* const rows = smem + (wave * 2 + j % 2) * 16 * kPitch;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) *(f4_t*)(rows + r * kPitch + i * 16 + q * 4) = sum[i][j];
+    for (int i = 0; i < FM; i += 2) *(u4_t*)(rows + r * kPitch + (i + q % 2) * 32 + q / 2 * 16) = result.eight_of(sum[i][j], sum[i + 1][j]);
     __builtin_amdgcn_wave_barrier();
-    const int first = n * T::kTokens + (wave_n * FN + j) * 16;
-#pragma unroll 1
-    for (int t = lane / kLanes; t < 16 && first + t < p.tokens; t += 64 / kLanes) {
-      const f4_t v0 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8), v1 = *(const f4_t*)(rows + t * kPitch + lane % kLanes * 8 + 4);
-      const float v[8] = {v0.x + bias[0], v0.y + bias[1], v0.z + bias[2], v0.w + bias[3], v1.x + bias[4], v1.y + bias[5], v1.z + bias[6], v1.w + bias[7]};
-      result.put(first + t, row, v);
+    const int token = (wave_n * FN + j) * 16 + lane / kLanes + n * T::kTokens;
+#pragma unroll
+    for (int t = 0; t < 16; t += kAtOnceTokens) {
+      const u4_t eight = *(const u4_t*)(rows + (lane / kLanes + t) * kPitch + lane % kLanes * 16);
+      if (token + t < p.tokens) result.put_eight(token + t, row + lane % kLanes * 8, eight);
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
