@@ -6,7 +6,7 @@
 // those that make up a share of the mass not below the value above which the groups' largest make it up alone; so that the filters
 // see a list of few candidates, from the few groups that reach that value, in the order of their indices. Where a list would not hold them they go over the row's groups instead.
 //
-// Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 10 to 12 us whatever the number of rows;
+// Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 8 to 9 us whatever the number of rows;
 // 64 rows of 4096, in one kernel, 5.6. A row of 131072 that keeps more candidates than a list holds takes one workgroup 85 to 250 us, for the arithmetic of its weights.
 #include "onebit_decoder_device.h"
 #include "onebit_head_launch.h"
@@ -389,49 +389,48 @@ __device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t
 #pragma unroll
   for (int i = 0; i < kCount; ++i) distance[i] = most[i] >= kLeast ? most[i] == scale.largest ? 0.f : (scale.top - value_of(most[i])) * steep : INFINITY;
   if (p.top_k != kAll || p.top_p < 1.f) {
-    // The groups' largest within `reach` are top_k, or have top_p of the mass: found by quarters, five times. In fp32, and therefore with some room. First with the
-    // threads' largest alone; where they do not come to it, with all.
+    // The groups' largest within `reach` are top_k, or have top_p of the mass: from a histogram of their distances, 256 bins for each doubling of an eighth and the distance. First with the
+    // threads' largest alone; where they do not come to it, with all. Masses in 2^-31 of the row's, cut off, and with some room.
     const bool by_rank = p.top_k != kAll;
-    const float target = by_rank ? (float)p.top_k : (float)((double)p.top_p * mass * 0x1p-42) * (1.f + 0x1p-10f);
-    constexpr int kWaves = Block<THREADS>::kWaves;
-    auto quarters = [&](auto number, const auto& distance) __attribute__((always_inline)) {
-      constexpr int kNumber = decltype(number)::value;
-      float amount[kNumber], low = 0.f;
-      bool enough = false;
-      reach = kFarthest;
-#pragma unroll
-      for (int i = 0; i < kNumber; ++i) amount[i] = by_rank ? 1.f : __builtin_amdgcn_exp2f(-distance[i]);
-#pragma unroll 1
-      for (int round = 0; round < 5; ++round) {
-        const float step = (reach - low) * 0.25f;
-        f4_t sum = {};
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (q < 3 || round == 0) {
-#pragma unroll
-            for (int i = 0; i < kNumber; ++i) sum[q] += distance[i] <= low + (q + 1) * step ? amount[i] : 0.f;
-            sum[q] = of_lane(wave_running(sum[q]), 63);
-          }
-        float* const parts = (float*)s.bins + (round & 1) * 4 * kWaves;
-        if (block.lane == 0) *(f4_t*)(parts + 4 * block.wave) = sum;
-        __syncthreads();
-        const f4_t all = *(const f4_t*)(parts + 4 * (block.lane % kWaves));
-        int within = 0;
-#pragma unroll
-        for (int q = 0; q < 3; ++q) within += of_lane(row_running(all[q]), kWaves - 1) < target;
-        if (round == 0) enough = of_lane(row_running(all[3]), kWaves - 1) >= target;
-        if (!enough) return false;
-        if (within < 3) reach = low + (within + 1) * step;
-        low += within * step;
-      }
-      return true;
+    const float unit = by_rank ? 1.f : (float)(0x1p73 / mass);
+    const mass_t target = by_rank ? (mass_t)p.top_k : (mass_t)((double)p.top_p * 0x1p31 * (1. + 0x1p-10)) + 1;
+    uint32_t* const bins = (uint32_t*)s.bins;
+    constexpr uint32_t kEighth = 0x3e000000u, kEdges = ((0x42488000u - kEighth) >> 15) + 1;  // (50 and an eighth)
+    constexpr int kEach = (kEdges + THREADS - 1) / THREADS;
+    static_assert(sizeof(s.bins) >= kEach * THREADS * sizeof(uint32_t), "");
+    auto add = [&](float d) {
+      if (d <= kFarthest) atomicAdd(&bins[(__float_as_uint(d + 0.125f) - kEighth) >> 15], by_rank ? 1u : (uint32_t)(__builtin_amdgcn_exp2f(-d) * unit));
     };
-    float nearest[1] = {distance[0]};
+    float nearest = distance[0];
 #pragma unroll
-    for (int i = 1; i < kCount; ++i) nearest[0] = fminf(nearest[0], distance[i]);
-    if (!quarters(std::integral_constant<int, 1>(), nearest)) {
-      __syncthreads();  // the sums' readers are through
-      if (kCount > 1 && !quarters(std::integral_constant<int, kCount>(), distance)) reach = kFarthest;
+    for (int i = 1; i < kCount; ++i) nearest = fminf(nearest, distance[i]);
+#pragma unroll 1
+    for (int pass = 0; pass < (kCount > 1 ? 2 : 1); ++pass) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) bins[threadIdx.x + i * THREADS] = 0;
+      __syncthreads();
+      if (pass == 0) {
+        add(nearest);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) add(distance[i]);
+      }
+      __syncthreads();
+      uint32_t own[kEach], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += own[i] = bins[threadIdx.x * kEach + i];
+      uint32_t front = block.before(sum, total);
+      if (total < target) continue;  // (for all threads; the bins have been read)
+      if (front < target && front + sum >= target) {
+        uint32_t bin = threadIdx.x * kEach;
+#pragma unroll
+        for (int i = 0; i < kEach - 1; ++i)
+          if ((front += own[i]) < target) ++bin;
+        s.bin = bin;
+      }
+      __syncthreads();
+      reach = __uint_as_float(((s.bin + 1) << 15) + kEighth) - 0.125f;
+      break;
     }
   }
   // (a step further than fp32 rounds)
