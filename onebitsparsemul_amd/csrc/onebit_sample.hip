@@ -151,8 +151,8 @@ struct Shared {
   uint32_t indices[kListed + 4];  // candidates in the order of their indices
   uint32_t reaching[kGroups / 2];            // groups that reach the candidates' value, 16 bits each
   mass_t parts[2][THREADS / 64];
-  mass_t above;
-  uint32_t bin;
+  mass_t above, few_amounts[64];
+  uint32_t bin, few, few_keys[64];  // a bin's items
 };
 
 // A workgroup of THREADS on a row
@@ -182,8 +182,9 @@ struct Block {
   }
 
   // The key, from `high` down to `low`, with which the running sum of the items' amounts comes to `target` or more, the sum in front of it, and whether it comes to it. each(f) calls
-  // f(key) for the thread's items; of key `extra` there is extra_amount once. In each round the bin of 2^shift keys in which that happens.
-  template <class Each, class Amount>
+  // f(key) for the thread's items; of key `extra` there is extra_amount once. In each round the bin of 2^shift keys in which that happens; LISTED: its items, where
+  // they are at most 64, are compared with each other (two rounds less: 500 of 131072 with top_p 22.6 us for 25.9; where a look at the items is long it does not pay).
+  template <bool LISTED, class Each, class Amount>
   __device__ __forceinline__ bool search(uint32_t high, uint32_t low, mass_t target, Each each, Amount amount, uint32_t extra, mass_t extra_amount, uint32_t& key, mass_t& in_front) {
     mass_t above = 0;
     for (;;) {
@@ -206,11 +207,36 @@ struct Block {
         if (front < target && front + own[i] >= target) s.bin = threadIdx.x * kEach + i, s.above = front;
         front += own[i];
       }
+      if (LISTED && threadIdx.x == 0) s.few = 0;
       __syncthreads();
       above = s.above;
       high -= s.bin << shift;
       low = max(low, high - ((1u << shift) - 1));
       if (shift == 0) break;
+      if (LISTED) {
+        auto take = [&](uint32_t own, mass_t amount) {
+          if (const uint32_t at = atomicAdd(&s.few, 1u); at < 64) s.few_keys[at] = own, s.few_amounts[at] = amount;
+        };
+        each([&](uint32_t own) {
+          if (own <= high && own >= low) take(own, amount(own));
+        });
+        if (threadIdx.x == 0 && extra_amount && extra <= high && extra >= low) take(extra, extra_amount);
+        __syncthreads();
+        const int few = __builtin_amdgcn_readfirstlane((int)s.few);
+        if (few <= 64) {
+          const uint32_t own_key = s.few_keys[lane];
+          mass_t larger = above, with = above;
+          for (int j = 0; j < few; ++j) {
+            const uint32_t other = s.few_keys[j];
+            const mass_t amount = s.few_amounts[j];
+            larger += other > own_key ? amount : 0;
+            with += other >= own_key ? amount : 0;
+          }
+          const int here = __builtin_ctzll(__ballot(lane < few && larger < target && with >= target));
+          high = (uint32_t)of_lane((int)own_key, here), above = of_lane(larger, here);
+          break;
+        }
+      }
     }
     key = high;
     in_front = above;
@@ -219,12 +245,12 @@ struct Block {
 };
 
 // The filters by rank and by share. each(f) calls f(key) for the thread's items, all of them from key `low` on, in any order; mass: the row's, where it counts.
-template <int THREADS, class Each>
+template <bool LISTED, int THREADS, class Each>
 __device__ __forceinline__ Kept filtered(Block<THREADS>& block, const Scale& scale, const Parameters& p, uint32_t low, double mass, Each each) {
   Kept kept = {kNothing, kAll};
   uint32_t key;
   mass_t in_front;
-  if (p.top_k != kAll && block.search(scale.largest, low, p.top_k, each, [](uint32_t) { return (mass_t)1; }, 0, 0, key, in_front)) kept = {key, p.top_k - (int)in_front};
+  if (p.top_k != kAll && block.template search<LISTED>(scale.largest, low, p.top_k, each, [](uint32_t) { return (mass_t)1; }, 0, 0, key, in_front)) kept = {key, p.top_k - (int)in_front};
   if (p.top_p < 1.f) {
     const mass_t tied = kept.ties == kAll ? 0 : scale.weight(kept.key) * kept.ties;
     auto above = [&](auto f) {
@@ -240,7 +266,7 @@ __device__ __forceinline__ Kept filtered(Block<THREADS>& block, const Scale& sca
     }
     // (where rounding leaves the running sum below: all stay)
     const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
-    if (block.search(scale.largest, max(low, kept.key), target, above, [&](uint32_t own) { return scale.weight(own); }, kept.key, tied, key, in_front)) {
+    if (block.template search<LISTED>(scale.largest, max(low, kept.key), target, above, [&](uint32_t own) { return scale.weight(own); }, kept.key, tied, key, in_front)) {
       const mass_t one = scale.weight(key);
       kept = {key, (int)((target - in_front + one - 1) / one)};
     }
@@ -341,11 +367,14 @@ __device__ __forceinline__ void choose(Block<THREADS>& block, const Last& last, 
 }
 
 // Few candidates: each is compared with each other, wavefronts taking every so manieth of them: how many are in front of it, and their mass
-constexpr int kPaired = 256;
+// (with 256 threads 100 take 13.7 us in this way and 12.5 in the other, with 512 150 11.5 and 12.0, with 1024 200 15.6 and 16.2)
+template <int THREADS>
+constexpr int kPaired = 64 + THREADS / 8;
 template <int THREADS>
 __device__ __forceinline__ void choose_of_few(Block<THREADS>& block, const Scale& scale, const Last& last, const Parameters& p, double mass, float uniform, int count, long long* token) {
   Shared<THREADS>& s = block.s;
-  mass_t *const weights = s.bins, *const fronts = s.bins + kPaired, *const ranks = s.bins + 2 * kPaired;
+  constexpr int kMost = kPaired<THREADS>;
+  mass_t *const weights = s.bins, *const fronts = s.bins + kMost, *const ranks = s.bins + 2 * kMost;
   const int own = threadIdx.x;
   if (own < count) weights[own] = scale.weight(s.keys[own]), fronts[own] = ranks[own] = 0;
   __syncthreads();
@@ -353,6 +382,7 @@ __device__ __forceinline__ void choose_of_few(Block<THREADS>& block, const Scale
     const uint32_t key = s.keys[i];
     mass_t front = 0;
     int rank = 0;
+#pragma unroll 4
     for (int j = block.wave; j < count; j += THREADS / 64) {
       const uint32_t other = s.keys[j];
       const bool better = other > key || (other == key && j < i);
@@ -390,7 +420,7 @@ __device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t
   for (int i = 0; i < kCount; ++i) distance[i] = most[i] >= kLeast ? most[i] == scale.largest ? 0.f : (scale.top - value_of(most[i])) * steep : INFINITY;
   if (p.top_k != kAll || p.top_p < 1.f) {
     // The groups' largest within `reach` are top_k, or have top_p of the mass: from a histogram of their distances, 256 bins for each doubling of an eighth and the distance. First with the
-    // threads' largest alone; where they do not come to it, with all. Masses in 2^-31 of the row's, cut off, and with some room.
+    // threads' largest alone; where they do not come to it, or would be most of them, with all (top_k 1000 and top_p 0.9 of 131072, 16 rows: 24.6 us, by the threads' largest 153). Masses in 2^-31 of the row's, cut off, and with some room.
     const bool by_rank = p.top_k != kAll;
     const float unit = by_rank ? 1.f : (float)(0x1p73 / mass);
     const mass_t target = by_rank ? (mass_t)p.top_k : (mass_t)((double)p.top_p * 0x1p31 * (1. + 0x1p-10)) + 1;
@@ -405,7 +435,7 @@ __device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t
 #pragma unroll
     for (int i = 1; i < kCount; ++i) nearest = fminf(nearest, distance[i]);
 #pragma unroll 1
-    for (int pass = 0; pass < (kCount > 1 ? 2 : 1); ++pass) {
+    for (int pass = kCount > 1 && by_rank && p.top_k > THREADS / 2; pass < (kCount > 1 ? 2 : 1); ++pass) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) bins[threadIdx.x + i * THREADS] = 0;
       __syncthreads();
@@ -497,10 +527,10 @@ __device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t
   }
   if (threadIdx.x < 4 && listed <= kListed) s.keys[listed + threadIdx.x] = kNothing;
   __syncthreads();
-  if (listed <= kPaired) {
+  if (listed <= kPaired<THREADS>) {
     choose_of_few(block, scale, last, p, mass, uniform, listed, token);
   } else if (listed <= kListed) {
-    const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
+    const Kept kept = filtered<true>(block, scale, p, low, mass, [&](auto f) {
       for (int i = threadIdx.x; i < listed; i += THREADS) f(s.keys[i]);
     });
     choose(block, last, kept, uniform, -1., (listed + 3) / 4, [&](int i) { return *(const u4_t*)(s.keys + 4 * i); }, [&](int i) { return (long long)s.indices[i]; }, token);
@@ -511,7 +541,7 @@ __device__ __forceinline__ void sample_row(Block<THREADS>& block, const uint32_t
       for (int e = 0; e < 4; ++e) one[e] = one[e] >= low ? one[e] : kNothing;
       return one;
     };
-    const Kept kept = filtered(block, scale, p, low, mass, [&](auto f) {
+    const Kept kept = filtered<false>(block, scale, p, low, mass, [&](auto f) {
       for (int i = threadIdx.x; i < fours; i += 2 * THREADS) {
         const u4_t one = reached(i), other = i + THREADS < fours ? reached(i + THREADS) : u4_t{kNothing, kNothing, kNothing, kNothing};
         each_of(one, other, f);
