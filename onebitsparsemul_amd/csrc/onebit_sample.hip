@@ -7,7 +7,7 @@
 // see a list of few candidates, from the few groups that reach that value, in the order of their indices. Where a list would not hold them they go over the row's groups instead.
 //
 // Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 8 to 9 us whatever the number of rows;
-// 64 rows of 4096, in one kernel, 5.6. A row of 131072 that keeps more candidates than a list holds takes one workgroup 85 to 250 us, for the arithmetic of its weights.
+// 64 rows of 4096, in one kernel, 5.6. A row of 131072 that keeps more candidates than a list holds takes one workgroup 85 to 200 us, for the arithmetic of its weights.
 #include "onebit_decoder_device.h"
 #include "onebit_head_launch.h"
 
@@ -181,9 +181,25 @@ struct Block {
     return running - x + (wave ? of_lane(parts, wave - 1) : 0);
   }
 
+  // The bin in which the running sum over the bins, `above` in front of them, comes to `target`, into s.bin, and the sum in front of it into s.above, for after the next barrier
+  __device__ __forceinline__ bool locate(mass_t target, mass_t above) {
+    constexpr int kEach = kBins / THREADS;
+    mass_t own[kEach], sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += own[i] = s.bins[threadIdx.x * kEach + i];
+    mass_t front = above + before(sum, total);
+    if (above + total < target) return false;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (front < target && front + own[i] >= target) s.bin = threadIdx.x * kEach + i, s.above = front;
+      front += own[i];
+    }
+    return true;
+  }
+
   // The key, from `high` down to `low`, with which the running sum of the items' amounts comes to `target` or more, the sum in front of it, and whether it comes to it. each(f) calls
   // f(key) for the thread's items; of key `extra` there is extra_amount once. In each round the bin of 2^shift keys in which that happens; LISTED: its items, where
-  // they are at most 64, are compared with each other (two rounds less: 500 of 131072 with top_p 22.6 us for 25.9; where a look at the items is long it does not pay).
+  // they are at most 64, are compared with each other (two rounds less: top_k 500 and top_p 0.9 of 719 candidates 6.1 us for 9.5).
   template <bool LISTED, class Each, class Amount>
   __device__ __forceinline__ bool search(uint32_t high, uint32_t low, mass_t target, Each each, Amount amount, uint32_t extra, mass_t extra_amount, uint32_t& key, mass_t& in_front) {
     mass_t above = 0;
@@ -196,17 +212,7 @@ struct Block {
       });
       if (threadIdx.x == 0 && extra_amount && extra <= high && extra >= low) atomicAdd(&s.bins[(high - extra) >> shift], extra_amount);
       __syncthreads();
-      constexpr int kEach = kBins / THREADS;
-      mass_t own[kEach], sum = 0, total;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) sum += own[i] = s.bins[threadIdx.x * kEach + i];
-      mass_t front = above + before(sum, total);
-      if (above + total < target) return false;  // (in the first round, and for all threads)
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        if (front < target && front + own[i] >= target) s.bin = threadIdx.x * kEach + i, s.above = front;
-        front += own[i];
-      }
+      if (!locate(target, above)) return false;  // (in the first round, and for all threads)
       if (LISTED && threadIdx.x == 0) s.few = 0;
       __syncthreads();
       above = s.above;
@@ -242,6 +248,45 @@ struct Block {
     in_front = above;
     return true;
   }
+
+  // The same of items that take long to look at: once for bins that are as wide as each other in logits, once for a list of that bin's, in which the rest is found. (A row of 131072 of
+  // which top_p keeps most: 200 us, with rounds over all of them 252.)
+  template <class Each, class Amount>
+  __device__ __forceinline__ bool search_many(uint32_t high, uint32_t low, mass_t target, Each each, Amount amount, uint32_t extra, mass_t extra_amount, uint32_t& key, mass_t& in_front) {
+    const float top = value_of(high), width = (kBins - 1) / (top - value_of(low));
+    auto place = [&](uint32_t own) { return (uint32_t)fminf((top - value_of(own)) * width, kBins - 1.f); };  // (NaN, of infinities: the last)
+    for (int i = threadIdx.x; i < kBins; i += THREADS) s.bins[i] = 0;
+    __syncthreads();
+    each([&](uint32_t own) {
+      if (own <= high && own >= low) atomicAdd(&s.bins[place(own)], amount(own));
+    });
+    if (threadIdx.x == 0 && extra_amount && extra <= high && extra >= low) atomicAdd(&s.bins[place(extra)], extra_amount);
+    __syncthreads();
+    if (!locate(target, 0)) return false;
+    if (threadIdx.x == 0) s.few = 0;
+    __syncthreads();
+    const uint32_t bin = s.bin;
+    const mass_t above = s.above;
+    each([&](uint32_t own) {
+      if (own <= high && own >= low && place(own) == bin)
+        if (const uint32_t at = atomicAdd(&s.few, 1u); at < kListed) s.keys[at] = own;
+    });
+    __syncthreads();
+    const int count = (int)s.few;
+    if (count > kListed) return search<false>(high, low, target, each, amount, extra, extra_amount, key, in_front);
+    auto each_listed = [&](auto f) {
+      for (int i = threadIdx.x; i < count; i += THREADS) f(s.keys[i]);
+    };
+    if (extra_amount && (extra > high || extra < low || place(extra) != bin)) extra_amount = 0;
+    search<true>(high, low, target - above, each_listed, amount, extra, extra_amount, key, in_front);
+    in_front += above;
+    return true;
+  }
+  template <bool LISTED, class Each, class Amount>
+  __device__ __forceinline__ bool search_any(uint32_t high, uint32_t low, mass_t target, Each each, Amount amount, uint32_t extra, mass_t extra_amount, uint32_t& key, mass_t& in_front) {
+    if constexpr (LISTED) return search<true>(high, low, target, each, amount, extra, extra_amount, key, in_front);
+    else return search_many(high, low, target, each, amount, extra, extra_amount, key, in_front);
+  }
 };
 
 // The filters by rank and by share. each(f) calls f(key) for the thread's items, all of them from key `low` on, in any order; mass: the row's, where it counts.
@@ -250,7 +295,7 @@ __device__ __forceinline__ Kept filtered(Block<THREADS>& block, const Scale& sca
   Kept kept = {kNothing, kAll};
   uint32_t key;
   mass_t in_front;
-  if (p.top_k != kAll && block.template search<LISTED>(scale.largest, low, p.top_k, each, [](uint32_t) { return (mass_t)1; }, 0, 0, key, in_front)) kept = {key, p.top_k - (int)in_front};
+  if (p.top_k != kAll && block.template search_any<LISTED>(scale.largest, low, p.top_k, each, [](uint32_t) { return (mass_t)1; }, 0, 0, key, in_front)) kept = {key, p.top_k - (int)in_front};
   if (p.top_p < 1.f) {
     const mass_t tied = kept.ties == kAll ? 0 : scale.weight(kept.key) * kept.ties;
     auto above = [&](auto f) {
@@ -266,7 +311,7 @@ __device__ __forceinline__ Kept filtered(Block<THREADS>& block, const Scale& sca
     }
     // (where rounding leaves the running sum below: all stay)
     const mass_t target = max((mass_t)ceil((double)p.top_p * mass), (mass_t)1);
-    if (block.template search<LISTED>(scale.largest, max(low, kept.key), target, above, [&](uint32_t own) { return scale.weight(own); }, kept.key, tied, key, in_front)) {
+    if (block.template search_any<LISTED>(scale.largest, max(low, kept.key), target, above, [&](uint32_t own) { return scale.weight(own); }, kept.key, tied, key, in_front)) {
       const mass_t one = scale.weight(key);
       kept = {key, (int)((target - in_front + one - 1) / one)};
     }
