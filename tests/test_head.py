@@ -388,6 +388,22 @@ def test_tokens_with_parameters_of_their_own(rows, vocabulary, dtype):
         check_tokens(logits, share(), temperature=share() + 0.5, top_p=share())
 
 
+@pytest.mark.parametrize("options", [dict(top_k=300), dict(top_k=700, top_p=0.9), dict(top_k=3000, top_p=0.5), dict(top_k=20000), dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.9995),
+                                     dict(top_p=0.99, min_p=0.001), dict(min_p=0.01), dict(top_p=0.9, temperature=1.5)], ids=str)
+@pytest.mark.parametrize("kind", ["spread", "flat", "two values", "steps", "ranks"])
+@pytest.mark.parametrize("vocabulary", [3000, 8000, 40001, 131072])
+def test_many_candidates(vocabulary, kind, options):
+    """Lists of some hundred, of thousands, and rows that keep more than a list holds; bins full of equal logits"""
+    g = generator(vocabulary)
+    rows = 4
+    ranks = torch.argsort(torch.rand((rows, vocabulary), generator=g), dim=1).float()
+    logits = {"spread": lambda: torch.randn((rows, vocabulary), generator=g) * 2.5, "flat": lambda: torch.randn((rows, vocabulary), generator=g) * 0.3,
+              "two values": lambda: (torch.rand((rows, vocabulary), generator=g) < 0.3).float() * 2, "steps": lambda: (torch.randn((rows, vocabulary), generator=g) * 8).round() / 4,
+              "ranks": lambda: 12 - torch.tensor([1.0, 1.2, 1.5, 0.8])[:, None] * torch.log(ranks + 1)}[kind]()
+    check_tokens(logits, torch.rand(rows, generator=g), **options)
+    check_tokens(logits.bfloat16(), torch.rand(rows, generator=g), **options)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_equal_logits_go_by_index(dtype):
     """All equal, and few values: borders that fall on whole masses, ties that a filter takes in part"""
