@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
     }
     if (p.top_p >= 1.f) {  // no filter: the chunk, then the token in it
       const float uniform = a.uniform[row];
-      const double at = uniform < 1.f ? (uniform > 0.f ? (double)uniform * mass : 0.) : mass;
+      const double at = uniform > 0.f ? (uniform < 1.f ? (double)uniform * mass : mass) : 0.;  // (NaN: 0)
       const mass_t beyond = front + own > at && own > 0. ? 1 : 0, any = own > 0. ? 1 : 0;
       // the first chunk beyond, or the last one with a mass
       const mass_t found = block.most(beyond ? (mass_t)1 << 40 | (mass_t)(kLongThreads - threadIdx.x) : any ? (mass_t)threadIdx.x + 1 : 0);

@@ -614,3 +614,15 @@ def test_two_graphs_of_one_call_keep_apart(count):
         torch.cuda.synchronize()
         for got, expected in zip([*results, eager], [*want, want[0]]):
             assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+# ---- rows of several chunks of 4096 logits without a filter
+
+
+@pytest.mark.parametrize("vocabulary", [700, 8193, 40000, 131072])
+def test_a_random_number_that_is_none_counts_as_0(vocabulary):
+    logits = random_logits(3, vocabulary, generator(vocabulary), torch.float32)
+    u = torch.tensor([math.nan, -1.0, 0.0])
+    for options in (dict(), dict(top_k=10), dict(top_p=0.9), dict(min_p=0.1)):
+        assert plain_tokens(logits, u, **options) == plain_tokens(logits, torch.zeros(3), **options)
+        check_tokens(logits, u, **options)
