@@ -773,16 +773,16 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
       const mass_t found = block.most(beyond ? (mass_t)1 << 40 | (mass_t)(kLongThreads - threadIdx.x) : any ? (mass_t)threadIdx.x + 1 : 0);
       const bool over = found >> 40;
       const int chunk = over ? kLongThreads - (int)(found & 0xffffffff) : (int)found - 1;
-      if ((int)threadIdx.x == chunk) ((double*)s.bins)[16] = over ? at - front : -1.;
+      // (of chunks whose sums are rounded, one may begin behind the number that the one in front of it does not come to: its first token)
+      if ((int)threadIdx.x == chunk) ((double*)s.bins)[16] = over ? fmax(at - front, 0.) : 0x1p62;
       __syncthreads();
-      double rest = ((double*)s.bins)[16];
+      const double rest = ((double*)s.bins)[16];
       const int begin = chunk * kChunk, count = min(kChunk, a.vocabulary - begin);
       // (a chunk whose weights all round to nothing beside the row's largest: its largest)
       if (scale.weight((uint32_t)(c.best[(long long)row * c.chunks + chunk] >> 32)) == 0) {
         if (threadIdx.x == 0) a.tokens[row] = 0xffffffffu - (uint32_t)c.best[(long long)row * c.chunks + chunk];
         return;
       }
-      if (rest < 0.) rest = 0x1p62;
       choose(block, Last(scale, p), {kNothing, kAll}, uniform, rest, (count + 3) / 4, [&](int i) { return four_at(begin + 4 * i); }, [&](int i) { return (long long)(begin + i); }, a.tokens + row);
       return;
     }

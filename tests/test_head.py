@@ -626,3 +626,19 @@ def test_a_random_number_that_is_none_counts_as_0(vocabulary):
     for options in (dict(), dict(top_k=10), dict(top_p=0.9), dict(min_p=0.1)):
         assert plain_tokens(logits, u, **options) == plain_tokens(logits, torch.zeros(3), **options)
         check_tokens(logits, u, **options)
+
+
+def test_a_number_between_two_chunks_sums():
+    """Three chunks' masses a, b, c in 2^-42, a = b + c, whole numbers below 2^53. uniform 0.5 of a + b + c = 2 a is a, which the first chunk's sum does not exceed: the token is the second chunk's
+    first. a + b is beyond 2^53 and lies between two doubles, of which the upper one is even: less b it is a + 1, which is where the second chunk seems to begin."""
+    chunk, least = 4096, -42 * math.log(2)  # a weight of 1
+    row = torch.full((1, 4 * chunk), -math.inf)
+    row[0, chunk + 100:chunk + 1600] = 0.0  # a = 1500 2^42
+    row[0, 2 * chunk + 100:2 * chunk + 1100], row[0, 2 * chunk + 1100:2 * chunk + 1103] = 0.0, least  # b = 1000 2^42 + 3
+    row[0, 3 * chunk + 100:3 * chunk + 599], row[0, 3 * chunk + 599] = 0.0, -3 * 2.0**-42  # c = 499 2^42 + (2^42 - 3): of e^-x the rest, x^2 / 2 2^42, is 2^-39.8
+    a, b = 1500 * 2**42, 1000 * 2**42 + 3
+    assert int(float(a + b)) - b == a + 1 and float(2 * a) == 2 * a
+    assert onebit.sample(row.cuda(), torch.tensor([0.5], device="cuda")).item() == 2 * chunk + 100
+    below, above = 0.5 - 2.0**-25, 0.5 + 2.0**-24
+    assert onebit.sample(row.cuda(), torch.tensor([below], device="cuda")).item() == chunk + 1599
+    assert onebit.sample(row.cuda(), torch.tensor([above], device="cuda")).item() == 2 * chunk + 100
