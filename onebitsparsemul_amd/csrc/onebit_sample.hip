@@ -752,9 +752,10 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
   double mass = 0.;
   if (p.masses) {
     // The chunks' masses in the row's unit, in their order: 64 bits of a float, rounded alike each time
+    // (one whose largest's weight rounds to 0 beside the row's has none)
     double own = 0.;
-    if ((int)threadIdx.x < c.chunks && (uint32_t)(own_best >> 32) >= kLeast)
-      own = (double)c.mass[(long long)row * c.chunks + threadIdx.x] * exp2(scale.distance(value_of((uint32_t)(own_best >> 32))));
+    const uint32_t own_key = (uint32_t)(own_best >> 32);
+    if (own_key >= kLeast && scale.weight(own_key) != 0) own = (double)c.mass[(long long)row * c.chunks + threadIdx.x] * exp2(scale.distance(value_of(own_key)));
     // (at most 256 chunks: four wavefronts)
     double* const sums = (double*)s.bins;
     const double running = wave_running(own);
@@ -767,7 +768,7 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
     }
     if (p.top_p >= 1.f) {  // no filter: the chunk, then the token in it
       const float uniform = a.uniform[row];
-      const double at = uniform > 0.f ? (uniform < 1.f ? (double)uniform * mass : mass) : 0.;  // (NaN: 0)
+      const double at = uniform > 0.f ? (uniform < 1.f ? (double)uniform * mass : INFINITY) : 0.;  // (NaN: 0)
       const mass_t beyond = front + own > at && own > 0. ? 1 : 0, any = own > 0. ? 1 : 0;
       // the first chunk beyond, or the last one with a mass
       const mass_t found = block.most(beyond ? (mass_t)1 << 40 | (mass_t)(kLongThreads - threadIdx.x) : any ? (mass_t)threadIdx.x + 1 : 0);
@@ -778,11 +779,6 @@ __global__ __launch_bounds__(kLongThreads) void sample_long_kernel(onebit_sampli
       __syncthreads();
       const double rest = ((double*)s.bins)[16];
       const int begin = chunk * kChunk, count = min(kChunk, a.vocabulary - begin);
-      // (a chunk whose weights all round to nothing beside the row's largest: its largest)
-      if (scale.weight((uint32_t)(c.best[(long long)row * c.chunks + chunk] >> 32)) == 0) {
-        if (threadIdx.x == 0) a.tokens[row] = 0xffffffffu - (uint32_t)c.best[(long long)row * c.chunks + chunk];
-        return;
-      }
       choose(block, Last(scale, p), {kNothing, kAll}, uniform, rest, (count + 3) / 4, [&](int i) { return four_at(begin + 4 * i); }, [&](int i) { return (long long)(begin + i); }, a.tokens + row);
       return;
     }

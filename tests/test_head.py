@@ -642,3 +642,22 @@ def test_a_number_between_two_chunks_sums():
     below, above = 0.5 - 2.0**-25, 0.5 + 2.0**-24
     assert onebit.sample(row.cuda(), torch.tensor([below], device="cuda")).item() == chunk + 1599
     assert onebit.sample(row.cuda(), torch.tensor([above], device="cuda")).item() == 2 * chunk + 100
+
+
+def test_chunks_whose_weights_are_all_0():
+    """-40 below the largest is e^-40 = 2^-57.7 of it: less than half of 2^-42, a weight of 0, so that the last token with a weight is the largest logit, whatever stands behind it"""
+    chunk = 4096
+    row = torch.full((5, 3 * chunk), -40.0)
+    row[:, 5] = 0.0
+    u = torch.tensor([1.0, 1.5, math.inf, 1 - 2.0**-24, 0.0])
+    assert onebit.sample(row.cuda(), u.cuda()).tolist() == [5] * 5
+    # at an infinite temperature all finite logits weigh the same, beside an infinite one nothing
+    row = torch.zeros((3, 3 * chunk))
+    u = torch.tensor([0.2, 0.7, 1.0])
+    assert onebit.sample(row.cuda(), u.cuda(), temperature=math.inf).tolist() == [math.floor(float(u[0]) * 3 * chunk), math.floor(float(u[1]) * 3 * chunk), 3 * chunk - 1]
+    row[:, 5] = row[:, 9000] = math.inf
+    for temperature in (1.0, math.inf):
+        assert onebit.sample(row.cuda(), u.cuda(), temperature=temperature).tolist() == [5, 9000, 9000]
+        # 0.6 of the mass takes both of the two, 0.4 the first
+        assert onebit.sample(row.cuda(), u.cuda(), temperature=temperature, top_p=0.6).tolist() == [5, 9000, 9000]
+        assert onebit.sample(row.cuda(), u.cuda(), temperature=temperature, top_p=0.4).tolist() == [5, 5, 5]
