@@ -28,6 +28,7 @@ def quantize_rows(x):
     return _binding().quantize_rows(x)
 
 
+@torch.no_grad()
 def quantize_weight(weight):
     """(codes, scales) of a weight (rows, columns), once: codes float8_e4m3fn (rows, columns rounded up to a multiple of 128), scales float32 (rows / 128 rounded
     up, columns / 128 rounded up), one for each 128 x 128 values, as by quantize_rows."""
@@ -67,7 +68,7 @@ class BlockLinear(torch.nn.Module):
         self.out_dtype = out_dtype
         self.register_buffer("codes", codes)
         self.register_buffer("scales", scales)
-        self.register_buffer("bias", bias)
+        self.register_buffer("bias", None if bias is None else bias.detach())
 
     def _apply(self, fn, recurse=True):
         # of a change of the module's type (half() and the like) codes and scales take the move alone

@@ -198,3 +198,17 @@ def test_the_binding_refuses():
     onebit.block_linear(codes, scales, w, ws, out=out)  # and goes on working
     torch.cuda.synchronize()
     assert bool((out == 0).all())
+
+
+def test_a_weight_that_is_learned_leaves_no_graph():
+    import copy
+    linear = torch.nn.Linear(200, 130)
+    layer, plain = onebit.BlockLinear(linear.weight, linear.bias), onebit.BlockLinear(linear.weight.detach().clone(), linear.bias.detach().clone())
+    for t in (*onebit.quantize_weight(linear.weight), *layer.buffers()):
+        assert not t.requires_grad and t.grad_fn is None
+    assert not list(layer.parameters()) and set(dict(layer.named_buffers())) == {"codes", "scales", "bias"}
+    for name, t in plain.named_buffers():
+        assert torch.equal(getattr(layer, name).float(), t.float())
+    other = copy.deepcopy(layer).half()
+    assert other.codes.dtype == torch.float8_e4m3fn and torch.equal(other.scales, layer.scales) and other.bias.dtype == torch.float16
+    assert linear.weight.requires_grad and linear.bias.requires_grad
