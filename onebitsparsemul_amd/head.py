@@ -39,11 +39,12 @@ def quantize_weight(weight):
     codes = torch.zeros((rows, groups * GROUP), dtype=torch.float8_e4m3fn, device=weight.device)
     scales = torch.empty((-(-rows // GROUP), groups), dtype=torch.float32, device=weight.device)
     step = 64 * GROUP  # what is held in 32 bits at a time
+    most = scales.new_full((), MOST)  # (by a Python number the GPU multiplies with its reciprocal, which is another scale half of the time)
     for first in range(0, rows, step):
         part = weight[first:first + step].float()
         count = part.shape[0]
         blocks = torch.nn.functional.pad(part, (0, groups * GROUP - columns, 0, -count % GROUP)).view(-1, GROUP, groups, GROUP)
-        scale = blocks.abs().amax((1, 3)) / MOST
+        scale = blocks.abs().amax((1, 3)) / most
         inside = ((scale > 0) & torch.isfinite(scale))[:, None, :, None]
         quotient = torch.where(inside, blocks / torch.where(inside, scale[:, None, :, None], 1.0), 0.0).clamp(-MOST, MOST)
         codes[first:first + count] = quotient.view(-1, groups * GROUP)[:count].to(torch.float8_e4m3fn)

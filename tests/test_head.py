@@ -661,3 +661,13 @@ def test_chunks_whose_weights_are_all_0():
         # 0.6 of the mass takes both of the two, 0.4 the first
         assert onebit.sample(row.cuda(), u.cuda(), temperature=temperature, top_p=0.6).tolist() == [5, 9000, 9000]
         assert onebit.sample(row.cuda(), u.cuda(), temperature=temperature, top_p=0.4).tolist() == [5, 5, 5]
+
+
+@pytest.mark.parametrize("rows,columns,dtype", [(1, 1, torch.float32), (130, 200, torch.float32), (1000, 1408, torch.bfloat16), (9000, 512, torch.float16)])
+def test_weights_as_codes_are_those_of_the_host(rows, columns, dtype):
+    """To the bit, and a weight of one row as quantize_rows has it"""
+    w = torch.randn((rows, columns), generator=generator(rows)).to(dtype)
+    for got, want in zip(onebit.quantize_weight(w.cuda()), onebit.quantize_weight(w)):
+        assert got.is_cuda and same(got, want)
+    for got, want in zip(onebit.quantize_weight(w[:1].cuda()), onebit.quantize_rows(w[:1].cuda())):
+        assert same(got, want)
