@@ -40,7 +40,7 @@ def quantize_weight(weight):
     scales = torch.empty((-(-rows // GROUP), groups), dtype=torch.float32, device=weight.device)
     step = 64 * GROUP  # what is held in 32 bits at a time
     most = scales.new_full((), MOST)  # (by a Python number the GPU multiplies with its reciprocal, which is another scale half of the time)
-    for first in range(0, rows, step):
+    for first in range(0, rows if columns else 0, step):
         part = weight[first:first + step].float()
         count = part.shape[0]
         blocks = torch.nn.functional.pad(part, (0, groups * GROUP - columns, 0, -count % GROUP)).view(-1, GROUP, groups, GROUP)

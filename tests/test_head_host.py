@@ -212,3 +212,10 @@ def test_a_weight_that_is_learned_leaves_no_graph():
     other = copy.deepcopy(layer).half()
     assert other.codes.dtype == torch.float8_e4m3fn and torch.equal(other.scales, layer.scales) and other.bias.dtype == torch.float16
     assert linear.weight.requires_grad and linear.bias.requires_grad
+
+
+@pytest.mark.parametrize("rows,columns", [(0, 0), (0, 200), (5, 0), (300, 0)])
+def test_weights_without_values(rows, columns):
+    codes, scales = onebit.quantize_weight(torch.zeros((rows, columns)))
+    assert codes.shape == (rows, -(-columns // 128) * 128) and codes.dtype == torch.float8_e4m3fn
+    assert scales.shape == (-(-rows // 128), -(-columns // 128)) and scales.dtype == torch.float32
