@@ -87,13 +87,15 @@ class Decoder:
     @torch.no_grad()
     def generate(self, prompt, uniform, **options):
         """prompt (sequences, length): ids; uniform (tokens, sequences): a random number in [0, 1) for each token and sequence; options: sample's. Returns the ids of
-        the tokens behind the prompt, (sequences, tokens); the caches hold the prompt and all but the last of them."""
+        the tokens behind the prompt, (sequences, tokens); the caches hold the prompt and all but the last of them. A sequence whose logits give no token (a NaN among
+        them) has -1 from there on, with id 0 in its caches."""
         count, new = uniform.shape[0], prompt.shape[1]
         ids, tokens = prompt.reshape(-1), []
         longest = int(self.lengths.max()) + new if count else 0
         for step in range(count):
-            tokens.append(sample(self.step(ids, new, longest), uniform[step], **options))
-            ids, new, longest = tokens[-1], 1, longest + 1
+            drawn = sample(self.step(ids, new, longest), uniform[step], **options)
+            tokens.append(torch.where(tokens[-1] < 0, -1, drawn) if tokens else drawn)
+            ids, new, longest = tokens[-1].clamp(min=0), 1, longest + 1
         return torch.stack(tokens, dim=1) if tokens else prompt.new_empty((prompt.shape[0], 0))
 
 

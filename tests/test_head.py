@@ -671,3 +671,13 @@ def test_weights_as_codes_are_those_of_the_host(rows, columns, dtype):
         assert got.is_cuda and same(got, want)
     for got, want in zip(onebit.quantize_weight(w[:1].cuda()), onebit.quantize_rows(w[:1].cuda())):
         assert same(got, want)
+
+
+def test_a_sequence_behind_a_nan_draws_nothing_any_more():
+    """A decoder without layers, whose logits come from the last id alone: an embedding with a NaN gives no token, and nothing is drawn from another id in its place"""
+    from onebitsparsemul_amd.decode import Decoder
+    decoder = Decoder(0, 3, 16, head="e4m3")
+    decoder.embedding[7, 5] = math.nan
+    prompt = torch.tensor([[7, 8], [8, 7], [9, 9]], device="cuda")
+    tokens = decoder.generate(prompt, torch.rand((4, 3), generator=generator(1)).cuda(), top_k=3)
+    assert bool((tokens[1] == -1).all()) and bool((tokens[[0, 2]] >= 0).all()) and bool((tokens[[0, 2]] != 7).all())

@@ -219,3 +219,25 @@ def test_weights_without_values(rows, columns):
     codes, scales = onebit.quantize_weight(torch.zeros((rows, columns)))
     assert codes.shape == (rows, -(-columns // 128) * 128) and codes.dtype == torch.float8_e4m3fn
     assert scales.shape == (-(-rows // 128), -(-columns // 128)) and scales.dtype == torch.float32
+
+
+def generating(monkeypatch, draws, length=64, caches=()):
+    """A decoder without layers on the host, whose draws are given, and the ids and bounds that its steps are called with"""
+    from onebitsparsemul_amd import decode
+    decoder, draws, calls = decode.Decoder.__new__(decode.Decoder), iter(draws), []
+    decoder.lengths, decoder.table, decoder.caches = torch.zeros(3, dtype=torch.int32), torch.zeros((length, 64)), list(caches)
+
+    def step(tokens, new, longest):
+        decoder.lengths += new
+        calls.append((tokens.tolist(), new, longest))
+    monkeypatch.setattr(decoder, "step", step)
+    monkeypatch.setattr(decode, "sample", lambda logits, uniform: torch.tensor(next(draws)))
+    return decoder, calls
+
+
+def test_a_sequence_without_a_token_gets_none_any_more(monkeypatch):
+    """-1 is no id: the rows that it stands for go on with id 0, and what they draw is not returned"""
+    decoder, calls = generating(monkeypatch, [[4, -1, 6], [5, 3, -1], [1, 2, 2]])
+    tokens = decoder.generate(torch.tensor([[1, 2], [3, 4], [5, 6]]), torch.zeros((3, 3)))
+    assert tokens.tolist() == [[4, 5, 1], [-1, -1, -1], [6, -1, -1]]
+    assert calls == [([1, 2, 3, 4, 5, 6], 2, 2), ([4, 0, 6], 1, 3), ([5, 0, 0], 1, 4)]
