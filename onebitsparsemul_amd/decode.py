@@ -92,6 +92,8 @@ class Decoder:
         count, new = uniform.shape[0], prompt.shape[1]
         ids, tokens = prompt.reshape(-1), []
         longest = int(self.lengths.max()) + new if count else 0
+        if longest + count - 1 > self.table.shape[0]:
+            raise ValueError(f"{count} tokens behind a length of {longest} need {longest + count - 1} places of a sequence, the decoder has {self.table.shape[0]}")
         for step in range(count):
             drawn = sample(self.step(ids, new, longest), uniform[step], **options)
             tokens.append(torch.where(tokens[-1] < 0, -1, drawn) if tokens else drawn)

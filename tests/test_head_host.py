@@ -241,3 +241,15 @@ def test_a_sequence_without_a_token_gets_none_any_more(monkeypatch):
     tokens = decoder.generate(torch.tensor([[1, 2], [3, 4], [5, 6]]), torch.zeros((3, 3)))
     assert tokens.tolist() == [[4, 5, 1], [-1, -1, -1], [6, -1, -1]]
     assert calls == [([1, 2, 3, 4, 5, 6], 2, 2), ([4, 0, 6], 1, 3), ([5, 0, 0], 1, 4)]
+
+
+def test_more_tokens_than_the_caches_hold_are_refused(monkeypatch):
+    """A prompt of two and four more, the last of which goes into no cache: five places"""
+    decoder, calls = generating(monkeypatch, [[1, 1, 1]] * 4, length=5)
+    assert decoder.generate(torch.zeros((3, 2), dtype=torch.int64), torch.zeros((4, 3))).shape == (3, 4) and len(calls) == 4
+    for lengths, count in ((0, 5), (1, 4), (5, 1)):
+        decoder, calls = generating(monkeypatch, [], length=5)
+        decoder.lengths += lengths
+        with pytest.raises(ValueError, match="places"):
+            decoder.generate(torch.zeros((3, 2), dtype=torch.int64), torch.zeros((count, 3)))
+        assert not calls and bool((decoder.lengths == lengths).all())
