@@ -98,7 +98,7 @@ class Decoder:
             drawn = sample(self.step(ids, new, longest), uniform[step], **options)
             tokens.append(torch.where(tokens[-1] < 0, -1, drawn) if tokens else drawn)
             ids, new, longest = tokens[-1].clamp(min=0), 1, longest + 1
-        return torch.stack(tokens, dim=1) if tokens else prompt.new_empty((prompt.shape[0], 0))
+        return torch.stack(tokens, dim=1) if tokens else prompt.new_empty((prompt.shape[0], 0), dtype=torch.int64)
 
 
 def main(argv=None):

@@ -253,3 +253,10 @@ def test_more_tokens_than_the_caches_hold_are_refused(monkeypatch):
         with pytest.raises(ValueError, match="places"):
             decoder.generate(torch.zeros((3, 2), dtype=torch.int64), torch.zeros((count, 3)))
         assert not calls and bool((decoder.lengths == lengths).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_no_tokens_are_ids_too(monkeypatch, dtype):
+    decoder, calls = generating(monkeypatch, [])
+    tokens = decoder.generate(torch.zeros((3, 2), dtype=dtype), torch.zeros((0, 3)))
+    assert tokens.shape == (3, 0) and tokens.dtype == torch.int64 and not calls
