@@ -681,3 +681,40 @@ def test_a_sequence_behind_a_nan_draws_nothing_any_more():
     prompt = torch.tensor([[7, 8], [8, 7], [9, 9]], device="cuda")
     tokens = decoder.generate(prompt, torch.rand((4, 3), generator=generator(1)).cuda(), top_k=3)
     assert bool((tokens[1] == -1).all()) and bool((tokens[[0, 2]] >= 0).all()) and bool((tokens[[0, 2]] != 7).all())
+
+
+@pytest.mark.parametrize("kind", ["positive", "outliers", "outlier in a group", "cancelling"])
+@pytest.mark.parametrize("tokens,rows,columns", [(300, 700, 4096), (64, 2304, 4096), (1000, 8192, 640), (600, 4099, 640)])
+def test_products_that_the_8_bit_instruction_cuts(tokens, rows, columns, kind):
+    """Seven products of eight neighbours lose less than 2^-13 of the largest of the eight each: the bound is 7 2^-13 of the sum of those largest ones, beside the roundings of the sums and the
+    result's own. A result that outliers cancel in is off by as much, whatever is left of it, and the mean of all errors by that bound's mean, beside the mean of as many roundings (six times
+    u / sqrt(3) of the results' root mean square, over the root of their number). fp32 results are cut nowhere."""
+    g = generator(columns + tokens)
+    x, w = (torch.randn((n, columns), generator=g, dtype=torch.float32).cuda() for n in (tokens, rows))
+    at = torch.arange(columns, device="cuda")
+    if kind == "positive":
+        x, w = x.abs() * 100, w.abs() * 100
+    elif kind == "cancelling":  # columns 3 and 11 of each group: 448 times the same weight, once less
+        x, w = torch.where((at % 128 == 3) | (at % 128 == 11), 448.0, x), w * 100
+        w[:, at % 128 == 11] = -w[:, at % 128 == 3]
+    else:
+        x, w = torch.where(at % (8 if kind == "outliers" else 128) == 3, x.sign() * 448, x), w * 100
+    x, w = (t.clamp(-448, 448).to(E4M3) for t in (x, w))
+    xs, ws = torch.full((tokens, columns // 128), 2.0**-8, device="cuda"), torch.full((-(-rows // 128), columns // 128), 2.0**-8, device="cuda")
+    xd, wd = x.double() * 2.0**-8, w.double() * 2.0**-8
+    want, size = xd @ wd.T.contiguous(), xd.abs() @ wd.abs().T.contiguous()
+    largest = torch.zeros_like(want)  # (products of two codes are exact in fp32)
+    for octet in range(0, columns, 8):
+        a, b = xd[:, octet:octet + 8].float().abs(), wd[:, octet:octet + 8].float().abs()
+        most = a[:, :1] * b[:, 0]
+        for i in range(1, 8):
+            most = torch.maximum(most, a[:, i:i + 1] * b[:, i])
+        largest += most
+    sums, cut = (130 + 3 * (columns // 128)) * 2.0**-23 * size, 7 * 2.0**-13 * largest
+    for dtype in DTYPES:
+        error = onebit.block_linear(x, xs, w, ws, out_dtype=dtype).double() - want
+        of_sums = sums + cut if dtype != torch.float32 else sums
+        bound = U[dtype] * (1 + 2.0**-10) * (want.abs() + of_sums) + of_sums + (2.0**-25 if dtype == torch.float16 else 0)
+        assert bool((error.abs() <= bound).all()), (dtype, float((error.abs() / bound).max()))
+        roundings = 6 * U[dtype] / math.sqrt(3) * float((want.norm() + of_sums.norm()) / want.numel())
+        assert abs(float(error.mean())) <= float(of_sums.mean()) + roundings
