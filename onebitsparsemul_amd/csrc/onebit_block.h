@@ -36,7 +36,7 @@ struct Operand<true> {
   }
 };
 
-// Eight values from any place on: rows of 4099 as fast as of 4096 (333 x 1408 -> 4099 9.4 us, by single values side by side 11.4)
+// Eight values from any place on: rows of 4099 as fast as of 4096
 template <int TYPE>
 __device__ inline void store_eight(void* base, long long at, const float (&x)[8]) {
   typedef typename Stored<TYPE>::type T;

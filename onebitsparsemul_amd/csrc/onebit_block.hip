@@ -1,7 +1,7 @@
 // The product of 8-bit codes with a scale for each 128 (onebit_head.h): few tokens, and which kernel takes a call.
 //
 // Codes go into the matrix instructions as fp16, exactly, whose products are exact and whose sums are fp32 (v_mfma_f32_16x16x32_f16: 9e-9 off over a group of 128
-// normal values; those of the 8-bit instructions cut the products of eight neighbours off at 2^-13 of the largest, 1.5e-5: they serve 16-bit results of many tokens). The sum of a group, from 0 on, times the
+// normal values; those of the 8-bit instructions cut the products of eight neighbours off at 2^-13 of the largest, 1.5e-5 over normal values: they serve 16-bit results of many tokens). The sum of a group, from 0 on, times the
 // product of the two scales is added to the sums in fp32. The weight is the matrix operand A, the tokens are B's columns: a lane then holds four neighbouring rows of y of
 // one token, so that its scale is one register, the weight's is the same for all lanes, and y is written in vectors.
 #include "onebit_block.h"
@@ -153,7 +153,8 @@ BlockGrid plan_block(const onebit_block_product& p, int compute_units) {
   const long long token_tiles = (p.tokens + 15) / 16;
   const double weight_bytes = (double)p.rows * p.columns;
   for (const Few& kind : few) {
-    // (eight wavefronts where each has more than four steps: one token on 11008 x 16384 38 us, with four 46; 8192 columns 18.2 and 19.1, 4096 10.6 and 10.2)
+    // (eight wavefronts where each has more than eight groups, four steps of two: one token on 11008 x 16384 38 us, with four 46. Up to there either is at most a tenth ahead: 11008 x 8192 18.2
+    // and 19.1, 11008 x 4096 10.6 and 10.2, sixteen tokens on 4096 x 4096 6.7 and 7.3.)
     if (kind.kernel == (groups > 64 ? kBlock16 : kBlock16Wide) || (kind.kernel == kBlock64 && token_tiles > 1 && tiles_may)) continue;
     const double blocks = (double)((p.rows + kind.rows - 1) / kind.rows) * token_tiles;
     const double through = 2.2 + std::max(weight_bytes / 4.9e6, (weight_bytes * token_tiles + blocks * std::min(p.tokens, 16) * p.columns) / 7e6);

@@ -1,9 +1,10 @@
 // The product of 8-bit codes for many tokens: tiles of both operands in LDS.
 //
-// Bound by the matrix instructions and the power that they draw, and by the copies' way through the caches: 4096 x 8192 x 8192 2.1 to 2.2 PFLOP/s, the same loop without its copies 2.6. Each product of
-// 16 x 16 x 128 takes the matrix unit 32 clocks, and its four values per lane four multiply-adds with the scales: two wavefronts to a SIMD hide them (34.4 clocks to a product,
-// with one wavefront 40), so that eight wavefronts have a tile; four with products of 128 x 128 each would read less from LDS, and spill. LDS is read without conflicts.
-// In fp16 the products run at 1.03 PFLOP/s. 2048 tokens x 4096 -> 11008 88 to 91 us; 333 x 1408 -> 4099 8.6 us.
+// Bound by the waits between the matrix instructions and by whole rounds of tiles: 2048 tokens x 4096 -> 11008 88 to 91 us, in which the matrix units are busy 45 % of the clocks (2.13 GHz), 4096 x 8192 -> 8192, two
+// rounds without a rest, 228 to 238 us = 2.3 to 2.4 PFLOP/s, busy 60 % of them (at 1.91 GHz: the clock falls with the load). Each product of
+// 16 x 16 x 128 takes the matrix unit 32 clocks, and its four values per lane four multiply-adds with the scales: two wavefronts to a SIMD hide them, so that eight wavefronts
+// have a tile; four with products of 128 x 128 each would read less from LDS, and spill. LDS is read without conflicts.
+// In fp16 (fp32 results) 2048 x 4096 -> 11008 198 to 201 us = 0.92 PFLOP/s, 4096 x 8192 -> 8192 490 us = 1.12, busy 40 and 50 %. 333 x 1408 -> 4099 8.6 us, 128 x 4096 -> 11008 17.0.
 #include "onebit_block.h"
 #include "onebit_device.h"
 

@@ -1,5 +1,5 @@
 // Rows of values as 8-bit codes with a scale for each 128 (onebit_head.h). Each value is moved once: bound by memory, small calls by the launch. 4001 x 5000 of 16 bits 13.5 us for
-// 61 MB = 4.5 TB/s, 16 x 11008 2.3.
+// 61 MB = 4.5 TB/s, 16 x 11008 2.3. Rows that do not begin at whole vectors go by single values: 4001 x 5001 28.0 us, 2.2 TB/s, 16 x 5001 2.7 (16 x 5000 2.3).
 #include "onebit_codes.h"
 #include "onebit_head_launch.h"
 

@@ -12,8 +12,9 @@ hipError_t launch_quantize_rows(const void* x, int dtype, long long x_stride, in
 enum BlockKernel { kBlock16, kBlock16Wide, kBlock64, kBlock128x32, kBlock64x64, kBlock128x64, kBlock256x128, kBlock256x256, kBlockMixed };
 // (rows of the weight, wide: on eight wavefronts; rows x tokens; mixed: the last two)
 constexpr int kLeastTileGroups = 4;  // of a tile's split
-// Tiles for 16-bit results of many tokens take the 8-bit matrix instruction, twice as fast. It cuts the products of eight neighbouring columns off at 2^-13 of the largest: 1.5e-5
-// off over normal values, a fourteenth of an fp16 result's own rounding. The others take the products in fp16.
+// Tiles for 16-bit results of many tokens take the 8-bit matrix instruction, twice as fast. It cuts the products of eight neighbouring columns off at 2^-13 of the largest: over 4096
+// columns 1.5e-5 of the result's norm for normal values, 6.3e-5 with one column of eight hundreds of times the others, where an fp16 result's own rounding is 2.1e-4. (At most 7 2^-13
+// of the sum of those largest: more than the rounding where they cancel.) The others take the products in fp16.
 inline bool narrow_products(const onebit_block_product& p) { return p.y_dtype != ONEBIT_DTYPE_F32 && p.tokens > 16; }
 struct BlockGrid {
   int tiles_n;  // of tokens, filled by the launcher

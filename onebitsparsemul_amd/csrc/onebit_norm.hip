@@ -1,6 +1,7 @@
 // The norms around a block (onebit_decoder.h): one workgroup for each row, the row in registers from its one read to its one write.
 // Bound by memory: 2048 x 8192, norm on both sides, residuals in fp32, 39.2 us for 201 MB = 5.1 TB/s, as a large copy. Small calls by the launch and one round
 // of loads, so every operand of a row is requested before the first is used: 16 x 4096 3.3 us. Codes instead of y: 41.4 us for 185 MB = 4.5 TB/s, and 3.8.
+// Rows that do not begin at whole vectors go by single values: 2048 x 5001 of fp16 52 us, as codes 47 (2048 x 5000: 15.7 and 19.2).
 #include "onebit_codes.h"
 #include "onebit_decoder_launch.h"
 

@@ -6,9 +6,9 @@
 // those that make up a share of the mass not below the value above which the groups' largest make it up alone; so that the filters
 // see a list of few candidates, from the few groups that reach that value, in the order of their indices. Where a list would not hold them they go over the row's groups instead.
 //
-// Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 8 to 9 us whatever the number of rows;
-// 64 rows of 4096, in one kernel, 5.6. Rows with some hundred candidates take 6 to 10 us more, and one of 131072 that keeps more than a list holds 85 to 200, for the arithmetic of its weights in one
-// workgroup.
+// Many rows are bound by the one pass over the logits (256 x 131072 fp32: 25 us, 5.3 TB/s), few by the second kernel's chain of steps over barriers, 8 to 10 us whatever the number of rows;
+// 64 rows of 4096, in one kernel, 5.6. Rows with some hundred candidates take 6 to 10 us more, and one that keeps more than a list holds 86 to 207 of 131072 logits (256 such rows 123 to 271) and 35 to 74 of 32000, for the
+// arithmetic of its weights in one workgroup.
 #include "onebit_decoder_device.h"
 #include "onebit_head_launch.h"
 
